@@ -1,0 +1,427 @@
+"""Timed cases of the operators around the experts of a mixture-of-experts layer and of the NVFP4 linear with its
+epilogue: each case in a plain form (elementary torch operations, 32-bit arithmetic, one rounding at the end) and, with
+``own`` set, through the library's entry points.
+
+linear_fused    y = residual + act(x W^T / divisor + bias), W packed NVFP4; with a gated activation ("silu_mul") the
+                first half of W's rows are the gate and the second half the up projection
+linear_grouped  the same product for rows sorted by expert, each expert its own W (and bias)
+expert_sort     every token's row copied to its experts' places, in expert order; its gradient adds them up again
+expert_return   every token's expert rows weighted and summed, with the residual; gradients to rows and weights
+"""
+
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+_TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+_BYTES = {"bf16": 2, "f16": 2, "f32": 4}
+_E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def listed():
+    return [
+        # The output projection of a 2048-wide layer for one token, back onto the residual stream.
+        {"name": "linear_one_token", "op": "linear", "tokens": 1, "cols": 2048, "rows": 2048, "type": "bf16",
+         "bias": True, "act": "none", "residual": True},
+        # The LM head for one token: 248,320 x 2,048, the largest weight stream.
+        {"name": "linear_lm_head", "op": "linear", "tokens": 1, "cols": 2048, "rows": 248320, "type": "bf16",
+         "bias": False, "act": "none", "residual": False},
+        # A ragged projection of an FP32 caller: odd rows, columns that end inside a tile.
+        {"name": "linear_f32_ragged", "op": "linear", "tokens": 301, "cols": 1008, "rows": 1003, "type": "f32",
+         "bias": True, "act": "gelu_tanh", "residual": True},
+        # Gate and up projection of a dense MLP over a 4096-token prompt.
+        {"name": "linear_prompt_gated", "op": "linear", "tokens": 4096, "cols": 2048, "rows": 8192, "type": "bf16",
+         "bias": False, "act": "silu_mul", "residual": False},
+        # Gate and up products of the eight experts of one token.
+        {"name": "grouped_one_token", "op": "grouped", "tokens": 1, "topk": 8, "experts": 256, "cols": 2048,
+         "rows": 1024, "type": "bf16", "bias": False, "act": "silu_mul", "skew": False, "drop": False},
+        # The same for a decode batch of 32 tokens: about 164 experts, one or two rows each.
+        {"name": "grouped_batch_32", "op": "grouped", "tokens": 32, "topk": 8, "experts": 256, "cols": 2048,
+         "rows": 1024, "type": "bf16", "bias": False, "act": "silu_mul", "skew": False, "drop": False},
+        # The same over a 4096-token prompt: about 128 rows an expert.
+        {"name": "grouped_prompt", "op": "grouped", "tokens": 4096, "topk": 8, "experts": 256, "cols": 2048,
+         "rows": 1024, "type": "bf16", "bias": False, "act": "silu_mul", "skew": False, "drop": False},
+        # Down products with biases under skewed routing, some picks dropped by a capacity limit.
+        {"name": "grouped_down_skewed", "op": "grouped", "tokens": 1501, "topk": 6, "experts": 64, "cols": 512,
+         "rows": 2048, "type": "f16", "bias": True, "act": "none", "skew": True, "drop": True},
+        # One token's row to its eight experts.
+        {"name": "sort_one_token", "op": "sort", "tokens": 1, "topk": 8, "experts": 256, "hidden": 2048,
+         "type": "bf16", "skew": False, "drop": False, "grad": False},
+        # A training step's rows to their experts, and their gradient back.
+        {"name": "sort_prompt_grad", "op": "sort", "tokens": 4096, "topk": 8, "experts": 256, "hidden": 2048,
+         "type": "bf16", "skew": True, "drop": False, "grad": True},
+        # A decode batch's expert rows back to their tokens.
+        {"name": "return_batch_32", "op": "return", "tokens": 32, "topk": 8, "experts": 256, "hidden": 2048,
+         "type": "bf16", "skew": False, "drop": False, "residual": True, "grad": False},
+        # A training step's expert rows back, with the gradients of rows and routing weights; FP32, odd sizes, drops.
+        {"name": "return_prompt_grad", "op": "return", "tokens": 2999, "topk": 6, "experts": 64, "hidden": 2052,
+         "type": "f32", "skew": True, "drop": True, "residual": True, "grad": True},
+    ]
+
+
+def _spread(rng, low, high):
+    """A whole number of [low, high], even over its logarithm."""
+    return max(low, min(high, int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))))
+
+
+def draw(rng):
+    op = rng.choice(["linear", "grouped", "sort", "return"])
+    kind = rng.choice(["bf16", "bf16", "f16", "f32"])
+    if op == "linear":
+        act = rng.choice(["none", "none", "relu", "silu", "gelu", "gelu_tanh", "silu_mul", "gelu_tanh_mul"])
+        tokens = _spread(rng, 1, 4096)
+        cols = 16 * _spread(rng, 4, 512)
+        most = min(32768, (1 << 35) // (tokens * cols))
+        rows = _spread(rng, 16, max(17, most))
+        return {"op": op, "tokens": tokens, "cols": cols, "rows": rows + rows % 2 * act.endswith("_mul"),
+                "type": kind, "bias": rng.random() < 0.5, "act": act, "residual": rng.random() < 0.5}
+    tokens = _spread(rng, 1, 4096)
+    topk = rng.choice([1, 2, 4, 6, 8])
+    experts = rng.choice([8, 16, 40, 64, 128, 160, 256])
+    skew, drop = rng.random() < 0.5, rng.random() < 0.3
+    case = {"op": op, "tokens": tokens, "topk": topk, "experts": experts, "type": kind, "skew": skew, "drop": drop}
+    if op == "grouped":
+        cols = 16 * _spread(rng, 8, 128)
+        rows = 2 * _spread(rng, 32, 512)
+        act = rng.choice(["none", "silu", "silu_mul", "gelu_tanh_mul"])
+        return {**case, "cols": cols, "rows": rows, "bias": rng.random() < 0.4, "act": act}
+    hidden = rng.choice([1, 8]) * _spread(rng, 64, 256)
+    case = {**case, "hidden": hidden, "grad": rng.random() < 0.5}
+    return {**case, "residual": rng.random() < 0.5} if op == "return" else case
+
+
+# ------------------------------------------------------------------ inputs
+
+
+def _weights(gen, groups, rows, cols):
+    """Packed NVFP4 weights of N(0, 0.02): codes [groups, rows, cols/2] (low nibble = even column), E4M3 scale bytes
+    [groups, rows, cols/16] and the divisor of each group."""
+    w = torch.randn(groups, rows, cols // 16, 16, generator=gen, device="cuda") * 0.02
+    unit = w.abs().amax(dim=(1, 2, 3)) / (6.0 * 448.0)
+    scale = (w.abs().amax(dim=3) / 6.0 / unit[:, None, None]).to(torch.float8_e4m3fn)
+    step = (scale.to(torch.float32) * unit[:, None, None]).clamp(min=1e-30)
+    edges = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], device="cuda")
+    code = torch.bucketize((w / step[..., None]).abs_(), edges, out_int32=True).to(torch.uint8)
+    code |= (w < 0).to(torch.uint8) << 3
+    code = code.reshape(groups, rows, cols // 2, 2)
+    return (code[..., 0] | (code[..., 1] << 4)).contiguous(), scale.view(torch.uint8).contiguous(), 1.0 / unit
+
+
+def _routing(gen, case):
+    """Distinct expert ids [tokens, topk] by descending logit, -1 where a pick is dropped, and the renormalised
+    softmax of their logits."""
+    logits = torch.randn(case["tokens"], case["experts"], generator=gen, device="cuda")
+    if case["skew"]:
+        rank = torch.randperm(case["experts"], generator=gen, device="cuda") + 1
+        logits = logits - 0.5 * torch.log(rank.to(torch.float32))
+    top, ids = torch.topk(logits, case["topk"], dim=1)
+    if case["drop"]:
+        ids = torch.where(torch.rand(ids.shape, generator=gen, device="cuda") < 0.1, -1, ids)
+    return ids.to(torch.int32), torch.softmax(top, dim=1)
+
+
+_runtime = None
+
+
+def _library():
+    global _runtime
+    if _runtime is None:
+        import os
+        import sys
+
+        sys.path.append(os.path.join(os.getcwd(), "x2-nvfp4-lab_b200"))
+        from vllm_nvfp4_cuda.runtime import Runtime
+
+        _runtime = Runtime()
+    return _runtime
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seed * 7919 + 13)
+    t = _TYPES[case["type"]]
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=gen, device="cuda").to(t)
+
+    s = {**case}
+    if case["op"] in ("linear", "grouped"):
+        groups = case.get("experts", 1)
+        rows, cols = case["rows"], case["cols"]
+        s["packed"], s["scales"], s["divisors"] = _weights(gen, groups, rows, cols)
+        width = rows // 2 if case["act"].endswith("_mul") else rows
+        count = case["tokens"]
+        if case["op"] == "grouped":
+            ids, _ = _routing(gen, case)
+            keys = torch.where(ids < 0, groups, ids).reshape(-1).long().sort().values
+            s["offsets"] = torch.searchsorted(keys, torch.arange(groups + 1, device="cuda")).to(torch.int32)
+            s["longest"] = int((s["offsets"][1:] - s["offsets"][:-1]).max())
+            count = keys.numel()
+            s["bias_rows"] = normal(groups, rows) * 0.1 if case["bias"] else None
+        else:
+            s["bias_rows"] = normal(rows) * 0.1 if case["bias"] else None
+        s["x"] = normal(count, cols)
+        s["residual_rows"] = normal(count, width) if case.get("residual") else None
+        # The weights as the program keeps them: uploaded once.
+        s["matrix"] = _library().upload_grouped(s["packed"], s["scales"], s["divisors"]) if own else None
+        return s
+    s["ids"], s["weights"] = _routing(gen, case)
+    if case["op"] == "sort":
+        s["x"] = normal(case["tokens"], case["hidden"])
+        s["x"].requires_grad_(case["grad"])
+        s["g"] = normal(case["tokens"] * case["topk"], case["hidden"]) if case["grad"] else None
+        return s
+    s["rows"] = normal(case["tokens"] * case["topk"], case["hidden"])
+    s["res"] = normal(case["tokens"], case["hidden"]) if case["residual"] else None
+    s["g"] = normal(case["tokens"], case["hidden"]) if case["grad"] else None
+    s["rows"].requires_grad_(case["grad"])
+    s["weights"].requires_grad_(case["grad"])
+    # The order of the rows, kept from the sort that brought them there.
+    s["order"] = None
+    if own:
+        s["order"] = _library().expert_sort(normal(case["tokens"], 8), s["ids"], case["experts"])[1]
+    else:
+        _, s["inverse"], _ = _order(s["ids"], case["experts"])
+    return s
+
+
+# ------------------------------------------------------------------ plain forms
+
+
+def _dequantise(s):
+    """FP32 weights [groups, rows, cols], the divisor left to the product."""
+    packed, table = s["packed"], torch.tensor(_E2M1, device="cuda")
+    code = torch.stack((packed & 15, packed >> 4), dim=-1).flatten(-2).to(torch.int32)
+    value = table[code & 7] * (1.0 - 2.0 * (code >> 3))
+    scale = s["scales"].view(torch.float8_e4m3fn).to(torch.float32)
+    return (value.unflatten(-1, (-1, 16)) * scale[..., None]).flatten(-2)
+
+
+def _activate(z, act):
+    base = act[:-4] if act.endswith("_mul") else act
+    up = None
+    if act.endswith("_mul"):
+        half = z.shape[-1] // 2
+        z, up = z[..., :half], z[..., half:]
+    if base == "relu":
+        z = torch.where(z < 0, torch.zeros_like(z), z)
+    elif base == "silu":
+        z = z / (1.0 + torch.exp(-z))
+    elif base == "gelu":
+        z = 0.5 * z * (1.0 + torch.erf(z * math.sqrt(0.5)))
+    elif base == "gelu_tanh":
+        z = z / (1.0 + torch.exp(-2.0 * math.sqrt(2.0 / math.pi) * (z + 0.044715 * z * z * z)))
+    return z if up is None else z * up
+
+
+def _linear(s):
+    z = s["x"].float() @ _dequantise(s)[0].t() / s["divisors"]
+    if s["bias_rows"] is not None:
+        z = z + s["bias_rows"].float()
+    z = _activate(z, s["act"])
+    if s["residual_rows"] is not None:
+        z = z + s["residual_rows"].float()
+    return z.to(s["x"].dtype)
+
+
+def _grouped(s):
+    """Every expert's rows padded to the longest: one batched product. Rows past the last expert's are zero."""
+    x, offsets = s["x"], s["offsets"].long()
+    at = offsets[:-1, None] + torch.arange(s["longest"], device="cuda")
+    inside = at < offsets[1:, None]
+    z = torch.bmm(x.float()[torch.where(inside, at, 0)], _dequantise(s).transpose(1, 2)) / s["divisors"][:, None, None]
+    if s["bias_rows"] is not None:
+        z = z + s["bias_rows"].float()[:, None]
+    z = _activate(z, s["act"])
+    out = torch.zeros(x.shape[0] + 1, z.shape[2], dtype=torch.float32, device="cuda")
+    out[torch.where(inside, at, x.shape[0])] = z
+    return out[:-1].to(x.dtype)
+
+
+def _order(ids, experts):
+    """perm (the flat pick of each row, -1 past the last expert's rows), inverse (the row of each pick, -1 where it
+    has none) and offsets (the first row of each expert, and the end)."""
+    flat = ids.reshape(-1).long()
+    key = torch.where((flat >= 0) & (flat < experts), flat, experts)
+    key_sorted, perm = torch.sort(key, stable=True)
+    inverse = torch.empty_like(perm)
+    inverse[perm] = torch.arange(perm.numel(), device="cuda")
+    inverse = torch.where(key < experts, inverse, -1).reshape(ids.shape)
+    perm = torch.where(key_sorted < experts, perm, -1)
+    offsets = torch.searchsorted(key_sorted, torch.arange(experts + 1, device="cuda"))
+    return perm.to(torch.int32), inverse.to(torch.int32), offsets.to(torch.int32)
+
+
+def _sort(s):
+    x = s["x"].detach()
+    perm, inverse, offsets = _order(s["ids"], s["experts"])
+    at = perm.long()
+    rows = torch.where(at[:, None] >= 0, x[torch.where(at < 0, 0, at) // s["topk"]], torch.zeros((), dtype=x.dtype, device="cuda"))
+    out = {"rows": rows, "perm": perm, "inverse": inverse, "offsets": offsets}
+    if s["grad"]:
+        taken = s["g"].float()[torch.where(inverse < 0, 0, inverse).long()]
+        out["dx"] = torch.where(inverse[..., None] >= 0, taken, 0.0).sum(1).to(x.dtype)
+    return out
+
+
+def _return(s):
+    rows, weights, inverse = s["rows"].detach(), s["weights"].detach(), s["inverse"]
+    has = inverse[..., None] >= 0
+    taken = torch.where(has, rows.float()[torch.where(inverse < 0, 0, inverse).long()], 0.0)
+    z = (weights[..., None] * taken).sum(1)
+    if s["res"] is not None:
+        z = z + s["res"].float()
+    out = {"out": z.to(rows.dtype)}
+    if s["grad"]:
+        g = s["g"].float()[:, None]
+        out["dweights"] = (g * taken).sum(2)
+        drows = torch.zeros(rows.shape[0] + 1, rows.shape[1], device="cuda")
+        drows[torch.where(inverse < 0, rows.shape[0], inverse).long()] = weights[..., None] * g
+        out["drows"] = drows[:-1].to(rows.dtype)
+    return out
+
+
+# ------------------------------------------------------------------ one pass
+
+
+def run(s):
+    if own:
+        return _own(s)
+    return {"linear": _linear, "grouped": _grouped, "sort": _sort, "return": _return}[s["op"]](s)
+
+
+def _own(s):
+    rt = _runtime
+    act = None if s.get("act") == "none" else s.get("act")
+    if s["op"] == "linear":
+        return rt.linear_fused(s["matrix"], s["x"], bias=s["bias_rows"], activation=act, residual=s["residual_rows"])
+    if s["op"] == "grouped":
+        return rt.linear_grouped(s["matrix"], s["x"], s["offsets"], bias=s["bias_rows"], activation=act)
+    if s["op"] == "sort":
+        rows, order = rt.expert_sort(s["x"], s["ids"], s["experts"])
+        out = {"rows": rows, "perm": order.perm, "inverse": order.inverse, "offsets": order.offsets}
+        if s["grad"]:
+            (out["dx"],) = torch.autograd.grad(rows, s["x"], s["g"])
+        return out
+    y = rt.expert_return(s["rows"], s["order"], s["weights"], residual=s["res"])
+    out = {"out": y}
+    if s["grad"]:
+        out["drows"], out["dweights"] = torch.autograd.grad(y, (s["rows"], s["weights"]), s["g"])
+    return out
+
+
+# ------------------------------------------------------------------ the work of one pass
+
+
+def work(case):
+    e = _BYTES[case["type"]]
+    if case["op"] in ("linear", "grouped"):
+        rows, cols = case["rows"], case["cols"]
+        width = rows // 2 if case["act"].endswith("_mul") else rows
+        picks = case["tokens"] * case.get("topk", 1)
+        groups = 1.0
+        if case["op"] == "grouped":  # the experts that a batch of that many tokens is expected to reach
+            n = case["experts"]
+            groups = n * (1.0 - (1.0 - case["topk"] / n) ** case["tokens"])
+        moved = groups * rows * cols * 9 / 16 + picks * (cols + width * (2 if case.get("residual") else 1)) * e
+        return {"bytes": moved + (groups * rows * e if case["bias"] else 0), "flops": 2.0 * picks * rows * cols}
+    tokens, picks, hidden = case["tokens"], case["tokens"] * case["topk"], case["hidden"]
+    if case["op"] == "sort":
+        once = (tokens + picks) * hidden * e
+        return {"bytes": once * (2 if case["grad"] else 1) + 12 * picks + 4 * case["experts"],
+                "flops": picks * hidden * (1.0 if case["grad"] else 0.0)}
+    forward = (picks + tokens * (2 if case["residual"] else 1)) * hidden * e + 8 * picks
+    back = (2 * picks + tokens) * hidden * e + 12 * picks
+    return {"bytes": forward + (back if case["grad"] else 0),
+            "flops": picks * hidden * (5.0 if case["grad"] else 2.0)}
+
+
+# ------------------------------------------------------------------ the definition in 64 bits
+
+
+def _exact_scales(b):
+    """E4M3 from its bits: 2^(e-7) (1 + m/8), or m/512 where e is 0."""
+    e, m = (b >> 3) & 15, (b & 7).double()
+    return torch.where(e == 0, m / 512.0, torch.ldexp(1.0 + m / 8.0, e - 7))
+
+
+def _exact_product(x, packed, scales, divisor):
+    """Rows of x times one group's weights: even and odd columns apart, each in 64 bits."""
+    table = torch.tensor(_E2M1 + tuple(-v for v in _E2M1), dtype=torch.float64, device="cuda")
+    scale = _exact_scales(scales.int()).repeat_interleave(8, dim=1)
+    x = x.detach().double()
+    low = x[:, 0::2] @ (table[(packed & 15).int()] * scale).T
+    high = x[:, 1::2] @ (table[(packed >> 4).int()] * scale).T
+    return (low + high) / divisor.double()
+
+
+def _exact_epilogue(z, bias, act, residual):
+    z = z if bias is None else z + bias.double()
+    name, gated = (act[:-4], True) if act.endswith("_mul") else (act, False)
+    gate, up = z.chunk(2, dim=1) if gated else (z, None)
+    if name == "relu":
+        gate = gate.clamp(min=0)
+    elif name == "silu":
+        gate = gate * torch.sigmoid(gate)
+    elif name == "gelu":
+        gate = gate * torch.special.ndtr(gate)
+    elif name == "gelu_tanh":
+        gate = gate * 0.5 * (1 + torch.tanh(math.sqrt(2 / math.pi) * (gate + 0.044715 * gate ** 3)))
+    z = gate * up if gated else gate
+    return z if residual is None else z + residual.double()
+
+
+def exact(case, seed):
+    global own
+    was, own = own, False
+    s = prepare(case, seed)
+    own = was
+    if case["op"] == "linear":
+        step = 16384 * 2048 // case["cols"] + 1
+        z = torch.cat([_exact_product(s["x"], s["packed"][0, i:i + step], s["scales"][0, i:i + step], s["divisors"][0])
+                       for i in range(0, case["rows"], step)], dim=1)
+        return _exact_epilogue(z, s["bias_rows"], case["act"], s["residual_rows"])
+    if case["op"] == "grouped":
+        ends = s["offsets"].tolist()
+        width = case["rows"] // 2 if case["act"].endswith("_mul") else case["rows"]
+        out = torch.zeros(s["x"].shape[0], width, dtype=torch.float64, device="cuda")
+        for e in range(case["experts"]):
+            a, b = ends[e], ends[e + 1]
+            if a < b:
+                z = _exact_product(s["x"][a:b], s["packed"][e], s["scales"][e], s["divisors"][e])
+                out[a:b] = _exact_epilogue(z, None if s["bias_rows"] is None else s["bias_rows"][e], case["act"], None)
+        return out
+    ids, experts, topk = s["ids"].cpu().numpy().reshape(-1), case["experts"], case["topk"]
+    kept = np.flatnonzero(ids >= 0)
+    picks = kept[np.lexsort((kept, ids[kept]))]  # the pick of each row, in expert order
+    tokens = torch.from_numpy(picks // topk).cuda()
+    count, hidden = len(picks), case["hidden"]
+    if case["op"] == "sort":
+        rows = torch.zeros(ids.size, hidden, dtype=torch.float64, device="cuda")
+        rows[:count] = s["x"].detach().double()[tokens]
+        perm = np.full(ids.size, -1, np.int32)
+        perm[:count] = picks
+        inverse = np.full(ids.size, -1, np.int32)
+        inverse[picks] = np.arange(count)
+        offsets = np.concatenate(([0], np.cumsum(np.bincount(ids[kept], minlength=experts)))).astype(np.int32)
+        out = {"rows": rows, "perm": torch.from_numpy(perm), "offsets": torch.from_numpy(offsets),
+               "inverse": torch.from_numpy(inverse).reshape(-1, topk)}
+        if case["grad"]:
+            out["dx"] = torch.zeros(case["tokens"], hidden, dtype=torch.float64, device="cuda")
+            out["dx"].index_add_(0, tokens, s["g"][:count].double())
+        return out
+    y, w = s["rows"].detach()[:count].double(), s["weights"].detach().double().reshape(-1)
+    at = torch.from_numpy(picks).cuda()
+    z = torch.zeros(case["tokens"], hidden, dtype=torch.float64, device="cuda").index_add_(0, tokens, y * w[at, None])
+    out = {"out": z if s["res"] is None else z + s["res"].double()}
+    if case["grad"]:
+        g = s["g"].double()[tokens]
+        out["drows"] = torch.zeros(ids.size, hidden, dtype=torch.float64, device="cuda")
+        out["drows"][:count] = g * w[at, None]
+        dw = torch.zeros(ids.size, dtype=torch.float64, device="cuda")
+        dw[at] = torch.einsum("ij,ij->i", g, y)
+        out["dweights"] = dw.reshape(-1, topk)
+    return out
