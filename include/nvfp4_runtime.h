@@ -328,6 +328,186 @@ NVFP4_API nvfp4_status nvfp4_linear_ptr_f32(
     float * dst,
     void * stream);
 
+/* ------------------------------------------- linear with epilogue, groups */
+
+/* additive: element types of the entry points below. */
+enum {
+    NVFP4_TYPE_BF16 = 0,
+    NVFP4_TYPE_F16 = 1,
+    NVFP4_TYPE_F32 = 2,
+};
+
+/* additive: activations. GELU is z * Phi(z), GELU_TANH its tanh form. With
+ * NVFP4_ACT_GATED added, the first half of the weight rows is the gate and
+ * the second half the value it multiplies: act(gate) * up, half as many
+ * output columns as weight rows. */
+enum {
+    NVFP4_ACT_NONE = 0,
+    NVFP4_ACT_RELU = 1,
+    NVFP4_ACT_SILU = 2,
+    NVFP4_ACT_GELU = 3,
+    NVFP4_ACT_GELU_TANH = 4,
+    NVFP4_ACT_GATED = 16,
+};
+
+/* additive: `groups` NVFP4 matrices of one shape (the experts of a layer),
+ * one after the other: packed [groups, rows, cols/2], scales_e4m3
+ * [groups, rows, cols/16], divisors FP32 [groups], in host or device memory
+ * (device sources must be complete: the copy runs on the runtime's stream and
+ * is waited for). 1 to 1024 groups, cols a multiple of 16, at most 49152. The
+ * handle works with nvfp4_linear_fused (one group), nvfp4_linear_grouped and
+ * nvfp4_matrix_destroy; the FP32 nvfp4_linear_* entry points refuse it. */
+NVFP4_API nvfp4_status nvfp4_matrix_upload_grouped(
+    nvfp4_runtime * runtime,
+    const void * packed,
+    size_t packed_bytes,
+    const void * scales_e4m3,
+    size_t scale_bytes,
+    const float * divisors,
+    int groups,
+    int rows,
+    int cols,
+    nvfp4_matrix ** out_matrix);
+
+/* additive: out[v, r] = residual[v, r] + act(sum_c W[r, c] x[v, c] / divisor
+ * + bias[r]) on device pointers, enqueued on `stream` (a cudaStream_t; NULL
+ * selects the runtime's stream). x [vectors, cols], residual and out
+ * [vectors, rows] (rows / 2 with a gate) are of `type`, each with its own row
+ * stride in elements (columns contiguous); bias [rows] has a type of its own;
+ * bias and residual may be NULL, residual may be out itself. The weights'
+ * values are exact in the products, sums are FP32, and the result is rounded
+ * once. BF16 and FP32 elements of x below 2^-29 of their row's largest finite
+ * value may lose low bits (by less than 2^-39 of that value). No memory is
+ * allocated and the matrix is only read: calls may overlap and be captured in
+ * CUDA graphs. Up to 2^31 - 1 vectors. */
+NVFP4_API nvfp4_status nvfp4_linear_fused(
+    nvfp4_runtime * runtime,
+    const nvfp4_matrix * matrix,
+    const void * x,
+    int type,
+    int64_t x_stride,
+    int vectors,
+    const void * bias,
+    int bias_type,
+    int activation,
+    const void * residual,
+    int64_t residual_stride,
+    void * out,
+    int64_t out_stride,
+    void * stream);
+
+/* additive: the same product for rows sorted by group: rows
+ * [offsets[g], offsets[g + 1]) of x go through group g's weights and bias
+ * ([groups, rows]). offsets is device int32 [groups + 1], not decreasing and
+ * within [0, vectors] (values outside are clamped to it). Rows of out before
+ * offsets[0] and from offsets[groups] on are left as they were, or set to
+ * zero with zero_rest. */
+NVFP4_API nvfp4_status nvfp4_linear_grouped(
+    nvfp4_runtime * runtime,
+    const nvfp4_matrix * matrix,
+    const void * x,
+    int type,
+    int64_t x_stride,
+    int vectors,
+    const int32_t * offsets,
+    const void * bias,
+    int bias_type,
+    int activation,
+    void * out,
+    int64_t out_stride,
+    int zero_rest,
+    void * stream);
+
+/* ------------------------------------------------- rows sorted by expert */
+
+/* additive: bytes of device workspace nvfp4_expert_sort needs (0 for few
+ * picks). */
+NVFP4_API size_t nvfp4_expert_sort_workspace_bytes(
+    int tokens,
+    int topk,
+    int experts);
+
+/* additive: token rows copied to their experts' places. x [tokens, hidden] of
+ * `type` (row stride in elements), ids [tokens, topk] of 4 or 8 bytes (row
+ * stride in elements); an id outside [0, experts) drops its pick. Outputs
+ * (device):
+ *   rows     [tokens * topk, hidden], contiguous: the picks' token rows by
+ *            expert ascending, then by token and pick; zeros past the last
+ *            expert's
+ *   perm     int32 [tokens * topk]: flat pick token * topk + k of each row,
+ *            -1 past the last expert's
+ *   inverse  int32 [tokens, topk]: the row of each pick, -1 for a dropped one
+ *   offsets  int32 [experts + 1]: each expert's first row, then the number of
+ *            rows in use
+ * topk <= 64, experts <= 1024, tokens * topk below 2^31 - 2048. Enqueued on `stream`
+ * (NULL: the runtime's stream); the workspace must not be shared by calls
+ * that overlap. */
+NVFP4_API nvfp4_status nvfp4_expert_sort(
+    nvfp4_runtime * runtime,
+    const void * x,
+    int type,
+    int64_t x_stride,
+    int tokens,
+    int hidden,
+    const void * ids,
+    int ids_bytes,
+    int64_t ids_stride,
+    int topk,
+    int experts,
+    void * rows,
+    int32_t * perm,
+    int32_t * inverse,
+    int32_t * offsets,
+    void * workspace,
+    size_t workspace_bytes,
+    void * stream);
+
+/* additive: out[t] = residual[t] + sum_k weights[t, k] * rows[inverse[t, k]],
+ * picks with inverse -1 left out, in FP32 and the order of k, rounded once.
+ * rows, residual and out are of `type` with row strides in elements; weights
+ * [tokens, topk] (contiguous, a type of their own) may be NULL for ones (the
+ * gradient of nvfp4_expert_sort to x), residual may be NULL. */
+NVFP4_API nvfp4_status nvfp4_expert_return(
+    nvfp4_runtime * runtime,
+    const void * rows,
+    int type,
+    int64_t rows_stride,
+    const int32_t * inverse,
+    const void * weights,
+    int weights_type,
+    const void * residual,
+    int64_t residual_stride,
+    int tokens,
+    int topk,
+    int hidden,
+    void * out,
+    int64_t out_stride,
+    void * stream);
+
+/* additive: gradients of nvfp4_expert_return: drows[inverse[t, k]] =
+ * weights[t, k] * dout[t] (contiguous [tokens * topk, hidden], zeros from row
+ * offsets[experts] on) and dweights[t, k] = <dout[t], rows[inverse[t, k]]>
+ * (weights_type, 0 for a dropped pick). Either output may be NULL (rows is
+ * only read for dweights, offsets for drows). */
+NVFP4_API nvfp4_status nvfp4_expert_return_backward(
+    nvfp4_runtime * runtime,
+    const void * dout,
+    int type,
+    int64_t dout_stride,
+    const void * rows,
+    int64_t rows_stride,
+    const int32_t * inverse,
+    const int32_t * offsets,
+    const void * weights,
+    int weights_type,
+    int tokens,
+    int topk,
+    int hidden,
+    int experts,
+    void * drows,
+    void * dweights,
+    void * stream);
+
 /* ------------------------------------------------------------- MoE bank */
 
 /* reference: nvfp4_runtime.h:392-403 (implemented at

@@ -7,6 +7,7 @@
 
 #include <chrono>
 #include <cstdint>
+#include <initializer_list>
 #include <mutex>
 #include <stdexcept>
 #include <string>
@@ -115,6 +116,29 @@ void raise_device_timeouts(nvfp4_runtime *runtime);
 // The BF16 RMSNorm kernel of nvfp4_rmsnorm_ptr_bf16 (runtime.cu), one CTA per row.
 cudaError_t launch_rmsnorm_bf16(const void *x, const void *weight, void *dst, int rows, int cols, float epsilon,
                                 cudaStream_t stream);
+
+// The runtime's device is current while this lives; the caller's is restored.
+class device_scope {
+  public:
+    explicit device_scope(const nvfp4_runtime *runtime) {
+        int now = 0;
+        check_cuda(cudaGetDevice(&now), "cudaGetDevice");
+        if (now == runtime->device) return;
+        check_cuda(cudaSetDevice(runtime->device), "cudaSetDevice");
+        back_ = now;
+    }
+    ~device_scope() {
+        if (back_ >= 0) cudaSetDevice(back_);
+    }
+    device_scope(const device_scope &) = delete;
+    device_scope &operator=(const device_scope &) = delete;
+
+  private:
+    int back_ = -1;
+};
+
+// Throws when one of `pointers` (NULL skipped) is device memory of another GPU than the runtime's.
+void check_on_device(const nvfp4_runtime *runtime, std::initializer_list<const void *> pointers, const char *operation);
 
 inline uint64_t host_now_ns() {
     return static_cast<uint64_t>(std::chrono::duration_cast<std::chrono::nanoseconds>(

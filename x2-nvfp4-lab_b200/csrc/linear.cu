@@ -33,7 +33,7 @@
 // index so that a warp's LDS.128 hits distinct bank groups.
 
 #include "internal.h"
-#include "linear_tc.cuh"
+#include "linear_matrix.cuh"
 #include "nvfp4_common.cuh"
 
 #include <cuda_fp16.h>
@@ -46,26 +46,6 @@
 #include <string>
 #include <vector>
 
-struct nvfp4_matrix {
-    nvfp4_runtime *runtime = nullptr;
-    int rows = 0;
-    int cols = 0;
-    int packed_pitch = 0;  // bytes per packed row (multiple of 16)
-    int scale_pitch = 0;   // bytes per scale row (multiple of 16)
-    uint8_t *packed = nullptr;
-    uint8_t *scales = nullptr;
-    float inv_global = 0.0f;
-    nvfp4::LinearTcState tc;               // tensor-core path: scale atoms, activation terms, tensor maps
-    volatile int *host_err = nullptr;      // pinned, device-mapped wait-timeout word (read at synchronize)
-
-    ~nvfp4_matrix() {
-        nvfp4::free_linear_tc(tc);
-        if (host_err) cudaFreeHost(const_cast<int *>(host_err));
-        if (packed) cudaFree(packed);
-        if (scales) cudaFree(scales);
-    }
-};
-
 namespace nvfp4 {
 namespace {
 
@@ -73,7 +53,8 @@ constexpr int kLinThreads = 256;
 constexpr int kLinWarps = kLinThreads / 32;
 constexpr int kLinRowsPerWarp = 4;
 constexpr int kLinChunksInFlight = 2;  // 32-column chunks per lane loaded before any math
-constexpr int kLinMaxCols = 49152;
+constexpr const char *kGroupedUpload =
+    "a matrix of nvfp4_matrix_upload_grouped runs through nvfp4_linear_fused and nvfp4_linear_grouped";
 constexpr size_t kLinSmemBudget = 200 * 1024;  // activation bytes of one pass
 
 struct LinearArgs {
@@ -398,6 +379,7 @@ extern "C" NVFP4_API nvfp4_status nvfp4_linear_f32(nvfp4_runtime *runtime, const
                                                    nvfp4_kernel_kind kernel_kind) {
     if (!runtime || !matrix || matrix->runtime != runtime || !x || !dst || vectors <= 0 || !valid_kind(kernel_kind))
         return fail_invalid("invalid linear arguments or mismatched runtime/matrix");
+    if (!matrix->has_terms()) return fail_invalid(kGroupedUpload);
     if (kernel_kind == NVFP4_KERNEL_TILED && vectors == 1)
         return fail_invalid("the tiled kernel requires more than one vector");
     if (kernel_kind == NVFP4_KERNEL_ROW_TILED && vectors != 1)
@@ -437,6 +419,7 @@ nvfp4_status check_device_linear(nvfp4_runtime *runtime, const nvfp4_matrix *mat
     if (!runtime || !matrix || matrix->runtime != runtime || !x || x->runtime != runtime || !dst ||
         dst->runtime != runtime || vectors <= 0 || !valid_kind(kernel_kind))
         return fail_invalid(invalid_message);
+    if (!matrix->has_terms()) return fail_invalid(kGroupedUpload);
     if (!kind_matches(kernel_kind, vectors))
         return fail_invalid(kernel_kind == NVFP4_KERNEL_TILED ? "the tiled kernel requires more than one vector"
                                                               : "the row-tiled kernel requires one vector");
@@ -498,6 +481,7 @@ extern "C" NVFP4_API nvfp4_status nvfp4_linear_ptr_f32(nvfp4_runtime *runtime, c
                                                        const float *x, int vectors, float *dst, void *stream) {
     if (!runtime || !matrix || matrix->runtime != runtime || !x || !dst || vectors <= 0)
         return fail_invalid("invalid linear arguments or mismatched runtime/matrix");
+    if (!matrix->has_terms()) return fail_invalid(kGroupedUpload);
     size_t in_bytes = 0, out_bytes = 0;
     if (!sizes_fit(matrix, vectors, &in_bytes, &out_bytes)) return fail_invalid("linear buffer size overflow");
     // The kernel reads the matrix on the runtime's device: activations and

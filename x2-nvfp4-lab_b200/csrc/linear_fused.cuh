@@ -1,0 +1,102 @@
+// The NVFP4 linear with its epilogue: arguments shared by the host entry
+// points (linear_fused.cu) and the two kernels (linear_gemv.cu, few rows;
+// linear_gemm.cu, many).
+//
+//   out[v, r] = residual[v, r] + act(inv * sum_c W[r, c] x[v, c] + bias[r])
+//
+// and with a gate, for r < rows / 2,
+//
+//   out[v, r] = residual[v, r] + act(z[v, r]) * z[v, rows / 2 + r].
+//
+// W = E2M1 * E4M3(block) has at most six significant bits, so it is exact in
+// FP16 and in BF16; products are exact and sums FP32 in both kernels.
+#pragma once
+
+#include "linear_matrix.cuh"
+#include "nvfp4_common.cuh"
+
+namespace nvfp4 {
+
+struct FusedLinearArgs {
+    const uint8_t *packed;
+    const uint8_t *scales;
+    int packed_pitch, scale_pitch;
+    const float *inv_globals;  // device [groups], or NULL:
+    float inv_global;
+    int groups;
+    int rows, cols;            // of a group's weights
+    int out_rows;              // rows, or rows / 2 with a gate
+    const void *x;
+    long long x_stride;        // elements
+    int type;                  // of x, residual and out
+    int vectors;               // rows of x
+    const int *offsets;        // device [groups + 1] row ranges of the groups, or NULL: one group of all rows
+    const void *bias;          // [groups, rows] or NULL
+    int bias_type;
+    int act;                   // NVFP4_ACT_*, without the gate flag
+    int gated;
+    const void *residual;
+    long long residual_stride;
+    void *out;
+    long long out_stride;
+    int zero_rest;             // rows outside the groups' ranges get zeros
+    int *err, *host_err;       // wait-timeout words of the matrix
+};
+
+__device__ __forceinline__ float load_as_f32(const void *p, int type, size_t i) {
+    if (type == NVFP4_TYPE_F32) return static_cast<const float *>(p)[i];
+    const uint16_t h = static_cast<const uint16_t *>(p)[i];
+    return type == NVFP4_TYPE_F16 ? __half2float(__ushort_as_half(h)) : bf16_bits_to_f32(h);
+}
+
+// The one rounding to the output's type.
+__device__ __forceinline__ void store_from_f32(void *p, int type, size_t i, float v) {
+    if (type == NVFP4_TYPE_F32)
+        static_cast<float *>(p)[i] = v;
+    else
+        static_cast<uint16_t *>(p)[i] =
+            type == NVFP4_TYPE_F16 ? __half_as_ushort(__float2half_rn(v)) : f32_to_bf16_bits(v);
+}
+
+__device__ __forceinline__ float activate(float z, int act) {
+    switch (act) {
+        case NVFP4_ACT_RELU: return z < 0.0f ? 0.0f : z;  // NaN stays NaN
+        case NVFP4_ACT_SILU: return z / (1.0f + expf(-z));
+        // z Phi(z); erfc keeps the small tail of negative z that 1 + erf rounds away.
+        case NVFP4_ACT_GELU: return 0.5f * z * erfcf(-0.70710678118654752f * z);
+        // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u)), u = sqrt(2 / pi) (z + 0.044715 z^3).
+        case NVFP4_ACT_GELU_TANH: return z / (1.0f + expf(-1.5957691216057308f * (z + 0.044715f * z * z * z)));
+        default: return z;
+    }
+}
+
+// First row and count of a group, whatever the offsets hold kept inside the call's rows.
+__device__ __forceinline__ void group_range(const FusedLinearArgs &a, int g, int *first, int *count) {
+    if (!a.offsets) {
+        *first = 0;
+        *count = a.vectors;
+        return;
+    }
+    const int lo = min(max(__ldg(a.offsets + g), 0), a.vectors);
+    *first = lo;
+    *count = min(max(__ldg(a.offsets + g + 1), lo), a.vectors) - lo;
+}
+
+// Zeros to the rows before the first group's and past the last one's (the
+// rows that no group owns when the offsets do not decrease).
+__device__ __forceinline__ void zero_other_rows(const FusedLinearArgs &a) {
+    if (!a.zero_rest || !a.offsets) return;
+    const int head = min(max(__ldg(a.offsets), 0), a.vectors);
+    const int tail = min(max(__ldg(a.offsets + a.groups), head), a.vectors);
+    const long long n = (long long)(head + a.vectors - tail) * a.out_rows;
+    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
+        long long v = i / a.out_rows;
+        const long long r = i - v * a.out_rows;
+        if (v >= head) v += tail - head;
+        store_from_f32(a.out, a.type, (size_t)(v * a.out_stride + r), 0.0f);
+    }
+}
+
+void launch_linear_gemv(const FusedLinearArgs &a, int sm_count, cudaStream_t stream);
+
+}  // namespace nvfp4

@@ -1,0 +1,41 @@
+// The resident NVFP4 weights behind nvfp4_matrix handles, shared by the
+// linear entry points (linear.cu: dense FP32; linear_fused.cu: epilogues and
+// groups).
+#pragma once
+
+#include "internal.h"
+#include "linear_tc.cuh"
+
+struct nvfp4_matrix {
+    nvfp4_runtime *runtime = nullptr;
+    int groups = 1;        // weight matrices of the same shape, one after the other
+    int rows = 0;          // per group
+    int cols = 0;
+    int packed_pitch = 0;  // bytes per packed row (multiple of 16)
+    int scale_pitch = 0;   // bytes per scale row (multiple of 16)
+    uint8_t *packed = nullptr;   // [groups * rows][packed_pitch]
+    uint8_t *scales = nullptr;   // [groups * rows][scale_pitch]
+    float inv_global = 0.0f;     // of a matrix uploaded on its own
+    float *inv_globals = nullptr;          // device [groups], of a grouped upload (NULL otherwise)
+    nvfp4::LinearTcState tc;               // FP32 tensor-core path (not of a grouped upload): scale atoms, terms, maps
+    CUtensorMap map_packed;                // grouped upload: packed rows, box 128 B x 128 rows, 128-byte swizzle
+    volatile int *host_err = nullptr;      // pinned, device-mapped wait-timeout word (read at synchronize)
+
+    // Whether nvfp4_linear_* (FP32, no epilogue) can run it.
+    bool has_terms() const { return tc.w_atoms != nullptr; }
+
+    ~nvfp4_matrix() {
+        nvfp4::free_linear_tc(tc);
+        if (host_err) cudaFreeHost(const_cast<int *>(host_err));
+        if (packed) cudaFree(packed);
+        if (scales) cudaFree(scales);
+        if (inv_globals) cudaFree(inv_globals);
+    }
+};
+
+namespace nvfp4 {
+
+constexpr int kLinMaxCols = 49152;
+constexpr int kLinMaxGroups = 1024;
+
+}  // namespace nvfp4

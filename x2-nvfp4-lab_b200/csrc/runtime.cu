@@ -267,6 +267,24 @@ void raise_device_timeouts(nvfp4_runtime *runtime) {
     }
 }
 
+void check_on_device(const nvfp4_runtime *runtime, std::initializer_list<const void *> pointers,
+                     const char *operation) {
+    for (const void *p : pointers) {
+        if (!p) continue;
+        cudaPointerAttributes attr{};
+        if (cudaPointerGetAttributes(&attr, p) != cudaSuccess) {
+            cudaGetLastError();
+            throw invalid_argument_error(std::string(operation) + ": cannot query the device of an argument");
+        }
+        if (attr.type == cudaMemoryTypeUnregistered || attr.type == cudaMemoryTypeHost)
+            throw invalid_argument_error(std::string(operation) + ": arguments must be device memory");
+        if (attr.type == cudaMemoryTypeDevice && attr.device != runtime->device)
+            throw invalid_argument_error(std::string(operation) + ": arguments must be on the runtime's device (cuda:" +
+                                         std::to_string(runtime->device) + "), got cuda:" +
+                                         std::to_string(attr.device));
+    }
+}
+
 }  // namespace nvfp4
 
 extern "C" NVFP4_API nvfp4_status nvfp4_runtime_synchronize(nvfp4_runtime *runtime) {

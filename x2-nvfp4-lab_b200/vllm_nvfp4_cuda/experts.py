@@ -1,0 +1,231 @@
+"""Token rows sorted by expert and brought back, with their gradients.
+
+The pieces between a router and experts that are not a ``MoeBank`` (other
+products, other top-k, training): ``expert_sort`` copies every token's row to
+its experts' places in expert order, the caller runs the experts on the rows
+(``Runtime.linear_grouped`` for NVFP4 weights, with ``order.offsets``), and
+``expert_return`` weights and sums every token's rows. Both are differentiable
+(once): the sort in x, the return in the rows, the weights and the residual.
+They are reached as ``Runtime.expert_sort`` and ``Runtime.expert_return``; the
+lab has no counterpart.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from .runtime import _stream_handle
+
+# Element types of the C ABI (NVFP4_TYPE_*).
+TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+MAX_TOPK, MAX_EXPERTS = 64, 1024
+
+
+@dataclass(frozen=True)
+class ExpertOrder:
+    """Where ``expert_sort`` put the picks (int32 CUDA tensors)."""
+
+    perm: torch.Tensor     # [T*K] flat pick token*K + k of each row, -1 past the last expert's rows
+    inverse: torch.Tensor  # [T, K] row of each pick, -1 where its id names no expert
+    offsets: torch.Tensor  # [experts + 1] first row of each expert, then the number of rows in use
+    experts: int
+
+
+def _rows_of(t: torch.Tensor) -> torch.Tensor:
+    """t with contiguous columns (a row stride is kept)."""
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def on_stream(stream, tensors, call):
+    """``call()`` on torch's current stream, or on ``stream``: what it allocates then belongs to that stream, and
+    the given tensors are kept from reuse until the stream is done with them."""
+    if stream is None:
+        return call()
+    with torch.cuda.stream(stream):
+        result = call()
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
+    return result
+
+
+def _handle(device) -> object:
+    return _stream_handle(torch.cuda.current_stream(device))
+
+
+# ------------------------------------------------------------------ one call each
+
+
+def _sort(rt, x, ids, experts):
+    tokens, hidden = x.shape
+    topk = ids.shape[1]
+    picks = tokens * topk
+    rows = x.new_empty((picks, hidden))
+    table = torch.empty(2 * picks + experts + 1, dtype=torch.int32, device=x.device)
+    perm, inverse, offsets = table[:picks], table[picks:2 * picks].view(tokens, topk), table[2 * picks:]
+    if tokens == 0:
+        offsets.zero_()
+        return rows, perm, inverse, offsets
+    x, ids = _rows_of(x), _rows_of(ids)
+    size = rt.lib.nvfp4_expert_sort_workspace_bytes(tokens, topk, experts)
+    workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    rt._check(
+        rt.lib.nvfp4_expert_sort(
+            rt.handle, x.data_ptr(), TYPES[x.dtype], _row_stride(x), tokens, hidden, ids.data_ptr(),
+            ids.element_size(), _row_stride(ids), topk, experts, rows.data_ptr(), perm.data_ptr(),
+            inverse.data_ptr(), offsets.data_ptr(), workspace.data_ptr() if size else None, size,
+            _handle(x.device)),
+        "nvfp4_expert_sort")
+    return rows, perm, inverse, offsets
+
+
+def _return(rt, rows, inverse, weights, residual, out):
+    tokens, topk = inverse.shape
+    hidden = rows.shape[1]
+    if out is None:
+        out = rows.new_empty((tokens, hidden))
+    if tokens == 0:
+        return out
+    rows = _rows_of(rows)
+    if residual is not None:
+        residual = _rows_of(residual)
+    if weights is not None:
+        weights = weights.contiguous()
+    rt._check(
+        rt.lib.nvfp4_expert_return(
+            rt.handle, rows.data_ptr(), TYPES[rows.dtype], _row_stride(rows), inverse.data_ptr(),
+            weights.data_ptr() if weights is not None else None,
+            TYPES[weights.dtype] if weights is not None else 0,
+            residual.data_ptr() if residual is not None else None,
+            _row_stride(residual) if residual is not None else 0, tokens, topk, hidden, out.data_ptr(),
+            _row_stride(out), _handle(rows.device)),
+        "nvfp4_expert_return")
+    return out
+
+
+def _return_backward(rt, dout, rows, inverse, offsets, weights, experts, need_rows, need_weights):
+    tokens, topk = inverse.shape
+    hidden = dout.shape[1]
+    drows = dout.new_empty((tokens * topk, hidden)) if need_rows else None
+    dweights = torch.empty((tokens, topk), dtype=weights.dtype, device=dout.device) if need_weights else None
+    if tokens == 0:
+        return drows, dweights
+    dout = _rows_of(dout)
+    if rows is not None:
+        rows = _rows_of(rows)
+    if weights is not None:
+        weights = weights.contiguous()
+    rt._check(
+        rt.lib.nvfp4_expert_return_backward(
+            rt.handle, dout.data_ptr(), TYPES[dout.dtype], _row_stride(dout),
+            rows.data_ptr() if need_weights else None, _row_stride(rows) if need_weights else 0,
+            inverse.data_ptr(), offsets.data_ptr(), weights.data_ptr() if weights is not None else None,
+            TYPES[weights.dtype] if weights is not None else 0, tokens, topk, hidden, experts,
+            drows.data_ptr() if need_rows else None, dweights.data_ptr() if need_weights else None,
+            _handle(dout.device)),
+        "nvfp4_expert_return_backward")
+    return drows, dweights
+
+
+# ------------------------------------------------------------------ gradients
+
+
+class _ExpertSort(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, rt, ids, experts):
+        rows, perm, inverse, offsets = _sort(rt, x, ids, experts)
+        ctx.rt = rt
+        ctx.save_for_backward(inverse)
+        ctx.mark_non_differentiable(perm, inverse, offsets)
+        return rows, perm, inverse, offsets
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, drows, *_):
+        (inverse,) = ctx.saved_tensors
+        return _return(ctx.rt, drows, inverse, None, None, None), None, None, None
+
+
+class _ExpertReturn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, weights, residual, rt, order):
+        ctx.rt = rt
+        ctx.experts = order.experts
+        ctx.given = (weights is not None, residual is not None)
+        # The rows are kept only for the weights' gradient.
+        keep = weights is not None and ctx.needs_input_grad[1]
+        ctx.save_for_backward(rows if keep else None, weights, order.inverse, order.offsets)
+        return _return(rt, rows, order.inverse, weights, residual, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        rows, weights, inverse, offsets = ctx.saved_tensors
+        need_rows, need_weights, need_residual = ctx.needs_input_grad[:3]
+        drows = dweights = None
+        if need_rows or need_weights:
+            drows, dweights = _return_backward(ctx.rt, dout, rows, inverse, offsets, weights, ctx.experts, need_rows,
+                                               need_weights)
+        return drows, dweights, dout if need_residual else None, None, None
+
+
+# ------------------------------------------------------------------ checks
+
+
+def _require(condition, message):
+    if not condition:
+        raise ValueError(message)
+
+
+def expert_sort(rt, x, ids, experts: int, stream=None):
+    _require(x.is_cuda and x.dim() == 2 and x.dtype in TYPES and x.shape[1] > 0,
+             "x must be a CUDA bfloat16, float16 or float32 tensor [tokens, hidden]")
+    _require(ids.dtype in (torch.int32, torch.int64) and ids.dim() == 2 and ids.shape[0] == x.shape[0]
+             and ids.device == x.device, "ids must be int32 or int64 [tokens, topk] on x's device")
+    _require(1 <= ids.shape[1] <= MAX_TOPK, f"the expert sort supports 1 to {MAX_TOPK} picks a token")
+    experts = int(experts)
+    _require(1 <= experts <= MAX_EXPERTS, f"the expert sort supports 1 to {MAX_EXPERTS} experts")
+
+    def call():
+        if x.requires_grad and torch.is_grad_enabled():
+            return _ExpertSort.apply(x, rt, ids, experts)
+        return _sort(rt, x, ids, experts)
+
+    rows, perm, inverse, offsets = on_stream(stream, (x, ids), call)
+    return rows, ExpertOrder(perm, inverse, offsets, experts)
+
+
+def expert_return(rt, rows, order: ExpertOrder, weights=None, residual=None, out=None, stream=None):
+    tokens, topk = order.inverse.shape
+    _require(rows.is_cuda and rows.dim() == 2 and rows.dtype in TYPES and rows.shape[0] == tokens * topk
+             and rows.shape[1] > 0 and rows.device == order.inverse.device,
+             "rows must be a CUDA bfloat16, float16 or float32 tensor [tokens * topk, hidden] on the order's device")
+    shape = (tokens, rows.shape[1])
+    if weights is not None:
+        _require(tuple(weights.shape) == (tokens, topk) and weights.dtype in TYPES and weights.device == rows.device,
+                 "weights must be bfloat16, float16 or float32 [tokens, topk] on the rows' device")
+    if residual is not None:
+        _require(tuple(residual.shape) == shape and residual.dtype == rows.dtype and residual.device == rows.device,
+                 "residual must match the rows' type and device, [tokens, hidden]")
+    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (rows, weights, residual))
+    if out is not None:
+        _require(tuple(out.shape) == shape and out.dtype == rows.dtype and out.device == rows.device
+                 and (out.stride(1) == 1 or shape[1] == 1) and (tokens < 2 or out.stride(0) >= shape[1]),
+                 "out must match the rows' type and device, [tokens, hidden] with contiguous columns")
+        _require(not grad and not out.requires_grad, "out cannot be given where gradients are recorded")
+
+    def call():
+        if grad:
+            return _ExpertReturn.apply(rows, weights, residual, rt, order)
+        return _return(rt, rows, order.inverse, weights, residual, out)
+
+    return on_stream(stream, (rows, order.inverse, order.offsets, weights, residual, out), call)
+
+
+__all__ = ["ExpertOrder", "expert_return", "expert_sort"]

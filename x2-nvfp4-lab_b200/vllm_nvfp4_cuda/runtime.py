@@ -187,6 +187,25 @@ _SIGNATURES: dict[str, tuple[list, object]] = {
     "nvfp4_linear_device_enqueue_f32": (
         [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int], C.c_int),
     "nvfp4_linear_ptr_f32": ([C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p], C.c_int),
+    "nvfp4_matrix_upload_grouped": (
+        [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p, C.c_int, C.c_int, C.c_int,
+         C.POINTER(C.c_void_p)], C.c_int),
+    "nvfp4_linear_fused": (
+        [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p,
+         C.c_int64, C.c_void_p, C.c_int64, C.c_void_p], C.c_int),
+    "nvfp4_linear_grouped": (
+        [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
+         C.c_void_p, C.c_int64, C.c_int, C.c_void_p], C.c_int),
+    "nvfp4_expert_sort_workspace_bytes": ([C.c_int, C.c_int, C.c_int], C.c_size_t),
+    "nvfp4_expert_sort": (
+        [C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_int,
+         C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p], C.c_int),
+    "nvfp4_expert_return": (
+        [C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int,
+         C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_void_p], C.c_int),
+    "nvfp4_expert_return_backward": (
+        [C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
+         C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
     "nvfp4_quantize_rows_enqueue": (
         [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p],
         C.c_int),
@@ -334,7 +353,10 @@ class EpContext:
 
 
 class NativeMatrix:
-    """A dense NVFP4 weight matrix resident on the device (runtime.py:94-115)."""
+    """A dense NVFP4 weight matrix resident on the device (runtime.py:94-115),
+    or several of one shape (additive: ``Runtime.upload_grouped``)."""
+
+    groups = 1
 
     def __init__(self, runtime: "Runtime", handle: C.c_void_p, rows: int, cols: int):
         self.runtime = runtime
@@ -355,6 +377,12 @@ class NativeMatrix:
         except Exception:
             pass
 
+
+# Activations of the linear with epilogue (NVFP4_ACT_*); "<name>_mul" is the
+# gated form, act(gate) * up.
+NVFP4_ACT_GATED = 16
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+ACTIVATIONS.update({f"{name}_mul": code | NVFP4_ACT_GATED for name, code in list(ACTIVATIONS.items()) if name})
 
 KERNEL_SCALAR, KERNEL_SUBGROUP, KERNEL_TILED, KERNEL_ROW_TILED = 0, 1, 2, 3
 
@@ -968,6 +996,88 @@ class Runtime:
             "nvfp4_linear_ptr_f32",
         )
         return out
+
+    def upload_grouped(self, packed, scales, divisors) -> NativeMatrix:
+        """additive: NVFP4 matrices of one shape (the experts of a layer):
+        packed uint8 [groups, rows, cols/2], scales E4M3 bytes [groups, rows,
+        cols/16], divisors float32 [groups], all numpy arrays or all CUDA
+        tensors (scales float8_e4m3fn or uint8). The handle is for
+        ``linear_grouped``, with one group for ``linear_fused``."""
+        if isinstance(packed, np.ndarray):
+            packed = np.ascontiguousarray(packed, dtype=np.uint8)
+            scales = np.ascontiguousarray(scales).view(np.uint8)
+            divisors = np.ascontiguousarray(divisors, dtype=np.float32).reshape(-1)
+            sizes = packed.nbytes, scales.nbytes
+            pointers = packed.ctypes.data, scales.ctypes.data, divisors.ctypes.data
+        else:
+            import torch
+
+            if not (packed.is_cuda and scales.is_cuda and divisors.is_cuda) or packed.dtype != torch.uint8 or \
+                    scales.element_size() != 1 or len({packed.device, scales.device, divisors.device}) != 1:
+                raise ValueError("packed, scales and divisors must be tensors of one CUDA device, the first two of bytes")
+            packed, scales = packed.contiguous(), scales.contiguous()
+            divisors = divisors.to(torch.float32).contiguous().reshape(-1)
+            # The copy runs on the runtime's own stream: wait for torch's.
+            torch.cuda.current_stream(packed.device).synchronize()
+            sizes = packed.numel(), scales.numel()
+            pointers = packed.data_ptr(), scales.data_ptr(), divisors.data_ptr()
+        if packed.ndim != 3 or scales.ndim != 3 or divisors.shape[0] != packed.shape[0] or \
+                tuple(scales.shape[:2]) != tuple(packed.shape[:2]):
+            raise ValueError("packed must be [groups, rows, cols/2], scales [groups, rows, cols/16], divisors [groups]")
+        groups, rows, cols = packed.shape[0], packed.shape[1], packed.shape[2] * 2
+        handle = C.c_void_p()
+        self._check(
+            self.lib.nvfp4_matrix_upload_grouped(self.handle, pointers[0], sizes[0], pointers[1], sizes[1],
+                                                 pointers[2], groups, rows, cols, C.byref(handle)),
+            "nvfp4_matrix_upload_grouped",
+        )
+        matrix = NativeMatrix(self, handle, rows, cols)
+        matrix.groups = groups
+        return matrix
+
+    def linear_fused(self, matrix: NativeMatrix, x, *, bias=None, activation: str | None = None, residual=None,
+                     out=None, stream=None):
+        """additive: ``residual + act(x W^T / divisor + bias)`` in one pass, on
+        CUDA tensors: x [..., cols] bfloat16, float16 or float32; bias [rows]
+        of any of these types; residual and out [..., rows] of x's type (out
+        may be the residual). ``activation``: None, "relu", "silu", "gelu",
+        "gelu_tanh", or the gated "<name>_mul" (the first half of the matrix
+        rows is the gate: act(gate) * up, rows / 2 outputs). Sums are FP32,
+        the result is rounded once. Inference only. Enqueued on ``stream``
+        (None: torch's current stream)."""
+        from . import fused
+
+        return fused.linear_fused(self, matrix, x, bias, activation, residual, out, stream)
+
+    def linear_grouped(self, matrix: NativeMatrix, x, offsets, *, bias=None, activation: str | None = None, out=None,
+                       stream=None):
+        """additive: ``linear_fused`` for rows sorted by group: rows
+        [offsets[g], offsets[g+1]) of x [rows, cols] through group g of the
+        matrix and bias[g] (bias [groups, rows]). offsets: int32 [groups + 1]
+        on the GPU (``ExpertOrder.offsets``). Rows of no group are zero in a
+        new out and left as they were in a given one."""
+        from . import fused
+
+        return fused.linear_grouped(self, matrix, x, offsets, bias, activation, out, stream)
+
+    def expert_sort(self, x, ids, experts: int, stream=None):
+        """additive: (rows, order): every token's row of x [tokens, hidden]
+        copied to its picks' places, by expert, then token and pick. ids int32
+        or int64 [tokens, topk]; a pick whose id is outside [0, experts) is
+        dropped, and as many rows at the end are zero. Differentiable in x
+        (vllm_nvfp4_cuda.experts). Enqueued on ``stream`` (None: torch's
+        current stream)."""
+        from . import experts as impl
+
+        return impl.expert_sort(self, x, ids, experts, stream)
+
+    def expert_return(self, rows, order, weights=None, residual=None, out=None, stream=None):
+        """additive: out[t] = residual[t] + sum_k weights[t, k] * rows[order.inverse[t, k]]
+        ([tokens, hidden], dropped picks left out, FP32 sums; weights None:
+        ones). Differentiable in rows, weights and residual."""
+        from . import experts as impl
+
+        return impl.expert_return(self, rows, order, weights, residual, out, stream)
 
     def quantize_rows(self, x, terms: int):
         """additive: split BF16/FP16 rows [rows, cols] (a CUDA tensor) into
