@@ -369,6 +369,18 @@ NVFP4_API nvfp4_status nvfp4_matrix_upload_grouped(
     int cols,
     nvfp4_matrix ** out_matrix);
 
+/* additive: bytes of 256-byte aligned device workspace that a call of
+ * nvfp4_linear_fused (grouped 0) or nvfp4_linear_grouped (1) with these
+ * arguments needs; 0 for many. Calls that overlap need workspaces of their
+ * own. */
+NVFP4_API size_t nvfp4_linear_workspace_bytes(
+    const nvfp4_matrix * matrix,
+    const void * x,
+    int type,
+    int64_t x_stride,
+    int vectors,
+    int grouped);
+
 /* additive: out[v, r] = residual[v, r] + act(sum_c W[r, c] x[v, c] / divisor
  * + bias[r]) on device pointers, enqueued on `stream` (a cudaStream_t; NULL
  * selects the runtime's stream). x [vectors, cols], residual and out
@@ -394,6 +406,8 @@ NVFP4_API nvfp4_status nvfp4_linear_fused(
     int64_t residual_stride,
     void * out,
     int64_t out_stride,
+    void * workspace,
+    size_t workspace_bytes,
     void * stream);
 
 /* additive: the same product for rows sorted by group: rows
@@ -416,6 +430,8 @@ NVFP4_API nvfp4_status nvfp4_linear_grouped(
     void * out,
     int64_t out_stride,
     int zero_rest,
+    void * workspace,
+    size_t workspace_bytes,
     void * stream);
 
 /* ------------------------------------------------- rows sorted by expert */

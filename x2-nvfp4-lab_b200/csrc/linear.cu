@@ -344,6 +344,7 @@ extern "C" NVFP4_API nvfp4_status nvfp4_matrix_upload(nvfp4_runtime *runtime, co
         check_cuda(init_linear_tc(m->tc, m->packed, m->packed_pitch, m->scales, m->scale_pitch, rows, cols,
                                   runtime->stream),
                    "tensor-core linear set-up");
+        make_matrix_maps(*m);
         int *host_err = nullptr;
         check_cuda(cudaHostAlloc(reinterpret_cast<void **>(&host_err), sizeof(int), cudaHostAllocMapped),
                    "cudaHostAlloc(matrix error word)");

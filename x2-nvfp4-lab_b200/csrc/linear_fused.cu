@@ -77,13 +77,25 @@ const char *fused_args(FusedLinearArgs &a, const nvfp4_runtime *runtime, const n
     return nullptr;
 }
 
-nvfp4_status run_fused(nvfp4_runtime *runtime, const FusedLinearArgs &a, void *stream, const char *operation) {
+// Few rows stream the weights through the GEMV kernel, more go to the tensor
+// memory kernel (average rows of a group, since the counts are on the device).
+bool few_rows(int vectors, int groups) { return vectors <= 32LL * groups; }
+
+nvfp4_status run_fused(nvfp4_runtime *runtime, const nvfp4_matrix *matrix, const FusedLinearArgs &a, void *workspace,
+                       size_t workspace_bytes, void *stream, const char *operation) {
+    const bool few = few_rows(a.vectors, a.offsets ? a.groups : 1);
+    if (!few && workspace_bytes < linear_gemm_workspace(a.type, a.x, a.x_stride, a.vectors, a.cols))
+        return fail_invalid("the linear's workspace is too small (nvfp4_linear_workspace_bytes)");
+    if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail_invalid("the linear's workspace must be 256-byte aligned");
     try {
         const device_scope scope(runtime);
         check_on_device(runtime, {a.x, a.out}, operation);
         std::lock_guard<std::mutex> lock(runtime->queue_mutex);
         runtime->direct_call(static_cast<cudaStream_t>(stream), [&](cudaStream_t os) {
-            runtime->profiled_kernel(operation, os, [&](cudaStream_t s) { launch_linear_gemv(a, runtime->sm_count, s); });
+            runtime->profiled_kernel(operation, os, [&](cudaStream_t s) {
+                if (few) launch_linear_gemv(a, runtime->sm_count, s);
+                else launch_linear_gemm(a, *matrix, workspace, runtime->sm_count, s);
+            });
         });
         clear_last_error();
         return NVFP4_STATUS_OK;
@@ -146,6 +158,7 @@ extern "C" NVFP4_API nvfp4_status nvfp4_matrix_upload_grouped(nvfp4_runtime *run
         check_cuda(cudaGetLastError(), "grouped_scales_kernel");
         inverse_kernel<<<1, 256, 0, s>>>(m->inv_globals, groups);
         check_cuda(cudaGetLastError(), "inverse_kernel");
+        make_matrix_maps(*m);
         int *host_err = nullptr;
         check_cuda(cudaHostAlloc(reinterpret_cast<void **>(&host_err), sizeof(int), cudaHostAllocMapped),
                    "cudaHostAlloc(matrix error word)");
@@ -163,11 +176,17 @@ extern "C" NVFP4_API nvfp4_status nvfp4_matrix_upload_grouped(nvfp4_runtime *run
     }
 }
 
+extern "C" NVFP4_API size_t nvfp4_linear_workspace_bytes(const nvfp4_matrix *matrix, const void *x, int type,
+                                                         int64_t x_stride, int vectors, int grouped) {
+    if (!matrix || !valid_type(type) || vectors <= 0 || few_rows(vectors, grouped ? matrix->groups : 1)) return 0;
+    return linear_gemm_workspace(type, x, x_stride, vectors, matrix->cols);
+}
+
 extern "C" NVFP4_API nvfp4_status nvfp4_linear_fused(nvfp4_runtime *runtime, const nvfp4_matrix *matrix, const void *x,
                                                      int type, int64_t x_stride, int vectors, const void *bias,
                                                      int bias_type, int activation, const void *residual,
                                                      int64_t residual_stride, void *out, int64_t out_stride,
-                                                     void *stream) {
+                                                     void *workspace, size_t workspace_bytes, void *stream) {
     FusedLinearArgs a{};
     if (const char *message = fused_args(a, runtime, matrix, x, type, x_stride, vectors, bias, bias_type, activation,
                                          out, out_stride))
@@ -177,14 +196,14 @@ extern "C" NVFP4_API nvfp4_status nvfp4_linear_fused(nvfp4_runtime *runtime, con
         return fail_invalid("invalid residual stride or alignment");
     a.residual = residual;
     a.residual_stride = residual_stride;
-    return run_fused(runtime, a, stream, "linear_fused");
+    return run_fused(runtime, matrix, a, workspace, workspace_bytes, stream, "linear_fused");
 }
 
 extern "C" NVFP4_API nvfp4_status nvfp4_linear_grouped(nvfp4_runtime *runtime, const nvfp4_matrix *matrix,
                                                        const void *x, int type, int64_t x_stride, int vectors,
                                                        const int32_t *offsets, const void *bias, int bias_type,
                                                        int activation, void *out, int64_t out_stride, int zero_rest,
-                                                       void *stream) {
+                                                       void *workspace, size_t workspace_bytes, void *stream) {
     FusedLinearArgs a{};
     if (const char *message = fused_args(a, runtime, matrix, x, type, x_stride, vectors, bias, bias_type, activation,
                                          out, out_stride))
@@ -192,5 +211,5 @@ extern "C" NVFP4_API nvfp4_status nvfp4_linear_grouped(nvfp4_runtime *runtime, c
     if (!offsets || (reinterpret_cast<uintptr_t>(offsets) & 3u)) return fail_invalid("grouped linear needs offsets");
     a.offsets = offsets;
     a.zero_rest = zero_rest != 0;
-    return run_fused(runtime, a, stream, "linear_grouped");
+    return run_fused(runtime, matrix, a, workspace, workspace_bytes, stream, "linear_grouped");
 }

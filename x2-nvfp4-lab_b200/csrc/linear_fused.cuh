@@ -99,4 +99,10 @@ __device__ __forceinline__ void zero_other_rows(const FusedLinearArgs &a) {
 
 void launch_linear_gemv(const FusedLinearArgs &a, int sm_count, cudaStream_t stream);
 
+// Device workspace of launch_linear_gemm for this call: 0 when the kernel can
+// read x where it lies.
+size_t linear_gemm_workspace(int type, const void *x, long long x_stride, int vectors, int cols);
+void launch_linear_gemm(const FusedLinearArgs &a, const nvfp4_matrix &matrix, void *workspace, int sm_count,
+                        cudaStream_t stream);
+
 }  // namespace nvfp4

@@ -1,0 +1,638 @@
+// NVFP4 linear with epilogue for many rows: tcgen05 with the weights decoded on
+// the way in.
+//
+// A weight E2M1 * E4M3 is exact in FP16 and in BF16, so the product runs as a
+// plain 16-bit MMA on x as it is: no rounding but the FP32 sums'. The weights
+// are the A operand (128 rows, M) and lie in tensor memory: conversion warps read
+// the packed bytes from shared memory, decode a row's 64 columns in registers
+// and store them with tcgen05.st, so that neither the decoded tile nor its
+// reads cross shared memory, whose bandwidth the B operand needs. The rows of
+// x are B (N = 16 to 192, as many as the tile has: the instruction's N is chosen per tile),
+// loaded by TMA. With a gate the tile is 64 gate and 64 up rows, 16 of each in
+// every lane quarter.
+//
+// Warps: 0 producer of x and 2 of weights (TMA), 1 MMA issuer, 4-11 conversion (two warpgroups, every
+// other 64-column step each), 12-15 epilogue. Tensor memory: two accumulators
+// of 192 columns, and four decoded steps of 32. The epilogue turns 32 columns
+// at a time through shared memory, so that a lane has four consecutive outputs
+// of one row of x: bias in registers, residual and stores as vectors.
+//
+// One persistent CTA per SM walks (group, weight tile, x tile) items; x tiles of
+// a group are of even size, and items of one weight tile are neighbours, so
+// that its bytes come from HBM once.
+//
+// FP32 x enters as two FP16 halves, scaled per row by a power of two
+// (linear_gemv.cu has the error), split by a kernel before; x that TMA cannot
+// read (16-byte addresses and strides) is copied by the same kernel.
+#include "linear_fused.cuh"
+#include "tcgen05_util.cuh"
+#include "tma_util.cuh"
+
+#include <algorithm>
+#include <atomic>
+
+namespace nvfp4 {
+namespace {
+
+constexpr int kGmThreads = 512;
+constexpr int kGmConvWarp0 = 4, kGmEpiWarp0 = 12;
+constexpr int kGmStages = 4;                        // 64-column steps in flight
+constexpr int kGmMaxN = 192;
+constexpr int kGmBoxRows = 32;                      // rows of x per TMA box
+constexpr int kGmStageB = kGmMaxN * 128;            // a step of x: up to 192 rows x 64 columns
+constexpr int kGmRawStages = 3;                     // 256 columns of packed weights each
+constexpr int kGmRawBytes = 128 * 128;
+constexpr int kGmRawScales = 128 * 16;
+constexpr int kGmRaw = kGmRawBytes + kGmRawScales;
+constexpr int kGmEpiPitch = 148;                    // floats per row of x in the epilogue's turn
+constexpr int kGmEpiBytes = 32 * kGmEpiPitch * 4;
+constexpr int kGmColA = 2 * kGmMaxN;                // tensor-memory column of the first decoded step
+constexpr int kGmOffB = 0;
+constexpr int kGmOffRaw = kGmOffB + kGmStages * kGmStageB;
+constexpr int kGmOffEpi = kGmOffRaw + kGmRawStages * kGmRaw;
+constexpr int kGmOffBars = kGmOffEpi + 2 * kGmEpiBytes;
+constexpr int kGmBars = 2 * kGmStages + kGmStages + 2 * kGmRawStages + 2 + 2 + 1;
+constexpr int kGmOffTiles = kGmOffBars + kGmBars * 8 + 16;
+constexpr size_t kGmSmem = 1024 + kGmOffTiles + sizeof(int) * (kLinMaxGroups + 1);
+static_assert(kGmSmem <= 232448, "shared memory overflow");
+static_assert(kGmColA + 32 * kGmStages <= 512, "tensor memory overflow");
+static_assert(kGmRawBytes % 1024 == 0 && kGmOffRaw % 1024 == 0 && kGmRaw % 1024 == 0, "swizzled tiles need 1024-byte alignment");
+
+enum GemmWaitSite : int {
+    kSiteFusedEmpty = 71,
+    kSiteFusedRawEmpty = 72,
+    kSiteFusedRawFull = 73,
+    kSiteFusedFull = 74,
+    kSiteFusedAccEmpty = 75,
+    kSiteFusedAccFull = 76,
+};
+
+struct GemmArgs {
+    FusedLinearArgs f;
+    const float *row_scale;  // [vectors] of split FP32 x (NULL: ones)
+    int terms;               // 16-bit parts of x
+    int max_n;               // rows of x per tile
+    int m_tiles;             // weight tiles of a group
+    int raw_steps;           // 256-column steps over K
+    int k_steps;             // 64-column steps over K
+    int wide_out, wide_res;  // four outputs may move as one vector
+};
+
+__device__ __forceinline__ bool wait_drain(uint64_t *bar, uint32_t parity) {
+    const unsigned long long t0 = global_ns();
+    for (uint32_t i = 0;; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 63u) == 63u && global_ns() - t0 > kWaitLimitNs) return false;
+    }
+}
+
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// Eight codes times their block scale as four 16-bit pairs. FP16: `scale` is the scale twice. BF16: an E2M1 value in
+// FP16 has its bits in the sign, the exponent and the first mantissa bit; three places to the right they are the
+// BF16 pattern of value * 2^-112, and `scale` carries 2^112.
+template <bool BF16>
+__device__ __forceinline__ void decode8(uint32_t codes, uint32_t scale, uint32_t *out) {
+    uint32_t h[4];
+    e2m1x8_to_f16x8(codes, h);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (BF16)
+            out[i] = mul_bf16x2(((h[i] >> 3) & 0x0FFF0FFFu) | (h[i] & 0x80008000u), scale);
+        else
+            out[i] = hmul2_u32(h[i], scale);
+    }
+}
+
+// The scale byte at place `i` of `word`, twice, as decode8 wants it. BF16: the byte's bits at the BF16 exponent's
+// end are scale * 2^-120 (subnormals too); two multiplications by 2^116.
+template <bool BF16>
+__device__ __forceinline__ uint32_t scale_pair(uint32_t word, int i) {
+    if constexpr (BF16) {
+        const uint32_t b = ((word >> (8 * i)) & 0x7Fu) * 0x00100010u;
+        return mul_bf16x2(mul_bf16x2(b, 0x79807980u), 0x79807980u);
+    } else {
+        const uint32_t s = e4m3x2_to_f16x2((uint16_t)(word >> (16 * (i >> 1))));
+        return (i & 1) ? f16x2_hi_hi(s) : f16x2_lo_lo(s);
+    }
+}
+
+struct Tile {
+    int group, m, row0, n;  // row0, n: rows of x
+};
+
+// Tile sizes of a group of `count` rows: as many tiles as needed, even, a multiple of 16 rows each.
+__device__ __forceinline__ int x_tiles(int count, int max_n) { return (count + max_n - 1) / max_n; }
+
+__device__ __forceinline__ Tile tile_of(const GemmArgs &a, const int *upto, int item) {
+    // The group with upto[g] * m_tiles <= item < upto[g + 1] * m_tiles.
+    Tile t;
+    const int at = item / a.m_tiles;
+    int lo = 0, hi = a.f.offsets ? a.f.groups : 1;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (upto[mid] <= at) lo = mid;
+        else hi = mid;
+    }
+    t.group = lo;
+    int first, count;
+    group_range(a.f, lo, &first, &count);
+    const int tiles = upto[lo + 1] - upto[lo];
+    const int in_group = item - upto[lo] * a.m_tiles;
+    t.m = in_group / tiles;
+    const int width = ((count + tiles - 1) / tiles + 15) & ~15;
+    const int v = (in_group - t.m * tiles) * width;
+    t.row0 = first + v;
+    t.n = min(width, count - v);
+    return t;
+}
+
+template <int TYPE>
+__device__ __forceinline__ void load4(const void *p, size_t at, bool wide, int valid, float (&v)[4]) {
+    if constexpr (TYPE == NVFP4_TYPE_F32) {
+        const float *q = static_cast<const float *>(p) + at;
+        if (wide && valid == 4) {
+            const float4 w = *reinterpret_cast<const float4 *>(q);
+            v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+            return;
+        }
+    } else if (wide && valid == 4) {
+        const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + at);
+        uint16_t h[4];
+        memcpy(h, &w, 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = TYPE == NVFP4_TYPE_F16 ? __half2float(__ushort_as_half(h[i])) : bf16_bits_to_f32(h[i]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < valid ? load_as_f32(p, TYPE, at + i) : 0.0f;
+}
+
+template <int TYPE>
+__device__ __forceinline__ void store4(void *p, size_t at, bool wide, int valid, const float (&v)[4]) {
+    if (wide && valid == 4) {
+        if constexpr (TYPE == NVFP4_TYPE_F32) {
+            *reinterpret_cast<float4 *>(static_cast<float *>(p) + at) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+            uint16_t h[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[i] = TYPE == NVFP4_TYPE_F16 ? __half_as_ushort(__float2half_rn(v[i])) : f32_to_bf16_bits(v[i]);
+            uint2 w;
+            memcpy(&w, h, 8);
+            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p) + at) = w;
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < valid) store_from_f32(p, TYPE, at + i, v[i]);
+}
+
+// TYPE: of x, residual and out; FP32 x arrives as FP16 parts.
+template <int TYPE>
+__global__ void __launch_bounds__(kGmThreads, 1)
+    linear_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_s,
+                       const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ GemmArgs a) {
+    constexpr bool kBf16 = TYPE == NVFP4_TYPE_BF16;
+    constexpr int S = kGmStages, R = kGmRawStages;
+    extern __shared__ uint8_t gm_smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(gm_smem_raw) + 1023) & ~uintptr_t(1023));
+    const FusedLinearArgs &f = a.f;
+    uint64_t *b_full = reinterpret_cast<uint64_t *>(smem + kGmOffBars);  // [S] rows of x have landed
+    uint64_t *a_full = b_full + S;                                       // [S] weights are decoded (four warps)
+    uint64_t *empty = a_full + S;                                        // [S] the step's MMAs are done with both
+    uint64_t *raw_full = empty + S;                                      // [R] packed weights and scales have landed
+    uint64_t *raw_empty = raw_full + R;                                  // [R] (eight conversion warps)
+    uint64_t *acc_full = raw_empty + R;                                  // [2]
+    uint64_t *acc_empty = acc_full + 2;                                  // [2] (four epilogue warps)
+    uint64_t *drain = acc_empty + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+    int *acc_ok = reinterpret_cast<int *>(tmem_slot + 1);
+    int *upto = reinterpret_cast<int *>(smem + kGmOffTiles);             // [groups + 1] x tiles of the groups before
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int *err = f.err;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S; ++i) {
+            mbar_init(b_full + i, 1);
+            mbar_init(a_full + i, 4);
+            mbar_init(empty + i, 1);
+        }
+        for (int i = 0; i < R; ++i) {
+            mbar_init(raw_full + i, 1);
+            mbar_init(raw_empty + i, 8);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(acc_full + i, 1);
+            mbar_init(acc_empty + i, 4);
+        }
+        mbar_init(drain, 1);
+        fence_barrier_init();
+        prefetch_tensormap(&tm_w);
+        prefetch_tensormap(&tm_s);
+        prefetch_tensormap(&tm_x);
+    }
+    if (warp == 1) {
+        tc::tmem_alloc(tmem_slot, 512);
+        tc::tmem_relinquish();
+    }
+    if (warp == 2) {
+        const int groups = f.offsets ? f.groups : 1;
+        const int per = (groups + 31) / 32, g0 = min(lane * per, groups), g1 = min(g0 + per, groups);
+        int own = 0;
+        for (int g = g0; g < g1; ++g) {
+            int first, count;
+            group_range(f, g, &first, &count);
+            own += x_tiles(count, a.max_n);
+        }
+        int before = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += v;
+        }
+        if (lane == 31) upto[groups] = before;
+        before -= own;
+        for (int g = g0; g < g1; ++g) {
+            int first, count;
+            group_range(f, g, &first, &count);
+            upto[g] = before;
+            before += x_tiles(count, a.max_n);
+        }
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    const int items = upto[f.offsets ? f.groups : 1] * a.m_tiles;
+    if (warp != 2) pdl_wait();  // the rows that the split kernel wrote; the weights wait for nothing
+
+    if (warp == 0) {
+        // ----------------------------------------------- producer of x
+        if (lane == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+                const Tile t = tile_of(a, upto, item);
+                const int boxes = (t.n + kGmBoxRows - 1) / kGmBoxRows;
+                for (int ks = 0; ks < a.k_steps; ++ks, ++it) {
+                    const int st = it % S;
+                    if (!mbar_wait(empty + st, ((it / S) & 1u) ^ 1u, err, kSiteFusedEmpty)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t *b = smem + kGmOffB + st * kGmStageB;
+                    mbar_arrive_expect_tx(b_full + st, a.terms * boxes * kGmBoxRows * 128);
+                    for (int j = 0; j < a.terms; ++j)
+                        for (int x = 0; x < boxes; ++x)
+                            tma_load_2d(b + (j * a.max_n + x * kGmBoxRows) * 128, &tm_x, b_full + st, ks * 128,
+                                        j * f.vectors + t.row0 + x * kGmBoxRows);
+                }
+            }
+            // After a failure the copies of the last stages issued land before the CTA ends.
+            if (!ok || *reinterpret_cast<volatile int *>(err) != 0)
+                for (uint32_t k = it > (uint32_t)S ? it - S : 0u; k < it; ++k) wait_drain(b_full + k % S, (k / S) & 1u);
+        }
+        __syncwarp();
+    } else if (warp == 2) {
+        // ----------------------------------------- producer of weights
+        if (lane == 0) {
+            uint32_t rt = 0;
+            bool ok = true;
+            for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+                const Tile t = tile_of(a, upto, item);
+                const int w0 = t.group * f.rows + t.m * (f.gated ? 64 : 128), w1 = w0 + (f.gated ? f.out_rows : 64);
+                for (int rs = 0; rs < a.raw_steps; ++rs, ++rt) {
+                    const int st = rt % R;
+                    if (!mbar_wait(raw_empty + st, ((rt / R) & 1u) ^ 1u, err, kSiteFusedRawEmpty)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t *raw = smem + kGmOffRaw + st * kGmRaw;
+                    mbar_arrive_expect_tx(raw_full + st, kGmRaw);
+                    tma_load_2d(raw, &tm_w, raw_full + st, rs * 128, w0);
+                    tma_load_2d(raw + kGmRawBytes / 2, &tm_w, raw_full + st, rs * 128, w1);
+                    tma_load_2d(raw + kGmRawBytes, &tm_s, raw_full + st, rs * 16, w0);
+                    tma_load_2d(raw + kGmRawBytes + kGmRawScales / 2, &tm_s, raw_full + st, rs * 16, w1);
+                }
+            }
+            if (!ok || *reinterpret_cast<volatile int *>(err) != 0)
+                for (uint32_t k = rt > (uint32_t)R ? rt - R : 0u; k < rt; ++k) wait_drain(raw_full + k % R, (k / R) & 1u);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ---------------------------------------------------------- MMA
+        if (lane == 0) {
+            const uint32_t base = smem_u32(smem) + kGmOffB;
+            uint32_t it = 0;
+            bool ok = true;
+            int use = 0;
+            for (int item = blockIdx.x; item < items && ok; item += gridDim.x, ++use) {
+                const Tile t = tile_of(a, upto, item);
+                const uint32_t idesc = tc::idesc_16bit((uint32_t)((t.n + 15) & ~15), kBf16 ? 1u : 0u);
+                const uint32_t buf = use & 1, acc = tmem + buf * kGmMaxN;
+                if (use > 1 && !mbar_wait(acc_empty + buf, ((use >> 1) - 1) & 1u, err, kSiteFusedAccEmpty)) break;
+                tc::fence_after_sync();
+                for (int ks = 0; ks < a.k_steps; ++ks, ++it) {
+                    const int st = it % S;
+                    const uint32_t ph = (it / S) & 1u;
+                    if (!mbar_wait(b_full + st, ph, err, kSiteFusedFull) ||
+                        !mbar_wait(a_full + st, ph, err, kSiteFusedFull)) {
+                        ok = false;
+                        break;
+                    }
+                    tc::fence_after_sync();
+                    for (int j = 0; j < a.terms; ++j) {
+                        const uint32_t b = base + st * kGmStageB + j * a.max_n * 128;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            tc::mma_16bit_ts(acc, tmem + kGmColA + 32 * st + 8 * i, tc::smem_desc_sw128(b + 32 * i), idesc,
+                                             (ks | j | i) != 0 ? 1u : 0u);
+                    }
+                    tc::commit(empty + st);
+                }
+                if (!ok) break;
+                tc::commit(acc_full + buf);
+            }
+            // Every MMA has completed before tensor memory is freed.
+            tc::commit(drain);
+            wait_drain(drain, 0);
+        }
+        __syncwarp();
+    } else if (warp >= kGmConvWarp0 && warp < kGmEpiWarp0) {
+        // --------------------------------------------------- conversion
+        const int half = (warp - kGmConvWarp0) >> 2, quarter = warp & 3;
+        // Row of the raw tile that this lane decodes into its tensor-memory lane.
+        const int row = f.gated ? (lane & 15) + 16 * quarter + (lane >= 16 ? 64 : 0) : 32 * quarter + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16) + kGmColA;
+        uint32_t it = 0, rt = 0;
+        bool ok = true;
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            for (int ks0 = 0; ks0 < a.k_steps && ok; ks0 += 4, ++rt) {
+                const int rs = rt % R;
+                if (!__all_sync(0xffffffffu, mbar_wait(raw_full + rs, (rt / R) & 1u, err, kSiteFusedRawFull))) {
+                    ok = false;
+                    break;
+                }
+                const uint8_t *raw = smem + kGmOffRaw + rs * kGmRaw;
+                const uint4 sc = *reinterpret_cast<const uint4 *>(raw + kGmRawBytes + row * 16);
+                const int steps = min(4, a.k_steps - ks0);
+#pragma unroll
+                for (int jj = 0; jj < 4; jj += 2) {
+                    const int j = jj + half;
+                    if (j >= steps) break;
+                    const uint32_t word = j == 0 ? sc.x : j == 1 ? sc.y : j == 2 ? sc.z : sc.w;
+                    const uint4 q0 = *reinterpret_cast<const uint4 *>(raw + row * 128 + (((2 * j) ^ (row & 7)) << 4));
+                    const uint4 q1 = *reinterpret_cast<const uint4 *>(raw + row * 128 + (((2 * j + 1) ^ (row & 7)) << 4));
+                    uint32_t r[32];
+                    const uint32_t s0 = scale_pair<kBf16>(word, 0), s1 = scale_pair<kBf16>(word, 1);
+                    const uint32_t s2 = scale_pair<kBf16>(word, 2), s3 = scale_pair<kBf16>(word, 3);
+                    decode8<kBf16>(q0.x, s0, r);
+                    decode8<kBf16>(q0.y, s0, r + 4);
+                    decode8<kBf16>(q0.z, s1, r + 8);
+                    decode8<kBf16>(q0.w, s1, r + 12);
+                    decode8<kBf16>(q1.x, s2, r + 16);
+                    decode8<kBf16>(q1.y, s2, r + 20);
+                    decode8<kBf16>(q1.z, s3, r + 24);
+                    decode8<kBf16>(q1.w, s3, r + 28);
+                    const uint32_t step = it + j;
+                    const int st = step % S;
+                    if (!__all_sync(0xffffffffu, mbar_wait(empty + st, ((step / S) & 1u) ^ 1u, err, kSiteFusedEmpty))) {
+                        ok = false;
+                        break;
+                    }
+                    tc::fence_after_sync();
+                    tc::st_32x32b_x32(lanes + 32 * st, r);
+                    tc::wait_st();
+                    tc::fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(a_full + st);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(raw_empty + rs);
+                it += steps;
+            }
+        }
+    } else if (warp >= kGmEpiWarp0) {
+        // ----------------------------------------------------- epilogue
+        const int quarter = warp & 3;
+        const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
+        float *turn = reinterpret_cast<float *>(smem + kGmOffEpi);
+        // Place of this lane's weight row in a turned row of x: gate rows first, the up rows 80 floats on.
+        const int place = !f.gated ? 32 * quarter + lane : lane < 16 ? 16 * quarter + lane : 80 + 16 * quarter + lane - 16;
+        // Outputs of this lane after the turn: four, of one row of x (with a gate 16 lanes cover a row).
+        const int lanes_row = f.gated ? 16 : 32;
+        const int col = 4 * (lane & (lanes_row - 1));
+        const int vec0 = quarter * (f.gated ? 2 : 1) + (f.gated ? lane >> 4 : 0), vec_step = f.gated ? 8 : 4;
+        const int tile_rows = f.gated ? 64 : 128;
+        int use = 0, chunk_no = 0;
+        for (int item = blockIdx.x; item < items; item += gridDim.x, ++use) {
+            const Tile t = tile_of(a, upto, item);
+            const uint32_t buf = use & 1;
+            const int out0 = t.m * tile_rows + col, valid = min(4, f.out_rows - out0);
+            const float inv = f.inv_globals ? __ldg(f.inv_globals + t.group) : f.inv_global;
+            float bias[4] = {0, 0, 0, 0}, bias_up[4] = {0, 0, 0, 0};
+            if (f.bias) {
+                const size_t b = (size_t)t.group * f.rows + out0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (i >= valid) continue;
+                    bias[i] = load_as_f32(f.bias, f.bias_type, b + i);
+                    if (f.gated) bias_up[i] = load_as_f32(f.bias, f.bias_type, b + f.out_rows + i);
+                }
+            }
+            // One thread waits, so that all four warps leave at the same place after a failure.
+            if (threadIdx.x == 32 * kGmEpiWarp0)
+                *acc_ok = mbar_wait(acc_full + buf, (use >> 1) & 1u, err, kSiteFusedAccFull) ? 1 : 0;
+            named_barrier(1, 128);
+            if (!*reinterpret_cast<volatile int *>(acc_ok)) break;
+            tc::fence_after_sync();
+            for (int c0 = 0; c0 < t.n; c0 += 32, ++chunk_no) {
+                float *page = turn + (chunk_no & 1) * (kGmEpiBytes / 4);
+                uint32_t r[32];
+                tc::ld_32x32b_x32(lanes + buf * kGmMaxN + c0, r);
+                tc::wait_ld();
+                if (c0 + 32 >= t.n) {
+                    tc::fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(acc_empty + buf);
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) page[i * kGmEpiPitch + place] = __uint_as_float(r[i]);
+                named_barrier(1, 128);
+                for (int v = vec0; v < min(32, t.n - c0); v += vec_step) {
+                    const long long row = (long long)t.row0 + c0 + v;
+                    const float scale = a.row_scale ? inv * __ldcg(a.row_scale + row) : inv;
+                    const float4 zg = *reinterpret_cast<const float4 *>(page + v * kGmEpiPitch + col);
+                    float z[4] = {zg.x, zg.y, zg.z, zg.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) z[i] = z[i] * scale + bias[i];
+                    if (f.act != NVFP4_ACT_NONE) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) z[i] = activate(z[i], f.act);
+                    }
+                    if (f.gated) {
+                        const float4 zu = *reinterpret_cast<const float4 *>(page + v * kGmEpiPitch + 80 + col);
+                        z[0] *= zu.x * scale + bias_up[0];
+                        z[1] *= zu.y * scale + bias_up[1];
+                        z[2] *= zu.z * scale + bias_up[2];
+                        z[3] *= zu.w * scale + bias_up[3];
+                    }
+                    if (valid <= 0) continue;
+                    if (f.residual) {
+                        float res[4];
+                        load4<TYPE>(f.residual, (size_t)(row * f.residual_stride + out0), a.wide_res, valid, res);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) z[i] += res[i];
+                    }
+                    store4<TYPE>(f.out, (size_t)(row * f.out_stride + out0), a.wide_out, valid, z);
+                }
+            }
+        }
+    }
+    zero_other_rows(f);
+
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        tc::fence_after_sync();
+        tc::tmem_dealloc(tmem, 512);
+    }
+    if (threadIdx.x == 0 && *reinterpret_cast<volatile int *>(err) != 0 && f.host_err) {
+        const int code = *reinterpret_cast<volatile int *>(err);
+        *reinterpret_cast<volatile int *>(f.host_err) = code != 0 ? code : kErrWaitTimeout;
+    }
+}
+
+// ------------------------------------------------------------------ rows of x that TMA cannot read as they are
+
+struct SplitArgs {
+    const void *x;
+    long long x_stride;
+    int type, vectors, cols;
+    uint16_t *parts;    // [2][vectors][cols] FP16 halves of FP32 x, or [vectors][cols] as it is
+    float *row_scale;   // [vectors]
+};
+
+// A CTA per row. FP32: the largest finite value to [2^14, 2^15) by a power of
+// two, then the high half and what it leaves over (linear_gemv.cu's parts).
+__global__ void __launch_bounds__(128) linear_split_kernel(SplitArgs a) {
+    __shared__ uint32_t warp_top[4];
+    pdl_launch_dependents();
+    const int row = blockIdx.x;
+    const size_t to = (size_t)row * a.cols;
+    if (a.type != NVFP4_TYPE_F32) {
+        const uint16_t *x = static_cast<const uint16_t *>(a.x) + row * a.x_stride;
+        for (int c = threadIdx.x; c < a.cols; c += blockDim.x) a.parts[to + c] = x[c];
+        return;
+    }
+    const float *x = static_cast<const float *>(a.x) + row * a.x_stride;
+    float m = 0.0f;
+    for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
+        const float v = fabsf(x[c]);
+        if (v <= 3.402823466e38f) m = fmaxf(m, v);
+    }
+    uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+    if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = max(max(warp_top[0], warp_top[1]), max(warp_top[2], warp_top[3]));
+    const int e = top ? max((int)(top >> 23) - 127, -112) : 14;
+    const float scale = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+    if (threadIdx.x == 0) a.row_scale[row] = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+    uint16_t *low = a.parts + (size_t)a.vectors * a.cols;
+    for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
+        const float y = x[c] * scale;
+        const __half h = __float2half_rn(y);
+        a.parts[to + c] = __half_as_ushort(h);
+        low[to + c] = __half_as_ushort(__float2half_rn(fabsf(y) <= 65504.0f ? y - __half2float(h) : 0.0f));
+    }
+}
+
+// TMA reads 16-bit rows in place when their addresses and stride are multiples of 16 bytes.
+bool in_place(int type, const void *x, long long x_stride, int cols) {
+    return type != NVFP4_TYPE_F32 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && x_stride % 8 == 0 && x_stride >= cols;
+}
+
+size_t parts_bytes(int type, int vectors, int cols) {
+    return ((size_t)vectors * cols * (type == NVFP4_TYPE_F32 ? 4 : 2) + 255) & ~size_t(255);
+}
+
+template <int TYPE>
+void launch(const GemmArgs &g, const nvfp4_matrix &matrix, const CUtensorMap &map_x, int grid, bool dependent,
+            cudaStream_t stream) {
+    check_cuda(cudaFuncSetAttribute(linear_gemm_kernel<TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    static_cast<int>(kGmSmem)),
+               "cudaFuncSetAttribute(linear_gemm_kernel)");
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kGmThreads);
+    cfg.dynamicSmemBytes = kGmSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = dependent ? 1 : 0;
+    check_cuda(cudaLaunchKernelEx(&cfg, linear_gemm_kernel<TYPE>, matrix.map_w, matrix.map_s, map_x, g),
+               "linear_gemm_kernel");
+}
+
+}  // namespace
+
+size_t linear_gemm_workspace(int type, const void *x, long long x_stride, int vectors, int cols) {
+    if (in_place(type, x, x_stride, cols)) return 0;
+    return parts_bytes(type, vectors, cols) + (type == NVFP4_TYPE_F32 ? sizeof(float) * (size_t)vectors : 0);
+}
+
+void launch_linear_gemm(const FusedLinearArgs &f, const nvfp4_matrix &matrix, void *workspace, int sm_count,
+                        cudaStream_t stream) {
+    GemmArgs g{};
+    g.f = f;
+    g.terms = f.type == NVFP4_TYPE_F32 ? 2 : 1;
+    g.max_n = kGmMaxN / g.terms;
+    g.m_tiles = f.gated ? (f.out_rows + 63) / 64 : (f.rows + 127) / 128;
+    g.k_steps = (f.cols + 63) / 64;
+    g.raw_steps = (f.cols + 255) / 256;
+    const int e = f.type == NVFP4_TYPE_F32 ? 4 : 2;
+    auto vectors_of_4 = [&](const void *p, long long stride) {
+        return (reinterpret_cast<uintptr_t>(p) % (4 * e)) == 0 && stride % 4 == 0 ? 1 : 0;
+    };
+    g.wide_out = vectors_of_4(f.out, f.out_stride);
+    g.wide_res = f.residual ? vectors_of_4(f.residual, f.residual_stride) : 0;
+    const bool direct = in_place(f.type, f.x, f.x_stride, f.cols);
+    const void *rows = f.x;
+    long long stride = f.x_stride;
+    if (!direct) {
+        SplitArgs s{};
+        s.x = f.x;
+        s.x_stride = f.x_stride;
+        s.type = f.type;
+        s.vectors = f.vectors;
+        s.cols = f.cols;
+        s.parts = static_cast<uint16_t *>(workspace);
+        if (f.type == NVFP4_TYPE_F32)
+            s.row_scale = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + parts_bytes(f.type, f.vectors, f.cols));
+        g.row_scale = s.row_scale;
+        linear_split_kernel<<<f.vectors, 128, 0, stream>>>(s);
+        check_cuda(cudaGetLastError(), "linear_split_kernel");
+        rows = workspace;
+        stride = f.cols;
+    }
+    CUtensorMap map_x;
+    check_cuda(make_tensor_map_u8(&map_x, rows, (uint64_t)f.cols * 2, (uint64_t)stride * 2,
+                                  (uint64_t)f.vectors * (direct ? 1 : g.terms), 128, kGmBoxRows,
+                                  CU_TENSOR_MAP_SWIZZLE_128B),
+               "cuTensorMapEncodeTiled(rows of x)");
+    // Items the call can have: every group may end inside a tile.
+    const long long x_tiles_most = (f.vectors + g.max_n - 1) / g.max_n + (f.offsets ? std::min(f.groups, f.vectors) : 0);
+    const int grid = static_cast<int>(std::min<long long>(sm_count, x_tiles_most * g.m_tiles));
+    if (f.type == NVFP4_TYPE_BF16) launch<NVFP4_TYPE_BF16>(g, matrix, map_x, grid, !direct, stream);
+    else if (f.type == NVFP4_TYPE_F16) launch<NVFP4_TYPE_F16>(g, matrix, map_x, grid, !direct, stream);
+    else launch<NVFP4_TYPE_F32>(g, matrix, map_x, grid, !direct, stream);
+}
+
+}  // namespace nvfp4

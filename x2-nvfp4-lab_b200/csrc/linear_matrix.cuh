@@ -5,6 +5,7 @@
 
 #include "internal.h"
 #include "linear_tc.cuh"
+#include "tma_util.cuh"
 
 struct nvfp4_matrix {
     nvfp4_runtime *runtime = nullptr;
@@ -18,7 +19,8 @@ struct nvfp4_matrix {
     float inv_global = 0.0f;     // of a matrix uploaded on its own
     float *inv_globals = nullptr;          // device [groups], of a grouped upload (NULL otherwise)
     nvfp4::LinearTcState tc;               // FP32 tensor-core path (not of a grouped upload): scale atoms, terms, maps
-    CUtensorMap map_packed;                // grouped upload: packed rows, box 128 B x 128 rows, 128-byte swizzle
+    CUtensorMap map_w;                     // packed rows: box 128 B x 64 rows, 128-byte swizzle (linear_gemm.cu)
+    CUtensorMap map_s;                     // scale rows: box 16 B x 64 rows
     volatile int *host_err = nullptr;      // pinned, device-mapped wait-timeout word (read at synchronize)
 
     // Whether nvfp4_linear_* (FP32, no epilogue) can run it.
@@ -36,6 +38,17 @@ struct nvfp4_matrix {
 namespace nvfp4 {
 
 constexpr int kLinMaxCols = 49152;
+
+// The tensor maps of a matrix whose arrays are allocated.
+inline void make_matrix_maps(nvfp4_matrix &m) {
+    const uint64_t rows = static_cast<uint64_t>(m.groups) * m.rows;
+    check_cuda(make_tensor_map_u8(&m.map_w, m.packed, m.packed_pitch, m.packed_pitch, rows, 128, 64,
+                                  CU_TENSOR_MAP_SWIZZLE_128B),
+               "cuTensorMapEncodeTiled(packed)");
+    check_cuda(make_tensor_map_u8(&m.map_s, m.scales, m.scale_pitch, m.scale_pitch, rows, 16, 64,
+                                  CU_TENSOR_MAP_SWIZZLE_NONE),
+               "cuTensorMapEncodeTiled(scales)");
+}
 constexpr int kLinMaxGroups = 1024;
 
 }  // namespace nvfp4

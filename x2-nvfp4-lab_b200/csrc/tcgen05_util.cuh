@@ -99,6 +99,23 @@ __device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uin
         : "memory");
 }
 
+// Instruction descriptor of kind::f16 with both operands FP16 (bf16 = 0) or
+// BF16 (1), FP32 accumulation, K-major, M = 128 and N = `n`.
+__device__ __forceinline__ uint32_t idesc_16bit(uint32_t n, uint32_t bf16) {
+    return (1u << 4) | (bf16 << 7) | (bf16 << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// D[tmem d] (+)= A[tmem a] * B[smem b]^T, 16-bit operands (K 16 per
+// instruction): A is 128 lanes x 8 columns, two consecutive K per column.
+__device__ __forceinline__ void mma_16bit_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 // D[tmem d] (+)= A[smem a] * B[smem b]^T with per-16 block scales read from
 // tensor memory at `sfa` and `sfb`. Issued by one thread.
 __device__ __forceinline__ void mma_mxf4nvf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,

@@ -38,6 +38,17 @@ def _checks(matrix, x, bias, activation, tensors):
     return matrix.rows // 2 if activation and activation.endswith("_mul") else matrix.rows
 
 
+def _workspace(rt, matrix, x, grouped):
+    """(tensor, address, bytes) of the call's device workspace, from torch's allocator on the current stream. The
+    tensor is held until the kernels are enqueued; its memory then goes to later work of the same stream."""
+    size = rt.lib.nvfp4_linear_workspace_bytes(matrix.handle, x.data_ptr(), TYPES[x.dtype], _row_stride(x), x.shape[0],
+                                               grouped)
+    if not size:
+        return None, None, 0
+    held = torch.empty(size, dtype=torch.uint8, device=x.device)
+    return held, held.data_ptr(), size
+
+
 def linear_fused(rt, matrix, x, bias, activation, residual, out, stream):
     width = _checks(matrix, x, bias, activation, (("bias", bias), ("residual", residual), ("out", out)))
     _require(matrix.groups == 1, "a matrix of several groups runs through linear_grouped")
@@ -62,12 +73,13 @@ def linear_fused(rt, matrix, x, bias, activation, residual, out, stream):
             return y
         r2 = _rows_of(residual.reshape(-1, width)) if residual is not None else None
         b = bias.contiguous() if bias is not None else None
+        _held, space, size = _workspace(rt, matrix, x2, 0)
         rt._check(
             rt.lib.nvfp4_linear_fused(
                 rt.handle, matrix.handle, x2.data_ptr(), TYPES[x.dtype], _row_stride(x2), x2.shape[0],
                 b.data_ptr() if b is not None else None, TYPES[b.dtype] if b is not None else 0,
                 ACTIVATIONS[activation], r2.data_ptr() if r2 is not None else None,
-                _row_stride(r2) if r2 is not None else 0, y2.data_ptr(), _row_stride(y2),
+                _row_stride(r2) if r2 is not None else 0, y2.data_ptr(), _row_stride(y2), space, size,
                 _stream_handle(torch.cuda.current_stream(x.device))),
             "nvfp4_linear_fused")
         return y
@@ -92,11 +104,12 @@ def linear_grouped(rt, matrix, x, offsets, bias, activation, out, stream):
             return y
         x2, o = _rows_of(x), offsets.contiguous()
         b = bias.contiguous() if bias is not None else None
+        _held, space, size = _workspace(rt, matrix, x2, 1)
         rt._check(
             rt.lib.nvfp4_linear_grouped(
                 rt.handle, matrix.handle, x2.data_ptr(), TYPES[x.dtype], _row_stride(x2), shape[0], o.data_ptr(),
                 b.data_ptr() if b is not None else None, TYPES[b.dtype] if b is not None else 0,
-                ACTIVATIONS[activation], y.data_ptr(), _row_stride(y), 1 if out is None else 0,
+                ACTIVATIONS[activation], y.data_ptr(), _row_stride(y), 1 if out is None else 0, space, size,
                 _stream_handle(torch.cuda.current_stream(x.device))),
             "nvfp4_linear_grouped")
         return y

@@ -192,10 +192,11 @@ _SIGNATURES: dict[str, tuple[list, object]] = {
          C.POINTER(C.c_void_p)], C.c_int),
     "nvfp4_linear_fused": (
         [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p,
-         C.c_int64, C.c_void_p, C.c_int64, C.c_void_p], C.c_int),
+         C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p], C.c_int),
+    "nvfp4_linear_workspace_bytes": ([C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int], C.c_size_t),
     "nvfp4_linear_grouped": (
         [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
-         C.c_void_p, C.c_int64, C.c_int, C.c_void_p], C.c_int),
+         C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p], C.c_int),
     "nvfp4_expert_sort_workspace_bytes": ([C.c_int, C.c_int, C.c_int], C.c_size_t),
     "nvfp4_expert_sort": (
         [C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_int,
