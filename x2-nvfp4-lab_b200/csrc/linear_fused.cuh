@@ -58,14 +58,26 @@ __device__ __forceinline__ void store_from_f32(void *p, int type, size_t i, floa
             type == NVFP4_TYPE_F16 ? __half_as_ushort(__float2half_rn(v)) : f32_to_bf16_bits(v);
 }
 
+// exp and the division are the fast ones: a few units of 2^-23 of the
+// exponential, which is at most 2^-21 of z in the result.
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+    if constexpr (ACT == NVFP4_ACT_RELU) return z < 0.0f ? 0.0f : z;  // NaN stays NaN
+    if constexpr (ACT == NVFP4_ACT_SILU) return __fdividef(z, 1.0f + __expf(-z));
+    // z Phi(z); erfc keeps the small tail of negative z that 1 + erf rounds away.
+    if constexpr (ACT == NVFP4_ACT_GELU) return 0.5f * z * erfcf(-0.70710678118654752f * z);
+    // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u)), u = sqrt(2 / pi) (z + 0.044715 z^3).
+    if constexpr (ACT == NVFP4_ACT_GELU_TANH)
+        return __fdividef(z, 1.0f + __expf(-1.5957691216057308f * fmaf(0.044715f * z * z, z, z)));
+    return z;
+}
+
 __device__ __forceinline__ float activate(float z, int act) {
     switch (act) {
-        case NVFP4_ACT_RELU: return z < 0.0f ? 0.0f : z;  // NaN stays NaN
-        case NVFP4_ACT_SILU: return z / (1.0f + expf(-z));
-        // z Phi(z); erfc keeps the small tail of negative z that 1 + erf rounds away.
-        case NVFP4_ACT_GELU: return 0.5f * z * erfcf(-0.70710678118654752f * z);
-        // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u)), u = sqrt(2 / pi) (z + 0.044715 z^3).
-        case NVFP4_ACT_GELU_TANH: return z / (1.0f + expf(-1.5957691216057308f * (z + 0.044715f * z * z * z)));
+        case NVFP4_ACT_RELU: return activate<NVFP4_ACT_RELU>(z);
+        case NVFP4_ACT_SILU: return activate<NVFP4_ACT_SILU>(z);
+        case NVFP4_ACT_GELU: return activate<NVFP4_ACT_GELU>(z);
+        case NVFP4_ACT_GELU_TANH: return activate<NVFP4_ACT_GELU_TANH>(z);
         default: return z;
     }
 }

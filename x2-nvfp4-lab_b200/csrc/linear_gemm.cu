@@ -11,19 +11,26 @@
 // loaded by TMA. With a gate the tile is 64 gate and 64 up rows, 16 of each in
 // every lane quarter.
 //
-// Warps: 0 producer of x and 2 of weights (TMA), 1 MMA issuer, 4-11 conversion (two warpgroups, every
-// other 64-column step each), 12-15 epilogue. Tensor memory: two accumulators
-// of 192 columns, and four decoded steps of 32. The epilogue turns 32 columns
-// at a time through shared memory, so that a lane has four consecutive outputs
-// of one row of x: bias in registers, residual and stores as vectors.
+// Warps: 0 producer of x and 2 of weights (TMA), 1 MMA issuer, 4-15 conversion
+// (three warpgroups, every third 64-column step each), 16-23 epilogue (two
+// warpgroups, every other 32 columns each). Tensor memory: two accumulators of
+// 192 columns, and four decoded steps of 32. The epilogue turns 32 columns at
+// a time through shared memory, so that a lane has four consecutive outputs of
+// one row of x: bias in registers, residual and stores as vectors.
 //
 // One persistent CTA per SM walks (group, weight tile, x tile) items; x tiles of
 // a group are of even size, and items of one weight tile are neighbours, so
 // that its bytes come from HBM once.
 //
+// An MMA (128 x N x 16, A in tensor memory) takes N / 2 + 10 cycles, measured;
+// with A in shared memory N / 2 + 43.
+//
 // FP32 x enters as two FP16 halves, scaled per row by a power of two
 // (linear_gemv.cu has the error), split by a kernel before; x that TMA cannot
-// read (16-byte addresses and strides) is copied by the same kernel.
+// read (16-byte addresses and strides) is copied by the same kernel. For FP32
+// the sums move to FP32 registers of the epilogue every 256 columns: the tensor
+// core rounds its running sum towards zero, and the bias of a long chain would
+// show.
 #include "linear_fused.cuh"
 #include "tcgen05_util.cuh"
 #include "tma_util.cuh"
@@ -34,11 +41,13 @@
 namespace nvfp4 {
 namespace {
 
-constexpr int kGmThreads = 512;
-constexpr int kGmConvWarp0 = 4, kGmEpiWarp0 = 12;
+constexpr int kGmConvWarp0 = 4, kGmConvGroups = 3, kGmEpiWarp0 = kGmConvWarp0 + 4 * kGmConvGroups;
+constexpr int kGmEpiGroups = 2;
+constexpr int kGmThreads = 32 * (kGmEpiWarp0 + 4 * kGmEpiGroups);
 constexpr int kGmStages = 4;                        // 64-column steps in flight
 constexpr int kGmMaxN = 192;
-constexpr int kGmBoxRows = 32;                      // rows of x per TMA box
+constexpr int kGmMaxN32 = 64;                       // of split FP32 x: one 32-column piece per epilogue warpgroup
+constexpr int kGmSegment32 = 4;                     // its steps per accumulator
 constexpr int kGmStageB = kGmMaxN * 128;            // a step of x: up to 192 rows x 64 columns
 constexpr int kGmRawStages = 3;                     // 256 columns of packed weights each
 constexpr int kGmRawBytes = 128 * 128;
@@ -50,11 +59,11 @@ constexpr int kGmColA = 2 * kGmMaxN;                // tensor-memory column of t
 constexpr int kGmOffB = 0;
 constexpr int kGmOffRaw = kGmOffB + kGmStages * kGmStageB;
 constexpr int kGmOffEpi = kGmOffRaw + kGmRawStages * kGmRaw;
-constexpr int kGmOffBars = kGmOffEpi + 2 * kGmEpiBytes;
+constexpr int kGmOffBars = kGmOffEpi + kGmEpiGroups * kGmEpiBytes;
 constexpr int kGmBars = 2 * kGmStages + kGmStages + 2 * kGmRawStages + 2 + 2 + 1;
-constexpr int kGmOffTiles = kGmOffBars + kGmBars * 8 + 16;
+constexpr int kGmOffTiles = kGmOffBars + kGmBars * 8 + 24;
 constexpr size_t kGmSmem = 1024 + kGmOffTiles + sizeof(int) * (kLinMaxGroups + 1);
-static_assert(kGmSmem <= 232448, "shared memory overflow");
+static_assert(kGmOffTiles % 4 == 0 && kGmSmem <= 232448, "shared memory overflow");
 static_assert(kGmColA + 32 * kGmStages <= 512, "tensor memory overflow");
 static_assert(kGmRawBytes % 1024 == 0 && kGmOffRaw % 1024 == 0 && kGmRaw % 1024 == 0, "swizzled tiles need 1024-byte alignment");
 
@@ -72,6 +81,8 @@ struct GemmArgs {
     const float *row_scale;  // [vectors] of split FP32 x (NULL: ones)
     int terms;               // 16-bit parts of x
     int max_n;               // rows of x per tile
+    int box_rows;            // rows of x per TMA box
+    int segment;             // steps per accumulator
     int m_tiles;             // weight tiles of a group
     int raw_steps;           // 256-column steps over K
     int k_steps;             // 64-column steps over K
@@ -192,6 +203,38 @@ __device__ __forceinline__ void store4(void *p, size_t at, bool wide, int valid,
         if (i < valid) store_from_f32(p, TYPE, at + i, v[i]);
 }
 
+// A turned page of up to 32 rows of x: scale, bias, activation, gate, residual, store. Lane: four outputs from `out0`.
+template <int TYPE, int ACT>
+__device__ __forceinline__ void finish_page(const GemmArgs &a, const float *page, int row0, int n, int first, int step,
+                                            int col, int out0, int valid, float inv, const float (&bias)[4],
+                                            const float (&bias_up)[4]) {
+    const FusedLinearArgs &f = a.f;
+    if (valid <= 0) return;
+#pragma unroll 4
+    for (int v = first; v < n; v += step) {
+        const long long row = (long long)row0 + v;
+        const float scale = a.row_scale ? inv * __ldcg(a.row_scale + row) : inv;
+        const float4 zg = *reinterpret_cast<const float4 *>(page + v * kGmEpiPitch + col);
+        float z[4] = {zg.x, zg.y, zg.z, zg.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[i] = activate<ACT>(fmaf(z[i], scale, bias[i]));
+        if (f.gated) {
+            const float4 zu = *reinterpret_cast<const float4 *>(page + v * kGmEpiPitch + 80 + col);
+            z[0] *= fmaf(zu.x, scale, bias_up[0]);
+            z[1] *= fmaf(zu.y, scale, bias_up[1]);
+            z[2] *= fmaf(zu.z, scale, bias_up[2]);
+            z[3] *= fmaf(zu.w, scale, bias_up[3]);
+        }
+        if (f.residual) {
+            float res[4];
+            load4<TYPE>(f.residual, (size_t)(row * f.residual_stride + out0), a.wide_res, valid, res);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[i] += res[i];
+        }
+        store4<TYPE>(f.out, (size_t)(row * f.out_stride + out0), a.wide_out, valid, z);
+    }
+}
+
 // TYPE: of x, residual and out; FP32 x arrives as FP16 parts.
 template <int TYPE>
 __global__ void __launch_bounds__(kGmThreads, 1)
@@ -206,12 +249,12 @@ __global__ void __launch_bounds__(kGmThreads, 1)
     uint64_t *a_full = b_full + S;                                       // [S] weights are decoded (four warps)
     uint64_t *empty = a_full + S;                                        // [S] the step's MMAs are done with both
     uint64_t *raw_full = empty + S;                                      // [R] packed weights and scales have landed
-    uint64_t *raw_empty = raw_full + R;                                  // [R] (eight conversion warps)
+    uint64_t *raw_empty = raw_full + R;                                  // [R] (every conversion warp)
     uint64_t *acc_full = raw_empty + R;                                  // [2]
-    uint64_t *acc_empty = acc_full + 2;                                  // [2] (four epilogue warps)
+    uint64_t *acc_empty = acc_full + 2;                                  // [2] (every epilogue warp)
     uint64_t *drain = acc_empty + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
-    int *acc_ok = reinterpret_cast<int *>(tmem_slot + 1);
+    int *acc_ok = reinterpret_cast<int *>(tmem_slot + 1);                // [epilogue warpgroups]
     int *upto = reinterpret_cast<int *>(smem + kGmOffTiles);             // [groups + 1] x tiles of the groups before
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int *err = f.err;
@@ -224,11 +267,11 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         }
         for (int i = 0; i < R; ++i) {
             mbar_init(raw_full + i, 1);
-            mbar_init(raw_empty + i, 8);
+            mbar_init(raw_empty + i, 4 * kGmConvGroups);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(acc_full + i, 1);
-            mbar_init(acc_empty + i, 4);
+            mbar_init(acc_empty + i, 4 * kGmEpiGroups);
         }
         mbar_init(drain, 1);
         fence_barrier_init();
@@ -267,109 +310,123 @@ __global__ void __launch_bounds__(kGmThreads, 1)
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     const int items = upto[f.offsets ? f.groups : 1] * a.m_tiles;
     if (warp != 2) pdl_wait();  // the rows that the split kernel wrote; the weights wait for nothing
 
     if (warp == 0) {
         // ----------------------------------------------- producer of x
-        if (lane == 0) {
-            uint32_t it = 0;
-            bool ok = true;
-            for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-                const Tile t = tile_of(a, upto, item);
-                const int boxes = (t.n + kGmBoxRows - 1) / kGmBoxRows;
-                for (int ks = 0; ks < a.k_steps; ++ks, ++it) {
-                    const int st = it % S;
-                    if (!mbar_wait(empty + st, ((it / S) & 1u) ^ 1u, err, kSiteFusedEmpty)) {
-                        ok = false;
-                        break;
-                    }
-                    uint8_t *b = smem + kGmOffB + st * kGmStageB;
-                    mbar_arrive_expect_tx(b_full + st, a.terms * boxes * kGmBoxRows * 128);
+        uint32_t it = 0;
+        bool ok = true;
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            const Tile t = tile_of(a, upto, item);
+            const int boxes = (t.n + a.box_rows - 1) / a.box_rows;
+            for (int ks = 0; ks < a.k_steps; ++ks, ++it) {
+                const int st = it % S;
+                if (!__all_sync(0xffffffffu, mbar_wait(empty + st, ((it / S) & 1u) ^ 1u, err, kSiteFusedEmpty))) {
+                    ok = false;
+                    break;
+                }
+                uint8_t *b = smem + kGmOffB + st * kGmStageB;
+                if (tc::elect_one()) {
+                    mbar_arrive_expect_tx(b_full + st, a.terms * boxes * a.box_rows * 128);
                     for (int j = 0; j < a.terms; ++j)
                         for (int x = 0; x < boxes; ++x)
-                            tma_load_2d(b + (j * a.max_n + x * kGmBoxRows) * 128, &tm_x, b_full + st, ks * 128,
-                                        j * f.vectors + t.row0 + x * kGmBoxRows);
+                            tma_load_2d(b + (j * a.max_n + x * a.box_rows) * 128, &tm_x, b_full + st, ks * 128,
+                                        j * f.vectors + t.row0 + x * a.box_rows);
                 }
+                __syncwarp();
             }
-            // After a failure the copies of the last stages issued land before the CTA ends.
-            if (!ok || *reinterpret_cast<volatile int *>(err) != 0)
-                for (uint32_t k = it > (uint32_t)S ? it - S : 0u; k < it; ++k) wait_drain(b_full + k % S, (k / S) & 1u);
         }
+        // After a failure the copies of the last stages issued land before the CTA ends.
+        if (!ok || *reinterpret_cast<volatile int *>(err) != 0)
+            for (uint32_t k = it > (uint32_t)S ? it - S : 0u; k < it; ++k) wait_drain(b_full + k % S, (k / S) & 1u);
         __syncwarp();
     } else if (warp == 2) {
         // ----------------------------------------- producer of weights
-        if (lane == 0) {
-            uint32_t rt = 0;
-            bool ok = true;
-            for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-                const Tile t = tile_of(a, upto, item);
-                const int w0 = t.group * f.rows + t.m * (f.gated ? 64 : 128), w1 = w0 + (f.gated ? f.out_rows : 64);
-                for (int rs = 0; rs < a.raw_steps; ++rs, ++rt) {
-                    const int st = rt % R;
-                    if (!mbar_wait(raw_empty + st, ((rt / R) & 1u) ^ 1u, err, kSiteFusedRawEmpty)) {
-                        ok = false;
-                        break;
-                    }
-                    uint8_t *raw = smem + kGmOffRaw + st * kGmRaw;
+        uint32_t rt = 0;
+        bool ok = true;
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            const Tile t = tile_of(a, upto, item);
+            const int w0 = t.group * f.rows + t.m * (f.gated ? 64 : 128), w1 = w0 + (f.gated ? f.out_rows : 64);
+            for (int rs = 0; rs < a.raw_steps; ++rs, ++rt) {
+                const int st = rt % R;
+                if (!__all_sync(0xffffffffu, mbar_wait(raw_empty + st, ((rt / R) & 1u) ^ 1u, err, kSiteFusedRawEmpty))) {
+                    ok = false;
+                    break;
+                }
+                uint8_t *raw = smem + kGmOffRaw + st * kGmRaw;
+                if (tc::elect_one()) {
                     mbar_arrive_expect_tx(raw_full + st, kGmRaw);
                     tma_load_2d(raw, &tm_w, raw_full + st, rs * 128, w0);
                     tma_load_2d(raw + kGmRawBytes / 2, &tm_w, raw_full + st, rs * 128, w1);
                     tma_load_2d(raw + kGmRawBytes, &tm_s, raw_full + st, rs * 16, w0);
                     tma_load_2d(raw + kGmRawBytes + kGmRawScales / 2, &tm_s, raw_full + st, rs * 16, w1);
                 }
+                __syncwarp();
             }
-            if (!ok || *reinterpret_cast<volatile int *>(err) != 0)
-                for (uint32_t k = rt > (uint32_t)R ? rt - R : 0u; k < rt; ++k) wait_drain(raw_full + k % R, (k / R) & 1u);
         }
+        if (!ok || *reinterpret_cast<volatile int *>(err) != 0)
+            for (uint32_t k = rt > (uint32_t)R ? rt - R : 0u; k < rt; ++k) wait_drain(raw_full + k % R, (k / R) & 1u);
         __syncwarp();
     } else if (warp == 1) {
         // ---------------------------------------------------------- MMA
-        if (lane == 0) {
-            const uint32_t base = smem_u32(smem) + kGmOffB;
-            uint32_t it = 0;
-            bool ok = true;
-            int use = 0;
-            for (int item = blockIdx.x; item < items && ok; item += gridDim.x, ++use) {
-                const Tile t = tile_of(a, upto, item);
-                const uint32_t idesc = tc::idesc_16bit((uint32_t)((t.n + 15) & ~15), kBf16 ? 1u : 0u);
+        const uint32_t base = smem_u32(smem) + kGmOffB;
+        uint32_t it = 0;
+        bool ok = true;
+        int use = 0;  // accumulators filled so far
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            const Tile t = tile_of(a, upto, item);
+            const uint32_t idesc = tc::idesc_16bit((uint32_t)((t.n + 15) & ~15), kBf16 ? 1u : 0u);
+            int left = 0;
+            for (int ks = 0; ks < a.k_steps; ++ks, ++it) {
                 const uint32_t buf = use & 1, acc = tmem + buf * kGmMaxN;
-                if (use > 1 && !mbar_wait(acc_empty + buf, ((use >> 1) - 1) & 1u, err, kSiteFusedAccEmpty)) break;
-                tc::fence_after_sync();
-                for (int ks = 0; ks < a.k_steps; ++ks, ++it) {
-                    const int st = it % S;
-                    const uint32_t ph = (it / S) & 1u;
-                    if (!mbar_wait(b_full + st, ph, err, kSiteFusedFull) ||
-                        !mbar_wait(a_full + st, ph, err, kSiteFusedFull)) {
+                const bool fresh = left == 0;
+                if (fresh) {
+                    left = min(a.segment, a.k_steps - ks);
+                    if (use > 1 &&
+                        !__all_sync(0xffffffffu, mbar_wait(acc_empty + buf, ((use >> 1) - 1) & 1u, err, kSiteFusedAccEmpty))) {
                         ok = false;
                         break;
                     }
-                    tc::fence_after_sync();
+                }
+                const int st = it % S;
+                const uint32_t ph = (it / S) & 1u;
+                if (!__all_sync(0xffffffffu, mbar_wait(b_full + st, ph, err, kSiteFusedFull)) ||
+                    !__all_sync(0xffffffffu, mbar_wait(a_full + st, ph, err, kSiteFusedFull))) {
+                    ok = false;
+                    break;
+                }
+                tc::fence_after_sync();
+                --left;
+                if (tc::elect_one()) {
                     for (int j = 0; j < a.terms; ++j) {
                         const uint32_t b = base + st * kGmStageB + j * a.max_n * 128;
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             tc::mma_16bit_ts(acc, tmem + kGmColA + 32 * st + 8 * i, tc::smem_desc_sw128(b + 32 * i), idesc,
-                                             (ks | j | i) != 0 ? 1u : 0u);
+                                             fresh && (j | i) == 0 ? 0u : 1u);
                     }
                     tc::commit(empty + st);
+                    if (left == 0) tc::commit(acc_full + buf);
                 }
-                if (!ok) break;
-                tc::commit(acc_full + buf);
+                __syncwarp();
+                if (left == 0) ++use;
             }
-            // Every MMA has completed before tensor memory is freed.
-            tc::commit(drain);
-            wait_drain(drain, 0);
         }
+        // Every MMA has completed before tensor memory is freed.
+        if (tc::elect_one()) tc::commit(drain);
+        __syncwarp();
+        wait_drain(drain, 0);
         __syncwarp();
     } else if (warp >= kGmConvWarp0 && warp < kGmEpiWarp0) {
         // --------------------------------------------------- conversion
-        const int half = (warp - kGmConvWarp0) >> 2, quarter = warp & 3;
+        const uint32_t mine = (warp - kGmConvWarp0) >> 2;  // steps it with it % groups == mine
+        const int quarter = warp & 3;
         // Row of the raw tile that this lane decodes into its tensor-memory lane.
         const int row = f.gated ? (lane & 15) + 16 * quarter + (lane >= 16 ? 64 : 0) : 32 * quarter + lane;
         const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16) + kGmColA;
-        uint32_t it = 0, rt = 0;
+        uint32_t it = 0, rt = 0, next = mine;
         bool ok = true;
         for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
             for (int ks0 = 0; ks0 < a.k_steps && ok; ks0 += 4, ++rt) {
@@ -379,13 +436,10 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                     break;
                 }
                 const uint8_t *raw = smem + kGmOffRaw + rs * kGmRaw;
-                const uint4 sc = *reinterpret_cast<const uint4 *>(raw + kGmRawBytes + row * 16);
-                const int steps = min(4, a.k_steps - ks0);
-#pragma unroll
-                for (int jj = 0; jj < 4; jj += 2) {
-                    const int j = jj + half;
-                    if (j >= steps) break;
-                    const uint32_t word = j == 0 ? sc.x : j == 1 ? sc.y : j == 2 ? sc.z : sc.w;
+                const uint32_t end = it + min(4, a.k_steps - ks0);
+                for (; next < end; next += kGmConvGroups) {
+                    const int j = next - it;
+                    const uint32_t word = *reinterpret_cast<const uint32_t *>(raw + kGmRawBytes + row * 16 + 4 * j);
                     const uint4 q0 = *reinterpret_cast<const uint4 *>(raw + row * 128 + (((2 * j) ^ (row & 7)) << 4));
                     const uint4 q1 = *reinterpret_cast<const uint4 *>(raw + row * 128 + (((2 * j + 1) ^ (row & 7)) << 4));
                     uint32_t r[32];
@@ -399,9 +453,8 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                     decode8<kBf16>(q1.y, s2, r + 20);
                     decode8<kBf16>(q1.z, s3, r + 24);
                     decode8<kBf16>(q1.w, s3, r + 28);
-                    const uint32_t step = it + j;
-                    const int st = step % S;
-                    if (!__all_sync(0xffffffffu, mbar_wait(empty + st, ((step / S) & 1u) ^ 1u, err, kSiteFusedEmpty))) {
+                    const int st = next % S;
+                    if (!__all_sync(0xffffffffu, mbar_wait(empty + st, ((next / S) & 1u) ^ 1u, err, kSiteFusedEmpty))) {
                         ok = false;
                         break;
                     }
@@ -414,14 +467,14 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(raw_empty + rs);
-                it += steps;
+                it = end;
             }
         }
     } else if (warp >= kGmEpiWarp0) {
         // ----------------------------------------------------- epilogue
-        const int quarter = warp & 3;
+        const int piece = (warp - kGmEpiWarp0) >> 2, quarter = warp & 3;
         const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
-        float *turn = reinterpret_cast<float *>(smem + kGmOffEpi);
+        float *page = reinterpret_cast<float *>(smem + kGmOffEpi + piece * kGmEpiBytes);
         // Place of this lane's weight row in a turned row of x: gate rows first, the up rows 80 floats on.
         const int place = !f.gated ? 32 * quarter + lane : lane < 16 ? 16 * quarter + lane : 80 + 16 * quarter + lane - 16;
         // Outputs of this lane after the turn: four, of one row of x (with a gate 16 lanes cover a row).
@@ -429,10 +482,24 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         const int col = 4 * (lane & (lanes_row - 1));
         const int vec0 = quarter * (f.gated ? 2 : 1) + (f.gated ? lane >> 4 : 0), vec_step = f.gated ? 8 : 4;
         const int tile_rows = f.gated ? 64 : 128;
-        int use = 0, chunk_no = 0;
-        for (int item = blockIdx.x; item < items; item += gridDim.x, ++use) {
+        int use = 0;
+        // One thread waits, so that the four warps leave at the same place after a failure.
+        auto filled = [&]() {
+            if ((threadIdx.x & 127) == 0)
+                acc_ok[piece] = mbar_wait(acc_full + (use & 1), (use >> 1) & 1u, err, kSiteFusedAccFull) ? 1 : 0;
+            named_barrier(1 + piece, 128);
+            const bool is = *reinterpret_cast<volatile int *>(acc_ok + piece) != 0;
+            tc::fence_after_sync();
+            return is;
+        };
+        auto release = [&]() {
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty + (use & 1));
+        };
+        bool ok = true;
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
             const Tile t = tile_of(a, upto, item);
-            const uint32_t buf = use & 1;
             const int out0 = t.m * tile_rows + col, valid = min(4, f.out_rows - out0);
             const float inv = f.inv_globals ? __ldg(f.inv_globals + t.group) : f.inv_global;
             float bias[4] = {0, 0, 0, 0}, bias_up[4] = {0, 0, 0, 0};
@@ -445,52 +512,54 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                     if (f.gated) bias_up[i] = load_as_f32(f.bias, f.bias_type, b + f.out_rows + i);
                 }
             }
-            // One thread waits, so that all four warps leave at the same place after a failure.
-            if (threadIdx.x == 32 * kGmEpiWarp0)
-                *acc_ok = mbar_wait(acc_full + buf, (use >> 1) & 1u, err, kSiteFusedAccFull) ? 1 : 0;
-            named_barrier(1, 128);
-            if (!*reinterpret_cast<volatile int *>(acc_ok)) break;
-            tc::fence_after_sync();
-            for (int c0 = 0; c0 < t.n; c0 += 32, ++chunk_no) {
-                float *page = turn + (chunk_no & 1) * (kGmEpiBytes / 4);
-                uint32_t r[32];
-                tc::ld_32x32b_x32(lanes + buf * kGmMaxN + c0, r);
-                tc::wait_ld();
-                if (c0 + 32 >= t.n) {
-                    tc::fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(acc_empty + buf);
+            auto finish = [&](int c0) {
+                named_barrier(1 + piece, 128);
+                const int row0 = t.row0 + c0, n = min(32, t.n - c0);
+                switch (f.act) {
+                    case NVFP4_ACT_RELU: finish_page<TYPE, NVFP4_ACT_RELU>(a, page, row0, n, vec0, vec_step, col, out0, valid, inv, bias, bias_up); break;
+                    case NVFP4_ACT_SILU: finish_page<TYPE, NVFP4_ACT_SILU>(a, page, row0, n, vec0, vec_step, col, out0, valid, inv, bias, bias_up); break;
+                    case NVFP4_ACT_GELU: finish_page<TYPE, NVFP4_ACT_GELU>(a, page, row0, n, vec0, vec_step, col, out0, valid, inv, bias, bias_up); break;
+                    case NVFP4_ACT_GELU_TANH: finish_page<TYPE, NVFP4_ACT_GELU_TANH>(a, page, row0, n, vec0, vec_step, col, out0, valid, inv, bias, bias_up); break;
+                    default: finish_page<TYPE, NVFP4_ACT_NONE>(a, page, row0, n, vec0, vec_step, col, out0, valid, inv, bias, bias_up);
                 }
+                named_barrier(1 + piece, 128);
+            };
+            if constexpr (TYPE == NVFP4_TYPE_F32) {
+                float sum[32];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) page[i * kGmEpiPitch + place] = __uint_as_float(r[i]);
-                named_barrier(1, 128);
-                for (int v = vec0; v < min(32, t.n - c0); v += vec_step) {
-                    const long long row = (long long)t.row0 + c0 + v;
-                    const float scale = a.row_scale ? inv * __ldcg(a.row_scale + row) : inv;
-                    const float4 zg = *reinterpret_cast<const float4 *>(page + v * kGmEpiPitch + col);
-                    float z[4] = {zg.x, zg.y, zg.z, zg.w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) z[i] = z[i] * scale + bias[i];
-                    if (f.act != NVFP4_ACT_NONE) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) z[i] = activate(z[i], f.act);
+                for (int i = 0; i < 32; ++i) sum[i] = 0.0f;
+                for (int ks = 0; ks < a.k_steps; ks += a.segment, ++use) {
+                    if (!filled()) {
+                        ok = false;
+                        break;
                     }
-                    if (f.gated) {
-                        const float4 zu = *reinterpret_cast<const float4 *>(page + v * kGmEpiPitch + 80 + col);
-                        z[0] *= zu.x * scale + bias_up[0];
-                        z[1] *= zu.y * scale + bias_up[1];
-                        z[2] *= zu.z * scale + bias_up[2];
-                        z[3] *= zu.w * scale + bias_up[3];
-                    }
-                    if (valid <= 0) continue;
-                    if (f.residual) {
-                        float res[4];
-                        load4<TYPE>(f.residual, (size_t)(row * f.residual_stride + out0), a.wide_res, valid, res);
+                    uint32_t r[32];
+                    tc::ld_32x32b_x32(lanes + (use & 1) * kGmMaxN + 32 * piece, r);
+                    tc::wait_ld();
+                    release();
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) z[i] += res[i];
-                    }
-                    store4<TYPE>(f.out, (size_t)(row * f.out_stride + out0), a.wide_out, valid, z);
+                    for (int i = 0; i < 32; ++i) sum[i] += __uint_as_float(r[i]);
                 }
+                if (!ok) break;
+                if (32 * piece < t.n) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) page[i * kGmEpiPitch + place] = sum[i];
+                    finish(32 * piece);
+                }
+            } else {
+                if (!filled()) break;
+                int c0 = 32 * piece;
+                for (; c0 < t.n; c0 += 32 * kGmEpiGroups) {
+                    uint32_t r[32];
+                    tc::ld_32x32b_x32(lanes + (use & 1) * kGmMaxN + c0, r);
+                    tc::wait_ld();
+                    if (c0 + 32 * kGmEpiGroups >= t.n) release();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) page[i * kGmEpiPitch + place] = __uint_as_float(r[i]);
+                    finish(c0);
+                }
+                if (32 * piece >= t.n) release();
+                ++use;
             }
         }
     }
@@ -593,10 +662,14 @@ void launch_linear_gemm(const FusedLinearArgs &f, const nvfp4_matrix &matrix, vo
     GemmArgs g{};
     g.f = f;
     g.terms = f.type == NVFP4_TYPE_F32 ? 2 : 1;
-    g.max_n = kGmMaxN / g.terms;
+    g.max_n = f.type == NVFP4_TYPE_F32 ? kGmMaxN32 : kGmMaxN;
     g.m_tiles = f.gated ? (f.out_rows + 63) / 64 : (f.rows + 127) / 128;
     g.k_steps = (f.cols + 63) / 64;
     g.raw_steps = (f.cols + 255) / 256;
+    g.segment = f.type == NVFP4_TYPE_F32 ? kGmSegment32 : g.k_steps;
+    // One box for the even tiles of a single group; 64 rows (32 where groups have fewer) for ranges known on the device.
+    const int tiles = (f.vectors + g.max_n - 1) / g.max_n;
+    g.box_rows = f.offsets ? ((long long)f.vectors <= 32LL * f.groups ? 32 : 64) : ((f.vectors + tiles - 1) / tiles + 15) / 16 * 16;
     const int e = f.type == NVFP4_TYPE_F32 ? 4 : 2;
     auto vectors_of_4 = [&](const void *p, long long stride) {
         return (reinterpret_cast<uintptr_t>(p) % (4 * e)) == 0 && stride % 4 == 0 ? 1 : 0;
@@ -624,11 +697,11 @@ void launch_linear_gemm(const FusedLinearArgs &f, const nvfp4_matrix &matrix, vo
     }
     CUtensorMap map_x;
     check_cuda(make_tensor_map_u8(&map_x, rows, (uint64_t)f.cols * 2, (uint64_t)stride * 2,
-                                  (uint64_t)f.vectors * (direct ? 1 : g.terms), 128, kGmBoxRows,
+                                  (uint64_t)f.vectors * g.terms, 128, g.box_rows,
                                   CU_TENSOR_MAP_SWIZZLE_128B),
                "cuTensorMapEncodeTiled(rows of x)");
     // Items the call can have: every group may end inside a tile.
-    const long long x_tiles_most = (f.vectors + g.max_n - 1) / g.max_n + (f.offsets ? std::min(f.groups, f.vectors) : 0);
+    const long long x_tiles_most = tiles + (f.offsets ? std::min(f.groups, f.vectors) : 0);
     const int grid = static_cast<int>(std::min<long long>(sm_count, x_tiles_most * g.m_tiles));
     if (f.type == NVFP4_TYPE_BF16) launch<NVFP4_TYPE_BF16>(g, matrix, map_x, grid, !direct, stream);
     else if (f.type == NVFP4_TYPE_F16) launch<NVFP4_TYPE_F16>(g, matrix, map_x, grid, !direct, stream);

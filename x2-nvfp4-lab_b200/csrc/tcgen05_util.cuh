@@ -41,6 +41,16 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// True in one lane of a converged warp. Tensor-core and TMA instructions
+// issued under it, from a warp that runs its loop as a whole, take their
+// operands from uniform registers; under `lane == 0` each one costs about a
+// hundred cycles of issue (measured: 104 per MMA against N / 2 + 10).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
 // ----------------------------------------------------- smem descriptors
 
 // K-major operand tile in shared memory with the 128-byte swizzle: rows of
