@@ -60,7 +60,7 @@ constexpr int kGmOffB = 0;
 constexpr int kGmOffRaw = kGmOffB + kGmStages * kGmStageB;
 constexpr int kGmOffEpi = kGmOffRaw + kGmRawStages * kGmRaw;
 constexpr int kGmOffBars = kGmOffEpi + kGmEpiGroups * kGmEpiBytes;
-constexpr int kGmBars = 2 * kGmStages + kGmStages + 2 * kGmRawStages + 2 + 2 + 1;
+constexpr int kGmBars = 2 * kGmStages + 2 * kGmRawStages + 2 + 2 + 1;
 constexpr int kGmOffTiles = kGmOffBars + kGmBars * 8 + 24;
 constexpr size_t kGmSmem = 1024 + kGmOffTiles + sizeof(int) * (kLinMaxGroups + 1);
 static_assert(kGmOffTiles % 4 == 0 && kGmSmem <= 232448, "shared memory overflow");
@@ -79,7 +79,6 @@ enum GemmWaitSite : int {
 struct GemmArgs {
     FusedLinearArgs f;
     const float *row_scale;  // [vectors] of split FP32 x (NULL: ones)
-    int terms;               // 16-bit parts of x
     int max_n;               // rows of x per tile
     int box_rows;            // rows of x per TMA box
     int segment;             // steps per accumulator
@@ -88,6 +87,17 @@ struct GemmArgs {
     int k_steps;             // 64-column steps over K
     int wide_out, wide_res;  // four outputs may move as one vector
 };
+
+// A warp's wait: one try and a vote on the way that matters, the bounded wait
+// out of line. The same answer in every lane, so that a warp stays whole.
+__device__ __noinline__ bool wait_long(uint64_t *bar, uint32_t parity, int *err, int site) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, site));
+}
+
+__device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, int *err, int site) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    return wait_long(bar, parity, err, site);
+}
 
 __device__ __forceinline__ bool wait_drain(uint64_t *bar, uint32_t parity) {
     const unsigned long long t0 = global_ns();
@@ -241,13 +251,13 @@ __global__ void __launch_bounds__(kGmThreads, 1)
     linear_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_s,
                        const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ GemmArgs a) {
     constexpr bool kBf16 = TYPE == NVFP4_TYPE_BF16;
+    constexpr int kTerms = TYPE == NVFP4_TYPE_F32 ? 2 : 1;
     constexpr int S = kGmStages, R = kGmRawStages;
     extern __shared__ uint8_t gm_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(gm_smem_raw) + 1023) & ~uintptr_t(1023));
     const FusedLinearArgs &f = a.f;
-    uint64_t *b_full = reinterpret_cast<uint64_t *>(smem + kGmOffBars);  // [S] rows of x have landed
-    uint64_t *a_full = b_full + S;                                       // [S] weights are decoded (four warps)
-    uint64_t *empty = a_full + S;                                        // [S] the step's MMAs are done with both
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + kGmOffBars);    // [S] rows of x have landed, weights are decoded (four warps)
+    uint64_t *empty = full + S;                                          // [S] the step's MMAs are done with both
     uint64_t *raw_full = empty + S;                                      // [R] packed weights and scales have landed
     uint64_t *raw_empty = raw_full + R;                                  // [R] (every conversion warp)
     uint64_t *acc_full = raw_empty + R;                                  // [2]
@@ -261,8 +271,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i) {
-            mbar_init(b_full + i, 1);
-            mbar_init(a_full + i, 4);
+            mbar_init(full + i, 1 + 4);
             mbar_init(empty + i, 1);
         }
         for (int i = 0; i < R; ++i) {
@@ -323,16 +332,16 @@ __global__ void __launch_bounds__(kGmThreads, 1)
             const int boxes = (t.n + a.box_rows - 1) / a.box_rows;
             for (int ks = 0; ks < a.k_steps; ++ks, ++it) {
                 const int st = it % S;
-                if (!__all_sync(0xffffffffu, mbar_wait(empty + st, ((it / S) & 1u) ^ 1u, err, kSiteFusedEmpty))) {
+                if (!wait_warp(empty + st, ((it / S) & 1u) ^ 1u, err, kSiteFusedEmpty)) {
                     ok = false;
                     break;
                 }
                 uint8_t *b = smem + kGmOffB + st * kGmStageB;
                 if (tc::elect_one()) {
-                    mbar_arrive_expect_tx(b_full + st, a.terms * boxes * a.box_rows * 128);
-                    for (int j = 0; j < a.terms; ++j)
+                    mbar_arrive_expect_tx(full + st, kTerms * boxes * a.box_rows * 128);
+                    for (int j = 0; j < kTerms; ++j)
                         for (int x = 0; x < boxes; ++x)
-                            tma_load_2d(b + (j * a.max_n + x * a.box_rows) * 128, &tm_x, b_full + st, ks * 128,
+                            tma_load_2d(b + (j * a.max_n + x * a.box_rows) * 128, &tm_x, full + st, ks * 128,
                                         j * f.vectors + t.row0 + x * a.box_rows);
                 }
                 __syncwarp();
@@ -340,7 +349,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         }
         // After a failure the copies of the last stages issued land before the CTA ends.
         if (!ok || *reinterpret_cast<volatile int *>(err) != 0)
-            for (uint32_t k = it > (uint32_t)S ? it - S : 0u; k < it; ++k) wait_drain(b_full + k % S, (k / S) & 1u);
+            for (uint32_t k = it > (uint32_t)S ? it - S : 0u; k < it; ++k) wait_drain(full + k % S, (k / S) & 1u);
         __syncwarp();
     } else if (warp == 2) {
         // ----------------------------------------- producer of weights
@@ -351,7 +360,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
             const int w0 = t.group * f.rows + t.m * (f.gated ? 64 : 128), w1 = w0 + (f.gated ? f.out_rows : 64);
             for (int rs = 0; rs < a.raw_steps; ++rs, ++rt) {
                 const int st = rt % R;
-                if (!__all_sync(0xffffffffu, mbar_wait(raw_empty + st, ((rt / R) & 1u) ^ 1u, err, kSiteFusedRawEmpty))) {
+                if (!wait_warp(raw_empty + st, ((rt / R) & 1u) ^ 1u, err, kSiteFusedRawEmpty)) {
                     ok = false;
                     break;
                 }
@@ -371,47 +380,45 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         __syncwarp();
     } else if (warp == 1) {
         // ---------------------------------------------------------- MMA
+        // Everything an instruction takes is the same in every lane and known to be (reductions, loop counters).
         const uint32_t base = smem_u32(smem) + kGmOffB;
-        uint32_t it = 0;
+        const int last = __reduce_max_sync(0xffffffffu, items);
+        uint32_t st = 0, ph = 0;
         bool ok = true;
-        int use = 0;  // accumulators filled so far
-        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-            const Tile t = tile_of(a, upto, item);
-            const uint32_t idesc = tc::idesc_16bit((uint32_t)((t.n + 15) & ~15), kBf16 ? 1u : 0u);
-            int left = 0;
-            for (int ks = 0; ks < a.k_steps; ++ks, ++it) {
+        uint32_t use = 0;  // accumulators filled so far
+        for (int item = blockIdx.x; item < last && ok; item += gridDim.x) {
+            const uint32_t n = __reduce_max_sync(0xffffffffu, tile_of(a, upto, item).n);
+            const uint32_t idesc = tc::idesc_16bit((n + 15) & ~15u, kBf16 ? 1u : 0u);
+            for (int left = a.k_steps; left > 0 && ok; left -= a.segment, ++use) {
                 const uint32_t buf = use & 1, acc = tmem + buf * kGmMaxN;
-                const bool fresh = left == 0;
-                if (fresh) {
-                    left = min(a.segment, a.k_steps - ks);
-                    if (use > 1 &&
-                        !__all_sync(0xffffffffu, mbar_wait(acc_empty + buf, ((use >> 1) - 1) & 1u, err, kSiteFusedAccEmpty))) {
-                        ok = false;
-                        break;
-                    }
-                }
-                const int st = it % S;
-                const uint32_t ph = (it / S) & 1u;
-                if (!__all_sync(0xffffffffu, mbar_wait(b_full + st, ph, err, kSiteFusedFull)) ||
-                    !__all_sync(0xffffffffu, mbar_wait(a_full + st, ph, err, kSiteFusedFull))) {
+                if (use > 1 && !wait_warp(acc_empty + buf, ((use >> 1) - 1) & 1u, err, kSiteFusedAccEmpty)) {
                     ok = false;
                     break;
                 }
-                tc::fence_after_sync();
-                --left;
-                if (tc::elect_one()) {
-                    for (int j = 0; j < a.terms; ++j) {
-                        const uint32_t b = base + st * kGmStageB + j * a.max_n * 128;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            tc::mma_16bit_ts(acc, tmem + kGmColA + 32 * st + 8 * i, tc::smem_desc_sw128(b + 32 * i), idesc,
-                                             fresh && (j | i) == 0 ? 0u : 1u);
+                const int steps = min(left, a.segment);
+                uint32_t more = 0;
+                for (int ks = 0; ks < steps; ++ks) {
+                    if (!wait_warp(full + st, ph, err, kSiteFusedFull)) {
+                        ok = false;
+                        break;
                     }
-                    tc::commit(empty + st);
-                    if (left == 0) tc::commit(acc_full + buf);
+                    tc::fence_after_sync();
+                    if (tc::elect_one()) {
+#pragma unroll
+                        for (int j = 0; j < kTerms; ++j)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                tc::mma_16bit_ts(acc, tmem + kGmColA + 32 * st + 8 * i,
+                                                 tc::smem_desc_sw128(base + st * kGmStageB + j * kGmMaxN32 * 128 + 32 * i),
+                                                 idesc, (j | i) != 0 ? 1u : more);
+                        tc::commit(empty + st);
+                    }
+                    __syncwarp();
+                    more = 1;
+                    if (++st == S) st = 0, ph ^= 1;
                 }
+                if (ok && tc::elect_one()) tc::commit(acc_full + buf);
                 __syncwarp();
-                if (left == 0) ++use;
             }
         }
         // Every MMA has completed before tensor memory is freed.
@@ -431,7 +438,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
             for (int ks0 = 0; ks0 < a.k_steps && ok; ks0 += 4, ++rt) {
                 const int rs = rt % R;
-                if (!__all_sync(0xffffffffu, mbar_wait(raw_full + rs, (rt / R) & 1u, err, kSiteFusedRawFull))) {
+                if (!wait_warp(raw_full + rs, (rt / R) & 1u, err, kSiteFusedRawFull)) {
                     ok = false;
                     break;
                 }
@@ -454,7 +461,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                     decode8<kBf16>(q1.z, s3, r + 24);
                     decode8<kBf16>(q1.w, s3, r + 28);
                     const int st = next % S;
-                    if (!__all_sync(0xffffffffu, mbar_wait(empty + st, ((next / S) & 1u) ^ 1u, err, kSiteFusedEmpty))) {
+                    if (!wait_warp(empty + st, ((next / S) & 1u) ^ 1u, err, kSiteFusedEmpty)) {
                         ok = false;
                         break;
                     }
@@ -463,7 +470,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                     tc::wait_st();
                     tc::fence_before_sync();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(a_full + st);
+                    if (lane == 0) mbar_arrive(full + st);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(raw_empty + rs);
@@ -661,7 +668,7 @@ void launch_linear_gemm(const FusedLinearArgs &f, const nvfp4_matrix &matrix, vo
                         cudaStream_t stream) {
     GemmArgs g{};
     g.f = f;
-    g.terms = f.type == NVFP4_TYPE_F32 ? 2 : 1;
+    const int terms = f.type == NVFP4_TYPE_F32 ? 2 : 1;  // 16-bit parts of x
     g.max_n = f.type == NVFP4_TYPE_F32 ? kGmMaxN32 : kGmMaxN;
     g.m_tiles = f.gated ? (f.out_rows + 63) / 64 : (f.rows + 127) / 128;
     g.k_steps = (f.cols + 63) / 64;
@@ -697,7 +704,7 @@ void launch_linear_gemm(const FusedLinearArgs &f, const nvfp4_matrix &matrix, vo
     }
     CUtensorMap map_x;
     check_cuda(make_tensor_map_u8(&map_x, rows, (uint64_t)f.cols * 2, (uint64_t)stride * 2,
-                                  (uint64_t)f.vectors * g.terms, 128, g.box_rows,
+                                  (uint64_t)f.vectors * terms, 128, g.box_rows,
                                   CU_TENSOR_MAP_SWIZZLE_128B),
                "cuTensorMapEncodeTiled(rows of x)");
     // Items the call can have: every group may end inside a tile.
