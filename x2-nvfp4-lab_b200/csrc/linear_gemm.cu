@@ -107,39 +107,26 @@ __device__ __forceinline__ bool wait_drain(uint64_t *bar, uint32_t parity) {
     }
 }
 
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
+// Two FP16 values times their scales as a BF16 pair: the products have at most six significant bits, so the FP32
+// results of the mixed-precision FMA are exact and so are their upper halves. (Shifting FP16 patterns into BF16 and
+// multiplying there takes two more instructions on the half-rate integer pipe: 29 against 44 weights per cycle and SM.)
+__device__ __forceinline__ uint32_t mul_f16x2_to_bf16x2(uint32_t a, uint32_t b) {
+    float lo, hi;
+    asm("{\n\t.reg .f16 a0, a1, b0, b1;\n\t"
+        "mov.b32 {a0, a1}, %2;\n\tmov.b32 {b0, b1}, %3;\n\t"
+        "fma.rn.f32.f16 %0, a0, b0, 0f00000000;\n\tfma.rn.f32.f16 %1, a1, b1, 0f00000000;\n\t}"
+        : "=f"(lo), "=f"(hi)
+        : "r"(a), "r"(b));
+    return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
 }
 
-// Eight codes times their block scale as four 16-bit pairs. FP16: `scale` is the scale twice. BF16: an E2M1 value in
-// FP16 has its bits in the sign, the exponent and the first mantissa bit; three places to the right they are the
-// BF16 pattern of value * 2^-112, and `scale` carries 2^112.
+// Eight codes times their block scale (FP16, twice) as four 16-bit pairs.
 template <bool BF16>
 __device__ __forceinline__ void decode8(uint32_t codes, uint32_t scale, uint32_t *out) {
     uint32_t h[4];
     e2m1x8_to_f16x8(codes, h);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (BF16)
-            out[i] = mul_bf16x2(((h[i] >> 3) & 0x0FFF0FFFu) | (h[i] & 0x80008000u), scale);
-        else
-            out[i] = hmul2_u32(h[i], scale);
-    }
-}
-
-// The scale byte at place `i` of `word`, twice, as decode8 wants it. BF16: the byte's bits at the BF16 exponent's
-// end are scale * 2^-120 (subnormals too); two multiplications by 2^116.
-template <bool BF16>
-__device__ __forceinline__ uint32_t scale_pair(uint32_t word, int i) {
-    if constexpr (BF16) {
-        const uint32_t b = ((word >> (8 * i)) & 0x7Fu) * 0x00100010u;
-        return mul_bf16x2(mul_bf16x2(b, 0x79807980u), 0x79807980u);
-    } else {
-        const uint32_t s = e4m3x2_to_f16x2((uint16_t)(word >> (16 * (i >> 1))));
-        return (i & 1) ? f16x2_hi_hi(s) : f16x2_lo_lo(s);
-    }
+    for (int i = 0; i < 4; ++i) out[i] = BF16 ? mul_f16x2_to_bf16x2(h[i], scale) : hmul2_u32(h[i], scale);
 }
 
 struct Tile {
@@ -450,8 +437,8 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                     const uint4 q0 = *reinterpret_cast<const uint4 *>(raw + row * 128 + (((2 * j) ^ (row & 7)) << 4));
                     const uint4 q1 = *reinterpret_cast<const uint4 *>(raw + row * 128 + (((2 * j + 1) ^ (row & 7)) << 4));
                     uint32_t r[32];
-                    const uint32_t s0 = scale_pair<kBf16>(word, 0), s1 = scale_pair<kBf16>(word, 1);
-                    const uint32_t s2 = scale_pair<kBf16>(word, 2), s3 = scale_pair<kBf16>(word, 3);
+                    const uint32_t s01 = e4m3x2_to_f16x2((uint16_t)word), s23 = e4m3x2_to_f16x2((uint16_t)(word >> 16));
+                    const uint32_t s0 = f16x2_lo_lo(s01), s1 = f16x2_hi_hi(s01), s2 = f16x2_lo_lo(s23), s3 = f16x2_hi_hi(s23);
                     decode8<kBf16>(q0.x, s0, r);
                     decode8<kBf16>(q0.y, s0, r + 4);
                     decode8<kBf16>(q0.z, s1, r + 8);
