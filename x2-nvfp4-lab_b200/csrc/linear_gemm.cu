@@ -7,14 +7,14 @@
 // the packed bytes from shared memory, decode a row's 64 columns in registers
 // and store them with tcgen05.st, so that neither the decoded tile nor its
 // reads cross shared memory, whose bandwidth the B operand needs. The rows of
-// x are B (N = 16 to 192, as many as the tile has: the instruction's N is chosen per tile),
+// x are B (N = 16 to 160, as many as the tile has: the instruction's N is chosen per tile),
 // loaded by TMA. With a gate the tile is 64 gate and 64 up rows, 16 of each in
 // every lane quarter.
 //
 // Warps: 0 producer of x and 2 of weights (TMA), 1 MMA issuer, 4-15 conversion
 // (three warpgroups, every third 64-column step each), 16-23 epilogue (two
 // warpgroups, every other 32 columns each). Tensor memory: two accumulators of
-// 192 columns, and four decoded steps of 32. The epilogue turns 32 columns at
+// 160 columns, and six decoded steps of 32. The epilogue turns 32 columns at
 // a time through shared memory, so that a lane has four consecutive outputs of
 // one row of x: bias in registers, residual and stores as vectors.
 //
@@ -48,7 +48,7 @@ constexpr int kGmStages = 4;                        // 64-column steps in flight
 constexpr int kGmMaxN = 192;
 constexpr int kGmMaxN32 = 64;                       // of split FP32 x: one 32-column piece per epilogue warpgroup
 constexpr int kGmSegment32 = 4;                     // its steps per accumulator
-constexpr int kGmStageB = kGmMaxN * 128;            // a step of x: up to 192 rows x 64 columns
+constexpr int kGmStageB = kGmMaxN / 2 * 128;        // a CTA's half of a step of x: up to 96 rows x 64 columns
 constexpr int kGmRawStages = 3;                     // 256 columns of packed weights each
 constexpr int kGmRawBytes = 128 * 128;
 constexpr int kGmRawScales = 128 * 16;
@@ -82,7 +82,7 @@ struct GemmArgs {
     int max_n;               // rows of x per tile
     int box_rows;            // rows of x per TMA box
     int segment;             // steps per accumulator
-    int m_tiles;             // weight tiles of a group
+    int m_pairs;             // pairs of weight tiles of a group
     int raw_steps;           // 256-column steps over K
     int k_steps;             // 64-column steps over K
     int wide_out, wide_res;  // four outputs may move as one vector
@@ -137,9 +137,9 @@ struct Tile {
 __device__ __forceinline__ int x_tiles(int count, int max_n) { return (count + max_n - 1) / max_n; }
 
 __device__ __forceinline__ Tile tile_of(const GemmArgs &a, const int *upto, int item) {
-    // The group with upto[g] * m_tiles <= item < upto[g + 1] * m_tiles.
+    // The group with upto[g] * m_pairs <= item < upto[g + 1] * m_pairs.
     Tile t;
-    const int at = item / a.m_tiles;
+    const int at = item / a.m_pairs;
     int lo = 0, hi = a.f.offsets ? a.f.groups : 1;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -150,10 +150,10 @@ __device__ __forceinline__ Tile tile_of(const GemmArgs &a, const int *upto, int 
     int first, count;
     group_range(a.f, lo, &first, &count);
     const int tiles = upto[lo + 1] - upto[lo];
-    const int in_group = item - upto[lo] * a.m_tiles;
-    t.m = in_group / tiles;
+    const int in_group = item - upto[lo] * a.m_pairs;
+    t.m = 2 * (in_group / tiles) + (int)cluster_rank();
     const int width = ((count + tiles - 1) / tiles + 15) & ~15;
-    const int v = (in_group - t.m * tiles) * width;
+    const int v = in_group % tiles * width;
     t.row0 = first + v;
     t.n = min(width, count - v);
     return t;
@@ -243,22 +243,24 @@ __global__ void __launch_bounds__(kGmThreads, 1)
     extern __shared__ uint8_t gm_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(gm_smem_raw) + 1023) & ~uintptr_t(1023));
     const FusedLinearArgs &f = a.f;
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + kGmOffBars);    // [S] rows of x have landed, weights are decoded (four warps)
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + kGmOffBars);    // [S] rows of x have landed, weights are decoded (four warps); even CTA: and the odd one's have
     uint64_t *empty = full + S;                                          // [S] the step's MMAs are done with both
     uint64_t *raw_full = empty + S;                                      // [R] packed weights and scales have landed
     uint64_t *raw_empty = raw_full + R;                                  // [R] (every conversion warp)
     uint64_t *acc_full = raw_empty + R;                                  // [2]
-    uint64_t *acc_empty = acc_full + 2;                                  // [2] (every epilogue warp)
+    uint64_t *acc_empty = acc_full + 2;                                  // [2] (every epilogue warp of both CTAs; even CTA)
     uint64_t *drain = acc_empty + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     int *acc_ok = reinterpret_cast<int *>(tmem_slot + 1);                // [epilogue warpgroups]
     int *upto = reinterpret_cast<int *>(smem + kGmOffTiles);             // [groups + 1] x tiles of the groups before
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int *err = f.err;
+    const uint32_t rank = cluster_rank();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i) {
-            mbar_init(full + i, 1 + 4);
+            mbar_init(full + i, 1 + 4 + (rank == 0 ? 1 : 0));
             mbar_init(empty + i, 1);
         }
         for (int i = 0; i < R; ++i) {
@@ -267,7 +269,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(acc_full + i, 1);
-            mbar_init(acc_empty + i, 4 * kGmEpiGroups);
+            mbar_init(acc_empty + i, 2 * 4 * kGmEpiGroups);
         }
         mbar_init(drain, 1);
         fence_barrier_init();
@@ -276,8 +278,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         prefetch_tensormap(&tm_x);
     }
     if (warp == 1) {
-        tc::tmem_alloc(tmem_slot, 512);
-        tc::tmem_relinquish();
+        tc::tmem_alloc_pair(tmem_slot, 512);
     }
     if (warp == 2) {
         const int groups = f.offsets ? f.groups : 1;
@@ -305,18 +306,21 @@ __global__ void __launch_bounds__(kGmThreads, 1)
     }
     tc::fence_before_sync();
     __syncthreads();
+    cluster_sync();  // the other CTA's barriers are ready too
     tc::fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-    const int items = upto[f.offsets ? f.groups : 1] * a.m_tiles;
+    const int items = upto[f.offsets ? f.groups : 1] * a.m_pairs;
     if (warp != 2) pdl_wait();  // the rows that the split kernel wrote; the weights wait for nothing
 
     if (warp == 0) {
         // ----------------------------------------------- producer of x
         uint32_t it = 0;
         bool ok = true;
-        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+        for (int item = pair; item < items && ok; item += pairs) {
             const Tile t = tile_of(a, upto, item);
-            const int boxes = (t.n + a.box_rows - 1) / a.box_rows;
+            // The pair splits the tile's rows: this CTA's are the first or the second half of N.
+            const int half = ((t.n + 15) & ~15) / 2, row0 = t.row0 + (int)rank * half;
+            const int boxes = (half + a.box_rows - 1) / a.box_rows;
             for (int ks = 0; ks < a.k_steps; ++ks, ++it) {
                 const int st = it % S;
                 if (!wait_warp(empty + st, ((it / S) & 1u) ^ 1u, err, kSiteFusedEmpty)) {
@@ -328,8 +332,8 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                     mbar_arrive_expect_tx(full + st, kTerms * boxes * a.box_rows * 128);
                     for (int j = 0; j < kTerms; ++j)
                         for (int x = 0; x < boxes; ++x)
-                            tma_load_2d(b + (j * a.max_n + x * a.box_rows) * 128, &tm_x, full + st, ks * 128,
-                                        j * f.vectors + t.row0 + x * a.box_rows);
+                            tma_load_2d(b + (j * (kGmMaxN32 / 2) + x * a.box_rows) * 128, &tm_x, full + st, ks * 128,
+                                        j * f.vectors + row0 + x * a.box_rows);
                 }
                 __syncwarp();
             }
@@ -342,7 +346,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         // ----------------------------------------- producer of weights
         uint32_t rt = 0;
         bool ok = true;
-        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+        for (int item = pair; item < items && ok; item += pairs) {
             const Tile t = tile_of(a, upto, item);
             const int w0 = t.group * f.rows + t.m * (f.gated ? 64 : 128), w1 = w0 + (f.gated ? f.out_rows : 64);
             for (int rs = 0; rs < a.raw_steps; ++rs, ++rt) {
@@ -373,45 +377,65 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         uint32_t st = 0, ph = 0;
         bool ok = true;
         uint32_t use = 0;  // accumulators filled so far
-        for (int item = blockIdx.x; item < last && ok; item += gridDim.x) {
-            const uint32_t n = __reduce_max_sync(0xffffffffu, tile_of(a, upto, item).n);
-            const uint32_t idesc = tc::idesc_16bit((n + 15) & ~15u, kBf16 ? 1u : 0u);
-            for (int left = a.k_steps; left > 0 && ok; left -= a.segment, ++use) {
-                const uint32_t buf = use & 1, acc = tmem + buf * kGmMaxN;
-                if (use > 1 && !wait_warp(acc_empty + buf, ((use >> 1) - 1) & 1u, err, kSiteFusedAccEmpty)) {
-                    ok = false;
-                    break;
-                }
-                const int steps = min(left, a.segment);
-                uint32_t more = 0;
-                for (int ks = 0; ks < steps; ++ks) {
+        if (rank == 1) {
+            // The odd CTA tells the even one, which issues for both, when its half of a step is there.
+            for (int item = pair; item < last && ok; item += pairs) {
+                for (int ks = 0; ks < a.k_steps; ++ks) {
                     if (!wait_warp(full + st, ph, err, kSiteFusedFull)) {
                         ok = false;
                         break;
                     }
                     tc::fence_after_sync();
-                    if (tc::elect_one()) {
-#pragma unroll
-                        for (int j = 0; j < kTerms; ++j)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                tc::mma_16bit_ts(acc, tmem + kGmColA + 32 * st + 8 * i,
-                                                 tc::smem_desc_sw128(base + st * kGmStageB + j * kGmMaxN32 * 128 + 32 * i),
-                                                 idesc, (j | i) != 0 ? 1u : more);
-                        tc::commit(empty + st);
-                    }
+                    tc::fence_before_sync();
+                    if (tc::elect_one()) mbar_arrive_at(full + st, 0);
                     __syncwarp();
-                    more = 1;
                     if (++st == S) st = 0, ph ^= 1;
                 }
-                if (ok && tc::elect_one()) tc::commit(acc_full + buf);
-                __syncwarp();
+            }
+        } else {
+            for (int item = pair; item < last && ok; item += pairs) {
+                const uint32_t n = __reduce_max_sync(0xffffffffu, tile_of(a, upto, item).n);
+                const uint32_t idesc = tc::idesc_16bit_pair((n + 15) & ~15u, kBf16 ? 1u : 0u);
+                for (int left = a.k_steps; left > 0 && ok; left -= a.segment, ++use) {
+                    const uint32_t buf = use & 1, acc = tmem + buf * kGmMaxN;
+                    if (use > 1 && !wait_warp(acc_empty + buf, ((use >> 1) - 1) & 1u, err, kSiteFusedAccEmpty)) {
+                        ok = false;
+                        break;
+                    }
+                    const int steps = min(left, a.segment);
+                    uint32_t more = 0;
+                    for (int ks = 0; ks < steps; ++ks) {
+                        if (!wait_warp(full + st, ph, err, kSiteFusedFull)) {
+                            ok = false;
+                            break;
+                        }
+                        tc::fence_after_sync();
+                        if (tc::elect_one()) {
+#pragma unroll
+                            for (int j = 0; j < kTerms; ++j)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    tc::mma_16bit_ts_pair(
+                                        acc, tmem + kGmColA + 32 * st + 8 * i,
+                                        tc::smem_desc_sw128(base + st * kGmStageB + j * (kGmMaxN32 / 2) * 128 + 32 * i),
+                                        idesc, (j | i) != 0 ? 1u : more);
+                            tc::commit_pair(empty + st);
+                        }
+                        __syncwarp();
+                        more = 1;
+                        if (++st == S) st = 0, ph ^= 1;
+                    }
+                    if (ok && tc::elect_one()) tc::commit_pair(acc_full + buf);
+                    __syncwarp();
+                }
             }
         }
-        // Every MMA has completed before tensor memory is freed.
-        if (tc::elect_one()) tc::commit(drain);
-        __syncwarp();
-        wait_drain(drain, 0);
+        // Every MMA has completed before tensor memory is freed (the odd CTA waits for the even one below).
+        if (rank == 0) {
+            if (tc::elect_one()) tc::commit_pair(drain);
+            __syncwarp();
+            wait_drain(drain, 0);
+        }
         __syncwarp();
     } else if (warp >= kGmConvWarp0 && warp < kGmEpiWarp0) {
         // --------------------------------------------------- conversion
@@ -422,7 +446,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16) + kGmColA;
         uint32_t it = 0, rt = 0, next = mine;
         bool ok = true;
-        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+        for (int item = pair; item < items && ok; item += pairs) {
             for (int ks0 = 0; ks0 < a.k_steps && ok; ks0 += 4, ++rt) {
                 const int rs = rt % R;
                 if (!wait_warp(raw_full + rs, (rt / R) & 1u, err, kSiteFusedRawFull)) {
@@ -489,10 +513,10 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         auto release = [&]() {
             tc::fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty + (use & 1));
+            if (lane == 0) mbar_arrive_at(acc_empty + (use & 1), 0);
         };
         bool ok = true;
-        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+        for (int item = pair; item < items && ok; item += pairs) {
             const Tile t = tile_of(a, upto, item);
             const int out0 = t.m * tile_rows + col, valid = min(4, f.out_rows - out0);
             const float inv = f.inv_globals ? __ldg(f.inv_globals + t.group) : f.inv_global;
@@ -561,9 +585,10 @@ __global__ void __launch_bounds__(kGmThreads, 1)
 
     tc::fence_before_sync();
     __syncthreads();
+    cluster_sync();  // neither CTA leaves while the other may reach its shared memory
     if (warp == 1) {
         tc::fence_after_sync();
-        tc::tmem_dealloc(tmem, 512);
+        tc::tmem_dealloc_pair(tmem, 512);
     }
     if (threadIdx.x == 0 && *reinterpret_cast<volatile int *>(err) != 0 && f.host_err) {
         const int code = *reinterpret_cast<volatile int *>(err);
@@ -635,11 +660,14 @@ void launch(const GemmArgs &g, const nvfp4_matrix &matrix, const CUtensorMap &ma
     cfg.blockDim = dim3(kGmThreads);
     cfg.dynamicSmemBytes = kGmSmem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = dependent ? 1 : 0;
+    cfg.numAttrs = dependent ? 2 : 1;
     check_cuda(cudaLaunchKernelEx(&cfg, linear_gemm_kernel<TYPE>, matrix.map_w, matrix.map_s, map_x, g),
                "linear_gemm_kernel");
 }
@@ -657,13 +685,15 @@ void launch_linear_gemm(const FusedLinearArgs &f, const nvfp4_matrix &matrix, vo
     g.f = f;
     const int terms = f.type == NVFP4_TYPE_F32 ? 2 : 1;  // 16-bit parts of x
     g.max_n = f.type == NVFP4_TYPE_F32 ? kGmMaxN32 : kGmMaxN;
-    g.m_tiles = f.gated ? (f.out_rows + 63) / 64 : (f.rows + 127) / 128;
+    g.m_pairs = f.gated ? (f.out_rows + 127) / 128 : (f.rows + 255) / 256;
     g.k_steps = (f.cols + 63) / 64;
     g.raw_steps = (f.cols + 255) / 256;
     g.segment = f.type == NVFP4_TYPE_F32 ? kGmSegment32 : g.k_steps;
-    // One box for the even tiles of a single group; 64 rows (32 where groups have fewer) for ranges known on the device.
+    // One box for half of the even tiles of a single group; 32 rows (16 where groups have few) for ranges known on the
+    // device.
     const int tiles = (f.vectors + g.max_n - 1) / g.max_n;
-    g.box_rows = f.offsets ? ((long long)f.vectors <= 32LL * f.groups ? 32 : 64) : ((f.vectors + tiles - 1) / tiles + 15) / 16 * 16;
+    g.box_rows = f.offsets ? ((long long)f.vectors <= 32LL * f.groups || f.type == NVFP4_TYPE_F32 ? 16 : 32)
+                           : ((f.vectors + tiles - 1) / tiles + 15) / 16 * 8;
     const int e = f.type == NVFP4_TYPE_F32 ? 4 : 2;
     auto vectors_of_4 = [&](const void *p, long long stride) {
         return (reinterpret_cast<uintptr_t>(p) % (4 * e)) == 0 && stride % 4 == 0 ? 1 : 0;
@@ -696,7 +726,7 @@ void launch_linear_gemm(const FusedLinearArgs &f, const nvfp4_matrix &matrix, vo
                "cuTensorMapEncodeTiled(rows of x)");
     // Items the call can have: every group may end inside a tile.
     const long long x_tiles_most = tiles + (f.offsets ? std::min(f.groups, f.vectors) : 0);
-    const int grid = static_cast<int>(std::min<long long>(sm_count, x_tiles_most * g.m_tiles));
+    const int grid = 2 * static_cast<int>(std::min<long long>(sm_count / 2, x_tiles_most * g.m_pairs));
     if (f.type == NVFP4_TYPE_BF16) launch<NVFP4_TYPE_BF16>(g, matrix, map_x, grid, !direct, stream);
     else if (f.type == NVFP4_TYPE_F16) launch<NVFP4_TYPE_F16>(g, matrix, map_x, grid, !direct, stream);
     else launch<NVFP4_TYPE_F32>(g, matrix, map_x, grid, !direct, stream);

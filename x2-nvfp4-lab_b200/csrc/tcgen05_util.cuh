@@ -109,20 +109,48 @@ __device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uin
         : "memory");
 }
 
+// ------------------------------------------------------- CTA pairs
+// cta_group::2: two CTAs of a cluster work on one tile of 256 rows. Each holds
+// its 128 rows of A and of D in its own tensor memory and half of B's rows in
+// its shared memory, at the same addresses; one thread of the even CTA issues.
+
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t *slot, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     static_cast<uint32_t>(__cvta_generic_to_shared(slot))),
+                 "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t base, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(ncols) : "memory");
+}
+
 // Instruction descriptor of kind::f16 with both operands FP16 (bf16 = 0) or
-// BF16 (1), FP32 accumulation, K-major, M = 128 and N = `n`.
-__device__ __forceinline__ uint32_t idesc_16bit(uint32_t n, uint32_t bf16) {
-    return (1u << 4) | (bf16 << 7) | (bf16 << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+// BF16 (1), FP32 accumulation, K-major, M = 256 and N = `n`.
+__device__ __forceinline__ uint32_t idesc_16bit_pair(uint32_t n, uint32_t bf16) {
+    return (1u << 4) | (bf16 << 7) | (bf16 << 10) | ((n >> 3) << 17) | ((256u >> 4) << 24);
 }
 
 // D[tmem d] (+)= A[tmem a] * B[smem b]^T, 16-bit operands (K 16 per
-// instruction): A is 128 lanes x 8 columns, two consecutive K per column.
-__device__ __forceinline__ void mma_16bit_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// instruction): A is 128 lanes x 8 columns in each CTA, two consecutive K per column.
+__device__ __forceinline__ void mma_16bit_ts_pair(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                                  uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Arrive once on the barrier at this offset in both CTAs when every tcgen05
+// operation this thread issued so far has completed.
+__device__ __forceinline__ void commit_pair(uint64_t *bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            static_cast<uint32_t>(__cvta_generic_to_shared(bar))),
+        "h"(static_cast<uint16_t>(3))
         : "memory");
 }
 

@@ -67,6 +67,27 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
     return ok != 0;
 }
 
+// Rank of this CTA in its cluster, and a barrier of all the cluster's threads.
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Arrive on the barrier at `bar`'s offset in the cluster's CTA `rank`.
+__device__ __forceinline__ void mbar_arrive_at(uint64_t *bar, uint32_t rank) {
+    asm volatile(
+        "{\n\t.reg .b32 remote;\n\t"
+        "mapa.shared::cluster.u32 remote, %0, %1;\n\t"
+        "mbarrier.arrive.shared::cluster.b64 _, [remote];\n\t}" ::"r"(smem_u32(bar)),
+        "r"(rank)
+        : "memory");
+}
+
 // Wait for the phase with the given parity to complete. Gives up after
 // kWaitLimitNs of wall-clock time, recording `site` (a nonzero code naming
 // the wait) in *err unless an earlier failure is recorded there, or at once
