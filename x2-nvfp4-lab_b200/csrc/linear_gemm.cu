@@ -12,9 +12,9 @@
 // every lane quarter.
 //
 // Warps: 0 producer of x and 2 of weights (TMA), 1 MMA issuer, 4-15 conversion
-// (three warpgroups, every third 64-column step each), 16-23 epilogue (two
+// (three warpgroups, every third 64 columns each), 16-23 epilogue (two
 // warpgroups, every other 32 columns each). Tensor memory: two accumulators of
-// 160 columns, and six decoded steps of 32. The epilogue turns 32 columns at
+// 160 columns, and three decoded steps of 64. The epilogue turns 32 columns at
 // a time through shared memory, so that a lane has four consecutive outputs of
 // one row of x: bias in registers, residual and stores as vectors.
 //
@@ -44,11 +44,12 @@ namespace {
 constexpr int kGmConvWarp0 = 4, kGmConvGroups = 3, kGmEpiWarp0 = kGmConvWarp0 + 4 * kGmConvGroups;
 constexpr int kGmEpiGroups = 2;
 constexpr int kGmThreads = 32 * (kGmEpiWarp0 + 4 * kGmEpiGroups);
-constexpr int kGmStages = 4;                        // 64-column steps in flight
-constexpr int kGmMaxN = 192;
+constexpr int kGmStages = 3;                        // 128-column steps in flight
+constexpr int kGmMaxN = 160;
 constexpr int kGmMaxN32 = 64;                       // of split FP32 x: one 32-column piece per epilogue warpgroup
-constexpr int kGmSegment32 = 4;                     // its steps per accumulator
-constexpr int kGmStageB = kGmMaxN / 2 * 128;        // a CTA's half of a step of x: up to 96 rows x 64 columns
+constexpr int kGmSegment32 = 2;                     // its steps per accumulator
+constexpr int kGmHalfB = kGmMaxN / 2 * 128;         // a CTA's half of x's rows in a tile, 64 columns of them
+constexpr int kGmStageB = 2 * kGmHalfB;
 constexpr int kGmRawStages = 3;                     // 256 columns of packed weights each
 constexpr int kGmRawBytes = 128 * 128;
 constexpr int kGmRawScales = 128 * 16;
@@ -64,7 +65,7 @@ constexpr int kGmBars = 2 * kGmStages + 2 * kGmRawStages + 2 + 2 + 1;
 constexpr int kGmOffTiles = kGmOffBars + kGmBars * 8 + 24;
 constexpr size_t kGmSmem = 1024 + kGmOffTiles + sizeof(int) * (kLinMaxGroups + 1);
 static_assert(kGmOffTiles % 4 == 0 && kGmSmem <= 232448, "shared memory overflow");
-static_assert(kGmColA + 32 * kGmStages <= 512, "tensor memory overflow");
+static_assert(kGmColA + 64 * kGmStages <= 512, "tensor memory overflow");
 static_assert(kGmRawBytes % 1024 == 0 && kGmOffRaw % 1024 == 0 && kGmRaw % 1024 == 0, "swizzled tiles need 1024-byte alignment");
 
 enum GemmWaitSite : int {
@@ -84,7 +85,7 @@ struct GemmArgs {
     int segment;             // steps per accumulator
     int m_pairs;             // pairs of weight tiles of a group
     int raw_steps;           // 256-column steps over K
-    int k_steps;             // 64-column steps over K
+    int k_steps;             // 128-column steps over K
     int wide_out, wide_res;  // four outputs may move as one vector
 };
 
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i) {
-            mbar_init(full + i, 1 + 4 + (rank == 0 ? 1 : 0));
+            mbar_init(full + i, 1 + 8 + (rank == 0 ? 1 : 0));
             mbar_init(empty + i, 1);
         }
         for (int i = 0; i < R; ++i) {
@@ -329,11 +330,14 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                 }
                 uint8_t *b = smem + kGmOffB + st * kGmStageB;
                 if (tc::elect_one()) {
-                    mbar_arrive_expect_tx(full + st, kTerms * boxes * a.box_rows * 128);
+                    mbar_arrive_expect_tx(full + st, 2 * kTerms * boxes * a.box_rows * 128);
                     for (int j = 0; j < kTerms; ++j)
-                        for (int x = 0; x < boxes; ++x)
-                            tma_load_2d(b + (j * (kGmMaxN32 / 2) + x * a.box_rows) * 128, &tm_x, full + st, ks * 128,
-                                        j * f.vectors + row0 + x * a.box_rows);
+                        for (int x = 0; x < boxes; ++x) {
+                            uint8_t *to = b + (j * (kGmMaxN32 / 2) + x * a.box_rows) * 128;
+                            const int row = j * f.vectors + row0 + x * a.box_rows;
+                            tma_load_2d(to, &tm_x, full + st, ks * 256, row);
+                            tma_load_2d(to + kGmHalfB, &tm_x, full + st, ks * 256 + 128, row);
+                        }
                 }
                 __syncwarp();
             }
@@ -372,7 +376,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
     } else if (warp == 1) {
         // ---------------------------------------------------------- MMA
         // Everything an instruction takes is the same in every lane and known to be (reductions, loop counters).
-        const uint32_t base = smem_u32(smem) + kGmOffB;
+        const uint64_t desc = tc::smem_desc_sw128(smem_u32(smem) + kGmOffB);  // its address field cannot overflow
         const int last = __reduce_max_sync(0xffffffffu, items);
         uint32_t st = 0, ph = 0;
         bool ok = true;
@@ -402,28 +406,36 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                         ok = false;
                         break;
                     }
-                    const int steps = min(left, a.segment);
                     uint32_t more = 0;
-                    for (int ks = 0; ks < steps; ++ks) {
-                        if (!wait_warp(full + st, ph, err, kSiteFusedFull)) {
-                            ok = false;
-                            break;
-                        }
-                        tc::fence_after_sync();
-                        if (tc::elect_one()) {
+                    // Unrolled over the ring, so that barriers and descriptors are constants away from a base (230
+                    // against 150 cycles of a step's issue, measured alone).
+                    for (int todo = min(left, a.segment); todo > 0 && ok;) {
 #pragma unroll
-                            for (int j = 0; j < kTerms; ++j)
+                        for (int stage = 0; stage < S; ++stage) {
+                            if (st != stage || todo == 0 || !ok) continue;
+                            if (!wait_warp(full + stage, ph, err, kSiteFusedFull)) {
+                                ok = false;
+                                continue;
+                            }
+                            tc::fence_after_sync();
+                            if (tc::elect_one()) {
 #pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    tc::mma_16bit_ts_pair(
-                                        acc, tmem + kGmColA + 32 * st + 8 * i,
-                                        tc::smem_desc_sw128(base + st * kGmStageB + j * (kGmMaxN32 / 2) * 128 + 32 * i),
-                                        idesc, (j | i) != 0 ? 1u : more);
-                            tc::commit_pair(empty + st);
+                                for (int j = 0; j < kTerms; ++j)
+#pragma unroll
+                                    for (int i = 0; i < 8; ++i)
+                                        tc::mma_16bit_ts_pair(
+                                            acc, tmem + kGmColA + 64 * stage + 8 * i,
+                                            desc + ((stage * kGmStageB + (i >> 2) * kGmHalfB + j * (kGmMaxN32 / 2) * 128 +
+                                                     32 * (i & 3)) >> 4),
+                                            idesc, (j | i) != 0 ? 1u : more);
+                                tc::commit_pair(empty + stage);
+                            }
+                            __syncwarp();
+                            more = 1;
+                            --todo;
+                            st = (stage + 1) % S;
+                            if (stage + 1 == S) ph ^= 1;
                         }
-                        __syncwarp();
-                        more = 1;
-                        if (++st == S) st = 0, ph ^= 1;
                     }
                     if (ok && tc::elect_one()) tc::commit_pair(acc_full + buf);
                     __syncwarp();
@@ -439,7 +451,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         __syncwarp();
     } else if (warp >= kGmConvWarp0 && warp < kGmEpiWarp0) {
         // --------------------------------------------------- conversion
-        const uint32_t mine = (warp - kGmConvWarp0) >> 2;  // steps it with it % groups == mine
+        const uint32_t mine = (warp - kGmConvWarp0) >> 2;  // half steps it with it % groups == mine
         const int quarter = warp & 3;
         // Row of the raw tile that this lane decodes into its tensor-memory lane.
         const int row = f.gated ? (lane & 15) + 16 * quarter + (lane >= 16 ? 64 : 0) : 32 * quarter + lane;
@@ -447,14 +459,14 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         uint32_t it = 0, rt = 0, next = mine;
         bool ok = true;
         for (int item = pair; item < items && ok; item += pairs) {
-            for (int ks0 = 0; ks0 < a.k_steps && ok; ks0 += 4, ++rt) {
+            for (int ks0 = 0; ks0 < a.k_steps && ok; ks0 += 2, ++rt) {
                 const int rs = rt % R;
                 if (!wait_warp(raw_full + rs, (rt / R) & 1u, err, kSiteFusedRawFull)) {
                     ok = false;
                     break;
                 }
                 const uint8_t *raw = smem + kGmOffRaw + rs * kGmRaw;
-                const uint32_t end = it + min(4, a.k_steps - ks0);
+                const uint32_t end = it + 2 * min(2, a.k_steps - ks0);
                 for (; next < end; next += kGmConvGroups) {
                     const int j = next - it;
                     const uint32_t word = *reinterpret_cast<const uint32_t *>(raw + kGmRawBytes + row * 16 + 4 * j);
@@ -471,13 +483,13 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                     decode8<kBf16>(q1.y, s2, r + 20);
                     decode8<kBf16>(q1.z, s3, r + 24);
                     decode8<kBf16>(q1.w, s3, r + 28);
-                    const int st = next % S;
-                    if (!wait_warp(empty + st, ((next / S) & 1u) ^ 1u, err, kSiteFusedEmpty)) {
+                    const int st = (next >> 1) % S;
+                    if (!wait_warp(empty + st, (((next >> 1) / S) & 1u) ^ 1u, err, kSiteFusedEmpty)) {
                         ok = false;
                         break;
                     }
                     tc::fence_after_sync();
-                    tc::st_32x32b_x32(lanes + 32 * st, r);
+                    tc::st_32x32b_x32(lanes + 64 * st + 32 * (next & 1), r);
                     tc::wait_st();
                     tc::fence_before_sync();
                     __syncwarp();
@@ -686,13 +698,13 @@ void launch_linear_gemm(const FusedLinearArgs &f, const nvfp4_matrix &matrix, vo
     const int terms = f.type == NVFP4_TYPE_F32 ? 2 : 1;  // 16-bit parts of x
     g.max_n = f.type == NVFP4_TYPE_F32 ? kGmMaxN32 : kGmMaxN;
     g.m_pairs = f.gated ? (f.out_rows + 127) / 128 : (f.rows + 255) / 256;
-    g.k_steps = (f.cols + 63) / 64;
+    g.k_steps = (f.cols + 127) / 128;
     g.raw_steps = (f.cols + 255) / 256;
     g.segment = f.type == NVFP4_TYPE_F32 ? kGmSegment32 : g.k_steps;
-    // One box for half of the even tiles of a single group; 32 rows (16 where groups have few) for ranges known on the
+    // One box for half of the even tiles of a single group; 16 rows for ranges known on the
     // device.
     const int tiles = (f.vectors + g.max_n - 1) / g.max_n;
-    g.box_rows = f.offsets ? ((long long)f.vectors <= 32LL * f.groups || f.type == NVFP4_TYPE_F32 ? 16 : 32)
+    g.box_rows = f.offsets ? ((long long)f.vectors <= 32LL * f.groups || f.type == NVFP4_TYPE_F32 ? 16 : 16)
                            : ((f.vectors + tiles - 1) / tiles + 15) / 16 * 8;
     const int e = f.type == NVFP4_TYPE_F32 ? 4 : 2;
     auto vectors_of_4 = [&](const void *p, long long stride) {
