@@ -8,7 +8,7 @@
 //   dst[v, r] = (1 / weight_global_scale) *
 //               sum_c E2M1(W[r, c]) * E4M3(S[r, c / 16]) * x[v, c].
 //
-// Storage (device, owned by the matrix): packed E2M1 rows padded to a 16-byte
+// Storage (device, owned by the matrix): packed E2M1 rows padded to a 32-byte
 // pitch, scale rows padded to a 16-byte pitch, both zero-filled beyond the
 // row, scale bytes sanitised at upload like the bank's (sign cleared, 0x7F ->
 // 0: the lab's decoding rule, nvfp4_gemv.cl:14-27).
@@ -318,7 +318,7 @@ extern "C" NVFP4_API nvfp4_status nvfp4_matrix_upload(nvfp4_runtime *runtime, co
         m->runtime = runtime;
         m->rows = rows;
         m->cols = cols;
-        m->packed_pitch = static_cast<int>((row_packed + 15) / 16 * 16);
+        m->packed_pitch = packed_pitch_of(cols);
         m->scale_pitch = static_cast<int>((row_scales + 15) / 16 * 16);
         m->inv_global = 1.0f / weight_global_scale;
         std::vector<uint8_t> sanitized(static_cast<size_t>(rows) * m->scale_pitch, 0);

@@ -77,13 +77,9 @@ const char *fused_args(FusedLinearArgs &a, const nvfp4_runtime *runtime, const n
     return nullptr;
 }
 
-// Few rows stream the weights through the GEMV kernel, more go to the tensor
-// memory kernel (average rows of a group, since the counts are on the device).
-bool few_rows(int vectors, int groups) { return vectors <= 32LL * groups; }
-
 nvfp4_status run_fused(nvfp4_runtime *runtime, const nvfp4_matrix *matrix, const FusedLinearArgs &a, void *workspace,
                        size_t workspace_bytes, void *stream, const char *operation) {
-    const bool few = few_rows(a.vectors, a.offsets ? a.groups : 1);
+    const bool few = linear_gemv_serves(a);
     if (!few && workspace_bytes < linear_gemm_workspace(a.type, a.x, a.x_stride, a.vectors, a.cols))
         return fail_invalid("the linear's workspace is too small (nvfp4_linear_workspace_bytes)");
     if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail_invalid("the linear's workspace must be 256-byte aligned");
@@ -131,7 +127,7 @@ extern "C" NVFP4_API nvfp4_status nvfp4_matrix_upload_grouped(nvfp4_runtime *run
         m->groups = groups;
         m->rows = rows;
         m->cols = cols;
-        m->packed_pitch = static_cast<int>((row_packed + 15) / 16 * 16);
+        m->packed_pitch = packed_pitch_of(cols);
         m->scale_pitch = static_cast<int>((row_scales + 15) / 16 * 16);
         const size_t packed_total = static_cast<size_t>(all_rows) * m->packed_pitch;
         std::lock_guard<std::mutex> lock(runtime->queue_mutex);
@@ -178,7 +174,15 @@ extern "C" NVFP4_API nvfp4_status nvfp4_matrix_upload_grouped(nvfp4_runtime *run
 
 extern "C" NVFP4_API size_t nvfp4_linear_workspace_bytes(const nvfp4_matrix *matrix, const void *x, int type,
                                                          int64_t x_stride, int vectors, int grouped) {
-    if (!matrix || !valid_type(type) || vectors <= 0 || few_rows(vectors, grouped ? matrix->groups : 1)) return 0;
+    if (!matrix || !valid_type(type) || vectors <= 0) return 0;
+    FusedLinearArgs a{};
+    a.type = type;
+    a.vectors = vectors;
+    a.cols = matrix->cols;
+    a.groups = matrix->groups;
+    static const int any = 0;
+    a.offsets = grouped ? &any : nullptr;  // only whether there are offsets counts here
+    if (linear_gemv_serves(a)) return 0;
     return linear_gemm_workspace(type, x, x_stride, vectors, matrix->cols);
 }
 

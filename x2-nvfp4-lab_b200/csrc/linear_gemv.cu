@@ -1,13 +1,13 @@
 // NVFP4 linear with epilogue for few rows: a weight stream.
 //
 // A warp owns 16 weight rows (with a gate eight gate rows and their eight up
-// rows, so that a lane holds both) and 128 columns at a time: lane (g, t)
-// loads 16 bytes (32 columns) of rows g and g + 8, decodes them to FP16 in
-// registers (E2M1 x E4M3 is exact there) and feeds them straight into
-// mma.sync m16n8k16 as the A operand; the rows of x, as FP16 in shared memory,
-// are its B columns. The order of K inside an MMA is free as long as both
-// operands agree: MMA i of a chunk takes columns 32 t + 4 i .. + 3 of lane t's
-// 32, so that a lane's 16 bytes feed eight MMAs without a shuffle.
+// rows, so that a lane holds both) and 256 columns at a time: lane (g, t)
+// loads 32 bytes (64 columns) of rows g and g + 8 and their four block scales,
+// decodes them to FP16 in registers (E2M1 x E4M3 is exact there) and feeds
+// them straight into mma.sync m16n8k16 as the A operand; the rows of x, as
+// FP16 in shared memory, are its B columns. The order of K inside an MMA is
+// free as long as both operands agree: an MMA takes four consecutive columns
+// of each lane's 64, so that a lane's 32 bytes feed 16 MMAs without a shuffle.
 //
 // Rows of x in FP16: FP16 as they are; BF16 scaled by a power of two per row
 // (largest finite value to [2^14, 2^15)), which is exact for every element
@@ -15,13 +15,13 @@
 // FP32 scaled the same way as two columns, high and low half (22 bits and a
 // sign, 2^-23 of an element). The scale comes back in the epilogue.
 //
-// Every 256 columns the MMAs' sums are added to FP32 registers: the tensor
+// Every 512 columns the MMAs' sums are added to FP32 registers: the tensor
 // core rounds its running sum towards zero, which over long rows would grow
 // into a bias.
 //
 // Bound by the weight stream (9/16 byte a weight) and, on B200, nearly as
-// much by the decode: about 12 instructions per lane and eight weights. Loads
-// run one batch (256 columns) ahead of the arithmetic. K is split over the
+// much by the decode (80 weights per cycle and SM with nothing else to do; HBM
+// brings 41). Two batches of loads are in flight per warp. K is split over the
 // warps of a CTA when there are too few row tiles to give every warp its own;
 // their sums meet in shared memory in warp order.
 #include "linear_fused.cuh"
@@ -34,151 +34,196 @@ namespace {
 
 constexpr int kGvThreads = 256;
 constexpr int kGvWarps = kGvThreads / 32;
-constexpr int kGvBatch = 2;                        // 128-column chunks loaded together
+constexpr int kGvCols = 8;                          // columns of an MMA: rows of x, or halves of FP32 rows
 constexpr int kGvRedPitch = 20;                    // floats per column of a partial tile: conflict-free stores
 constexpr size_t kGvSmem = 232448;                 // shared memory of a CTA
 
 struct GemvArgs {
     FusedLinearArgs f;
-    int chunks;       // 128-column chunks
+    int chunks;       // 256-column chunks
     int tiles;        // 16-row weight tiles of a group (eight outputs each with a gate)
     int warps_k;      // warps that share a tile's columns (a power of two)
-    int units;        // ceil(tiles / (warps / warps_k)): tiles a CTA takes together
     int pass_rows;    // rows of x staged at a time
     int pass_cols;    // their MMA columns (two per row for FP32)
     int token_stride; // bytes of a staged column
 };
 
+// A lane's part of 16 rows x 256 columns: 64 codes and four scales of two rows.
 struct Batch {
-    uint4 q[kGvBatch][2];
-    uint16_t s[kGvBatch][2];
+    uint32_t q[2][8];
+    uint32_t s[2];
 };
 
-__device__ __forceinline__ float finite_abs_bits(float v) {
+__device__ __forceinline__ void load_codes(const uint8_t *p, uint32_t (&q)[8]) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7])
+                 : "l"(p));
+}
+
+__device__ __forceinline__ uint32_t load_scales(const uint8_t *p) {
+    uint32_t s;
+    asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(s) : "l"(p));  // volatile: not moved to its use
+    return s;
+}
+
+// Byte of column octet `o` in a staged row: lane quarter t = (o / 8) % 4 has 128 of every 640 bytes, 160 apart, and
+// staged rows are 16 bytes apart modulo 128, so the LDS.128 of a B fragment (two rows, four quarters per phase) touches
+// eight different 16-byte units, at constant offsets from one address per lane.
+constexpr int kGvStagedChunk = 640;
+__device__ __forceinline__ int staged_byte(int o) {
+    return (o >> 5) * kGvStagedChunk + ((o >> 3) & 3) * 160 + (o & 7) * 16;
+}
+
+// mma_16816 with a zero addend.
+__device__ __forceinline__ void mma_16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+__device__ __forceinline__ float finite_abs(float v) {
     const float m = fabsf(v);
     return m <= 3.402823466e38f ? m : 0.0f;  // infinities and NaN do not set the scale
 }
 
-// Eight consecutive elements of a row of x as FP32.
+// Eight consecutive elements of a row of x as they lie in memory.
 template <int TYPE>
-__device__ __forceinline__ void load8(const FusedLinearArgs &f, long long row, int col, bool wide, float (&v)[8]) {
-    const size_t at = (size_t)(row * f.x_stride + col);
-    if constexpr (TYPE == NVFP4_TYPE_F32) {
-        const float *p = static_cast<const float *>(f.x) + at;
-        if (wide) {
-            const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __ldg(p + i);
-        }
-    } else {
-        const uint16_t *p = static_cast<const uint16_t *>(f.x) + at;
-        uint16_t h[8];
-        if (wide) {
-            const uint4 w = __ldg(reinterpret_cast<const uint4 *>(p));
-            memcpy(h, &w, 16);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) h[i] = __ldg(p + i);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = TYPE == NVFP4_TYPE_F16 ? __half2float(__ushort_as_half(h[i])) : bf16_bits_to_f32(h[i]);
+struct Octet {
+    static constexpr int kWords = TYPE == NVFP4_TYPE_F32 ? 8 : 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (TYPE == NVFP4_TYPE_F32) return __uint_as_float(w[i]);
+        const uint32_t h = (w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu;
+        return TYPE == NVFP4_TYPE_F16 ? __half2float(__ushort_as_half((uint16_t)h)) : bf16_bits_to_f32(h);
     }
+};
+
+template <int TYPE>
+__device__ __forceinline__ Octet<TYPE> load_octet(const FusedLinearArgs &f, long long row, int col, bool wide) {
+    Octet<TYPE> v;
+    const size_t at = (size_t)(row * f.x_stride + col);
+    if (wide) {
+        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(f.x) + at * (TYPE == NVFP4_TYPE_F32 ? 4 : 2));
+#pragma unroll
+        for (int i = 0; i < Octet<TYPE>::kWords / 4; ++i) {
+            const uint4 q = __ldg(p + i);
+            v.w[4 * i] = q.x, v.w[4 * i + 1] = q.y, v.w[4 * i + 2] = q.z, v.w[4 * i + 3] = q.w;
+        }
+    } else if constexpr (TYPE == NVFP4_TYPE_F32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v.w[i] = __ldg(static_cast<const uint32_t *>(f.x) + at + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            v.w[i] = (uint32_t)__ldg(static_cast<const uint16_t *>(f.x) + at + 2 * i) |
+                     ((uint32_t)__ldg(static_cast<const uint16_t *>(f.x) + at + 2 * i + 1) << 16);
+    }
+    return v;
 }
 
-// Rows [row0, row0 + n) of x as FP16 columns in shared memory, and their scales.
+// One octet as FP16 (FP32: high and low halves) at its place, scaled by its row's power of two.
+template <int TYPE>
+__device__ __forceinline__ void stage_octet(const GemvArgs &a, uint8_t *xs, const uint32_t *amax, float *back, int r, int o,
+                                            const Octet<TYPE> &v) {
+    uint8_t *to = xs + (TYPE == NVFP4_TYPE_F32 ? 2 * r : r) * a.token_stride + staged_byte(o);
+    if constexpr (TYPE == NVFP4_TYPE_F16) {
+        *reinterpret_cast<uint4 *>(to) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+        if (o == 0) back[r] = 1.0f;
+        return;
+    }
+    // 2^(14 - e) with e the exponent of the row's largest finite value, kept where both it and its inverse are normal
+    // numbers.
+    const uint32_t top = amax[r];
+    const int e = top ? max((int)(top >> 23) - 127, -112) : 14;
+    const float scale = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+    if (o == 0) back[r] = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        hi[j] = lo[j] = 0;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const float y = v.get(2 * j + b) * scale;
+            const __half h = __float2half_rn(y);
+            hi[j] |= (uint32_t)__half_as_ushort(h) << (16 * b);
+            if constexpr (TYPE == NVFP4_TYPE_F32)
+                lo[j] |= (uint32_t)__half_as_ushort(__float2half_rn(fabsf(y) <= 65504.0f ? y - __half2float(h) : 0.0f)) << (16 * b);
+        }
+    }
+    *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if constexpr (TYPE == NVFP4_TYPE_F32)
+        *reinterpret_cast<uint4 *>(to + a.token_stride) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+}
+
+// Rows [row0, row0 + n) of x as FP16 columns in shared memory, and their scales. A warp's 32 octets are of one row
+// (rows are padded to 256 columns). What a thread loads for the rows' maxima it keeps for the conversion; where that
+// does not fit its registers the rows are read a second time.
 template <int TYPE>
 __device__ __forceinline__ void stage_rows(const GemvArgs &a, uint8_t *xs, uint32_t *amax, float *back, int row0, int n) {
+    constexpr int kHeld = 16 / Octet<TYPE>::kWords;
     const FusedLinearArgs &f = a.f;
-    const int oct = a.chunks * 16, valid = f.cols / 8;  // groups of eight columns, padded and real
+    const int oct = a.chunks * 32, valid = f.cols / 8;  // groups of eight columns, padded and real
+    const int items = n * oct;
     const bool wide = ((reinterpret_cast<uintptr_t>(f.x) | (uintptr_t)(f.x_stride * (TYPE == NVFP4_TYPE_F32 ? 4 : 2))) & 15u) == 0;
+    const bool once = items <= kHeld * kGvThreads;
+    Octet<TYPE> v[kHeld];
+    auto load_held = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) {
+            const int i = i0 + u * kGvThreads, r = i / oct, o = i - r * oct;
+            if (i < items && o < valid) {
+                v[u] = load_octet<TYPE>(f, row0 + r, o * 8, wide);
+            } else {
+#pragma unroll
+                for (int j = 0; j < Octet<TYPE>::kWords; ++j) v[u].w[j] = 0u;
+            }
+        }
+    };
     if constexpr (TYPE != NVFP4_TYPE_F16) {
         for (int i = threadIdx.x; i < n; i += kGvThreads) amax[i] = 0u;
         __syncthreads();
-        // Whole warps per (row, 32 groups): one shared-memory maximum per warp.
-        const int spans = (valid + 31) / 32;
-        for (int i = threadIdx.x >> 5; i < n * spans; i += kGvWarps) {
-            const int r = i / spans, o = (i - r * spans) * 32 + (threadIdx.x & 31);
-            float m = 0.0f;
-            if (o < valid) {
-                float v[8];
-                load8<TYPE>(f, row0 + r, o * 8, wide, v);
+        for (int i0 = threadIdx.x; i0 < items; i0 += kHeld * kGvThreads) {
+            load_held(i0);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs_bits(v[j]));
+            for (int u = 0; u < kHeld; ++u) {
+                const int i = i0 + u * kGvThreads;
+                if (i >= items) break;
+                float m = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(v[u].get(j)));
+                const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+                if ((threadIdx.x & 31) == 0) atomicMax(amax + i / oct, top);
             }
-            const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
-            if ((threadIdx.x & 31) == 0) atomicMax(amax + r, top);
         }
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < n * oct; i += kGvThreads) {
-        const int r = i / oct, o = i - r * oct;
-        float v[8];
-        if (o < valid) {
-            load8<TYPE>(f, row0 + r, o * 8, wide, v);
-        } else {
+    for (int i0 = threadIdx.x; i0 < items; i0 += kHeld * kGvThreads) {
+        if (TYPE == NVFP4_TYPE_F16 || !once) load_held(i0);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-        }
-        const int off = act_tile_offset(0, 0, o >> 4, (o >> 2) & 3, o & 3);
-        uint32_t hi[4], lo[4];
-        if constexpr (TYPE == NVFP4_TYPE_F16) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) hi[j] = __half_as_ushort(__float2half_rn(v[2 * j])) |
-                                               ((uint32_t)__half_as_ushort(__float2half_rn(v[2 * j + 1])) << 16);
-            *reinterpret_cast<uint4 *>(xs + r * a.token_stride + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            if (o == 0) back[r] = 1.0f;
-        } else {
-            // 2^(14 - e) with e the exponent of the row's largest finite value, kept where both it and its inverse
-            // are normal numbers.
-            const uint32_t top = amax[r];
-            const int e = top ? max((int)(top >> 23) - 127, -112) : 14;
-            const float scale = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-            if (o == 0) back[r] = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t h2 = 0, l2 = 0;
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const float y = v[2 * j + b] * scale;
-                    const __half h = __float2half_rn(y);
-                    h2 |= (uint32_t)__half_as_ushort(h) << (16 * b);
-                    if constexpr (TYPE == NVFP4_TYPE_F32) {
-                        const bool fin = fabsf(y) <= 65504.0f;
-                        l2 |= (uint32_t)__half_as_ushort(__float2half_rn(fin ? y - __half2float(h) : 0.0f)) << (16 * b);
-                    }
-                }
-                hi[j] = h2;
-                lo[j] = l2;
-            }
-            if constexpr (TYPE == NVFP4_TYPE_F32) {
-                *reinterpret_cast<uint4 *>(xs + (2 * r) * a.token_stride + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<uint4 *>(xs + (2 * r + 1) * a.token_stride + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            } else {
-                *reinterpret_cast<uint4 *>(xs + r * a.token_stride + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            }
+        for (int u = 0; u < kHeld; ++u) {
+            const int i = i0 + u * kGvThreads, r = i / oct;
+            if (i < items) stage_octet<TYPE>(a, xs, amax, back, r, i - r * oct, v[u]);
         }
     }
     __syncthreads();
 }
 
-template <int NT, int TYPE>
-__global__ void __launch_bounds__(kGvThreads) linear_gemv_kernel(const __grid_constant__ GemvArgs a) {
-    constexpr int kCols = 8 * NT;
+template <int TYPE>
+__global__ void __launch_bounds__(kGvThreads, 2) linear_gemv_kernel(const __grid_constant__ GemvArgs a) {
     extern __shared__ __align__(16) uint8_t gv_smem[];
     const FusedLinearArgs &f = a.f;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
-    const int warps_k = a.warps_k, tiles_at_once = kGvWarps / warps_k;
+    const int warps_k = a.warps_k, teams = kGvWarps / warps_k;
     const int kw = warp & (warps_k - 1), wr = warp / warps_k;
 
     uint8_t *xs = gv_smem;
-    float *red = reinterpret_cast<float *>(gv_smem + (size_t)a.pass_cols * a.token_stride);  // [2][warps][kCols][pitch]
-    uint32_t *amax = reinterpret_cast<uint32_t *>(red + 2 * kGvWarps * kCols * kGvRedPitch);
-    float *back = reinterpret_cast<float *>(amax + kCols);
-    int *active = reinterpret_cast<int *>(back + kCols);  // [groups] groups with rows (grouped calls)
+    float *red = reinterpret_cast<float *>(gv_smem + (size_t)a.pass_cols * a.token_stride);  // [2][warps][kGvCols][pitch]
+    uint32_t *amax = reinterpret_cast<uint32_t *>(red + 2 * kGvWarps * kGvCols * kGvRedPitch);
+    float *back = reinterpret_cast<float *>(amax + kGvCols);
+    int *active = reinterpret_cast<int *>(back + kGvCols);  // [groups] groups with rows (grouped calls)
     __shared__ int warp_sum[kGvWarps];
     __shared__ int s_active;
 
@@ -213,17 +258,18 @@ __global__ void __launch_bounds__(kGvThreads) linear_gemv_kernel(const __grid_co
         n_active = s_active;
     }
 
-    const long long work = (long long)n_active * a.units;
+    // This CTA's row tiles: a run of (group, tile), taken in turn by its teams of warps_k warps.
+    const long long work = (long long)n_active * a.tiles;
     long long u = work * blockIdx.x / gridDim.x;
     const long long u_end = work * (blockIdx.x + 1) / gridDim.x;
-    const int batches = ((a.chunks + warps_k - 1) / warps_k + kGvBatch - 1) / kGvBatch;
+    const int batches = ((a.chunks - kw + warps_k - 1) / warps_k + 1) & ~1;  // of this warp; even: two buffers in turn
     int parity = 0;
 
     while (u < u_end) {
-        const int ai = (int)(u / a.units);
-        const int unit0 = (int)(u - (long long)ai * a.units);
-        const int unit1 = (int)min((long long)a.units, unit0 + (u_end - u));
-        u += unit1 - unit0;
+        const int ai = (int)(u / a.tiles);
+        const int tile0 = (int)(u - (long long)ai * a.tiles);
+        const int tile1 = (int)min((long long)a.tiles, tile0 + (u_end - u));
+        u += tile1 - tile0;
         const int group = f.offsets ? active[ai] : 0;
         int first, count;
         group_range(f, group, &first, &count);
@@ -231,132 +277,155 @@ __global__ void __launch_bounds__(kGvThreads) linear_gemv_kernel(const __grid_co
         const uint8_t *scales = f.scales + (size_t)group * f.rows * f.scale_pitch;
         const float inv = f.inv_globals ? __ldg(f.inv_globals + group) : f.inv_global;
 
-        // Weight rows of this lane in tile `tile`, clamped to the last row (its sums are not stored).
-        auto rows_of = [&](int tile, int &r0, int &r1) {
-            if (f.gated) {
-                r0 = min(tile * 8 + g, f.out_rows - 1);
-                r1 = r0 + f.out_rows;
-            } else {
-                r0 = min(tile * 16 + g, f.rows - 1);
-                r1 = min(tile * 16 + g + 8, f.rows - 1);
-            }
-        };
-        auto load = [&](Batch &b, int unit, int batch) {
-            int r0, r1;
-            rows_of(unit * tiles_at_once + wr, r0, r1);
-#pragma unroll
-            for (int i = 0; i < kGvBatch; ++i) {
-                const int c = (batch * kGvBatch + i) * warps_k + kw;
-                const int byte = c * 64 + t * 16;
-                const bool in = byte < f.packed_pitch;
-                b.q[i][0] = in ? ldg_stream128(packed + (size_t)r0 * f.packed_pitch + byte) : make_uint4(0, 0, 0, 0);
-                b.q[i][1] = in ? ldg_stream128(packed + (size_t)r1 * f.packed_pitch + byte) : make_uint4(0, 0, 0, 0);
-                b.s[i][0] = in ? ldg_u16(scales + (size_t)r0 * f.scale_pitch + c * 8 + t * 2) : (uint16_t)0;
-                b.s[i][1] = in ? ldg_u16(scales + (size_t)r1 * f.scale_pitch + c * 8 + t * 2) : (uint16_t)0;
-            }
-        };
-
         for (int v0 = 0; v0 < count; v0 += a.pass_rows) {
             const int n = min(a.pass_rows, count - v0);
             const int ncols = TYPE == NVFP4_TYPE_F32 ? 2 * n : n;
-            Batch cur;
-            load(cur, unit0, 0);
+
+            // The loads run ahead of the arithmetic: (l_tile, l_batch) is the next batch to request.
+            // A lane's chunks end with its row's pitch (zero scales follow the last column, whatever codes the padding
+            // holds); past it the scales are set to zero and nothing is read.
+            int l_tile = tile0 + wr, l_batch = 0, l_chunk = kw;
+            const int lane_chunks = (f.packed_pitch - t * 32 + 127) / 128;
+            const uint8_t *p0, *p1, *s0, *s1;
+            auto set_rows = [&]() {
+                // Rows of this lane, clamped to the last (its sums are not stored).
+                int r0, r1;
+                if (f.gated) {
+                    r0 = min(l_tile * 8 + g, f.out_rows - 1);
+                    r1 = r0 + f.out_rows;
+                } else {
+                    r0 = min(l_tile * 16 + g, f.rows - 1);
+                    r1 = min(l_tile * 16 + g + 8, f.rows - 1);
+                }
+                p0 = packed + (size_t)r0 * f.packed_pitch + kw * 128 + t * 32;
+                p1 = packed + (size_t)r1 * f.packed_pitch + kw * 128 + t * 32;
+                s0 = scales + (size_t)r0 * f.scale_pitch + kw * 16 + t * 4;
+                s1 = scales + (size_t)r1 * f.scale_pitch + kw * 16 + t * 4;
+                l_batch = 0;
+                l_chunk = l_tile < tile1 ? kw : a.chunks;
+            };
+            set_rows();
+            auto load = [&](Batch &b) {
+                if (l_chunk < lane_chunks) {
+                    load_codes(p0, b.q[0]);
+                    load_codes(p1, b.q[1]);
+                    b.s[0] = load_scales(s0);
+                    b.s[1] = load_scales(s1);
+                } else {
+                    b.s[0] = b.s[1] = 0u;
+                }
+                if (++l_batch == batches) {
+                    l_tile += teams;
+                    set_rows();
+                } else {
+                    p0 += warps_k * 128;
+                    p1 += warps_k * 128;
+                    s0 += warps_k * 16;
+                    s1 += warps_k * 16;
+                    l_chunk += warps_k;
+                }
+            };
+            Batch b0, b1;
+            load(b0);
+            load(b1);
             __syncthreads();  // the rows staged before are no longer read
             stage_rows<TYPE>(a, xs, amax, back, first + v0, n);
             // MMA columns past the staged ones repeat the last: their sums are not stored.
-            const uint8_t *bcol[NT];
-#pragma unroll
-            for (int j = 0; j < NT; ++j) bcol[j] = xs + min(8 * j + g, ncols - 1) * a.token_stride + t * 64;
+            const uint8_t *bcol = xs + min(g, ncols - 1) * a.token_stride + t * 160;
 
-            for (int unit = unit0; unit < unit1; ++unit, parity ^= 1) {
-                float sum[NT][4];
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+
+            // One output from its sum (and its up sum with a gate).
+            auto output = [&](int row, int v, float z, float z_up) {
+                const float scale = inv * back[v];
+                z *= scale;
+                const size_t at = (size_t)group * f.rows + row;
+                if (f.bias) z += load_as_f32(f.bias, f.bias_type, at);
+                z = activate(z, f.act);
+                if (f.gated) {
+                    z_up *= scale;
+                    if (f.bias) z_up += load_as_f32(f.bias, f.bias_type, at + f.out_rows);
+                    z *= z_up;
+                }
+                const long long vec = (long long)first + v0 + v;
+                if (f.residual) z += load_as_f32(f.residual, f.type, (size_t)(vec * f.residual_stride + row));
+                store_from_f32(f.out, f.type, (size_t)(vec * f.out_stride + row), z);
+            };
+            auto finish = [&](int tile) {
+                const int per_col = f.gated ? 8 : 16, row0 = tile * per_col;
+                if (warps_k == 1) {
+                    // The lane has rows g and g + 8 of MMA columns 2 t and 2 t + 1.
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sum[j][i] = 0.0f;
-                for (int batch = 0; batch < batches; ++batch) {
-                    Batch nxt;
-                    const bool more = batch + 1 < batches;
-                    if (more || unit + 1 < unit1) load(nxt, more ? unit : unit + 1, more ? batch + 1 : 0);
-                    float acc[NT][4];
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < kGvBatch; ++i) {
-                        const int c = (batch * kGvBatch + i) * warps_k + kw;
-                        if (c >= a.chunks) break;
-                        const uint32_t s0 = e4m3x2_to_f16x2(cur.s[i][0]), s1 = e4m3x2_to_f16x2(cur.s[i][1]);
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            const uint32_t q0 = w == 0 ? cur.q[i][0].x : w == 1 ? cur.q[i][0].y : w == 2 ? cur.q[i][0].z : cur.q[i][0].w;
-                            const uint32_t q1 = w == 0 ? cur.q[i][1].x : w == 1 ? cur.q[i][1].y : w == 2 ? cur.q[i][1].z : cur.q[i][1].w;
-                            const uint32_t k0 = w < 2 ? f16x2_lo_lo(s0) : f16x2_hi_hi(s0);
-                            const uint32_t k1 = w < 2 ? f16x2_lo_lo(s1) : f16x2_hi_hi(s1);
-                            uint32_t h0[4], h1[4];
-                            e2m1x8_to_f16x8(q0, h0);
-                            e2m1x8_to_f16x8(q1, h1);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                h0[e] = hmul2_u32(h0[e], k0);
-                                h1[e] = hmul2_u32(h1[e], k1);
-                            }
-#pragma unroll
-                            for (int j = 0; j < NT; ++j) {
-                                const uint4 b = *reinterpret_cast<const uint4 *>(bcol[j] + c * 256 + ((w ^ (t >> 1)) << 4));
-                                mma_16816(acc[j], h0[0], h1[0], h0[1], h1[1], b.x, b.y);
-                                mma_16816(acc[j], h0[2], h1[2], h0[3], h1[3], b.z, b.w);
-                            }
+                    for (int b = 0; b < (TYPE == NVFP4_TYPE_F32 ? 1 : 2); ++b) {
+                        const int v = TYPE == NVFP4_TYPE_F32 ? t : 2 * t + b;
+                        if (v >= n) continue;
+                        const float z = TYPE == NVFP4_TYPE_F32 ? sum[0] + sum[1] : sum[b];
+                        const float y = TYPE == NVFP4_TYPE_F32 ? sum[2] + sum[3] : sum[2 + b];
+                        if (row0 + g < f.out_rows) output(row0 + g, v, z, y);
+                        if (!f.gated && row0 + g + 8 < f.out_rows) output(row0 + g + 8, v, y, 0.0f);
+                    }
+                } else {
+                    // Partial tiles meet in shared memory; the warps of a tile share its epilogue.
+                    float *p = red + ((size_t)parity * kGvWarps + warp) * kGvCols * kGvRedPitch + 2 * t * kGvRedPitch + g;
+                    p[0] = sum[0];
+                    p[kGvRedPitch] = sum[1];
+                    p[8] = sum[2];
+                    p[kGvRedPitch + 8] = sum[3];
+                    named_barrier(1 + wr, warps_k * 32);
+                    const float *part = red + ((size_t)parity * kGvWarps + wr * warps_k) * kGvCols * kGvRedPitch;
+                    for (int i = kw * 32 + lane; i < n * per_col; i += warps_k * 32) {
+                        const int v = f.gated ? i >> 3 : i >> 4, r = i & (per_col - 1);
+                        if (row0 + r >= f.out_rows) continue;
+                        const int c0 = (TYPE == NVFP4_TYPE_F32 ? 2 * v : v) * kGvRedPitch + r;
+                        float z = 0.0f, z_up = 0.0f;
+                        for (int k = 0; k < warps_k; ++k) {
+                            const float *q = part + (size_t)k * kGvCols * kGvRedPitch + c0;
+                            z += TYPE == NVFP4_TYPE_F32 ? q[0] + q[kGvRedPitch] : q[0];
+                            if (f.gated) z_up += TYPE == NVFP4_TYPE_F32 ? q[8] + q[kGvRedPitch + 8] : q[8];
                         }
+                        output(row0 + r, v, z, z_up);
                     }
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) sum[j][i] += acc[j][i];
-                    if (more || unit + 1 < unit1) cur = nxt;
+                    parity ^= 1;
                 }
-
-                // Partial tiles meet in shared memory; the warps of a tile share its epilogue.
-                float *mine = red + ((size_t)parity * kGvWarps + warp) * kCols * kGvRedPitch;
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    float *p = mine + (8 * j + 2 * t) * kGvRedPitch + g;
-                    p[0] = sum[j][0];
-                    p[kGvRedPitch] = sum[j][1];
-                    p[8] = sum[j][2];
-                    p[kGvRedPitch + 8] = sum[j][3];
-                }
-                if (warps_k > 1) named_barrier(1 + wr, warps_k * 32);
-                else __syncwarp();
-                const int tile = unit * tiles_at_once + wr;
-                const int per_col = f.gated ? 8 : 16;
-                const float *part = red + ((size_t)parity * kGvWarps + wr * warps_k) * kCols * kGvRedPitch;
-                for (int i = kw * 32 + lane; i < n * per_col; i += warps_k * 32) {
-                    const int v = i / per_col, r = i - v * per_col;
-                    const int row = tile * per_col + r;
-                    if (row >= f.out_rows) continue;
-                    const int c0 = (TYPE == NVFP4_TYPE_F32 ? 2 * v : v) * kGvRedPitch + r;
-                    float z = 0.0f, z_up = 0.0f;
-                    for (int k = 0; k < warps_k; ++k) {
-                        const float *p = part + (size_t)k * kCols * kGvRedPitch + c0;
-                        z += TYPE == NVFP4_TYPE_F32 ? p[0] + p[kGvRedPitch] : p[0];
-                        if (f.gated) z_up += TYPE == NVFP4_TYPE_F32 ? p[8] + p[kGvRedPitch + 8] : p[8];
+                for (int i = 0; i < 4; ++i) sum[i] = 0.0f;
+            };
+            auto step = [&](const Batch &b, int c, float (&acc)[2][4], bool fresh) {
+                const uint32_t f0[2] = {e4m3x2_to_f16x2((uint16_t)b.s[0]), e4m3x2_to_f16x2((uint16_t)(b.s[0] >> 16))};
+                const uint32_t f1[2] = {e4m3x2_to_f16x2((uint16_t)b.s[1]), e4m3x2_to_f16x2((uint16_t)(b.s[1] >> 16))};
+#pragma unroll
+                for (int w = 0; w < 8; ++w) {
+                    const uint32_t k0 = (w & 2) ? f16x2_hi_hi(f0[w >> 2]) : f16x2_lo_lo(f0[w >> 2]);
+                    const uint32_t k1 = (w & 2) ? f16x2_hi_hi(f1[w >> 2]) : f16x2_lo_lo(f1[w >> 2]);
+                    uint32_t h0[4], h1[4];
+                    e2m1x8_to_f16x8(b.q[0][w], h0);
+                    e2m1x8_to_f16x8(b.q[1][w], h1);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        h0[e] = hmul2_u32(h0[e], k0);
+                        h1[e] = hmul2_u32(h1[e], k1);
                     }
-                    const float scale = inv * back[v];
-                    z *= scale;
-                    const size_t b0 = (size_t)group * f.rows + row;
-                    if (f.bias) z += load_as_f32(f.bias, f.bias_type, b0);
-                    z = activate(z, f.act);
-                    if (f.gated) {
-                        z_up *= scale;
-                        if (f.bias) z_up += load_as_f32(f.bias, f.bias_type, b0 + f.out_rows);
-                        z *= z_up;
+                    const uint4 x = *reinterpret_cast<const uint4 *>(bcol + c * kGvStagedChunk + w * 16);
+                    if (fresh && w == 0) {
+                        mma_16816_first(acc[0], h0[0], h1[0], h0[1], h1[1], x.x, x.y);
+                        mma_16816_first(acc[1], h0[2], h1[2], h0[3], h1[3], x.z, x.w);
+                    } else {
+                        mma_16816(acc[0], h0[0], h1[0], h0[1], h1[1], x.x, x.y);
+                        mma_16816(acc[1], h0[2], h1[2], h0[3], h1[3], x.z, x.w);
                     }
-                    const long long vec = (long long)first + v0 + v;
-                    if (f.residual) z += load_as_f32(f.residual, f.type, (size_t)(vec * f.residual_stride + row));
-                    store_from_f32(f.out, f.type, (size_t)(vec * f.out_stride + row), z);
                 }
+            };
+            for (int tile = tile0 + wr; tile < tile1; tile += teams) {
+                for (int c = kw; c < a.chunks; c += 2 * warps_k) {
+                    float acc[2][4];  // two chains
+                    step(b0, c, acc, true);
+                    load(b0);
+                    if (c + warps_k < a.chunks) step(b1, c + warps_k, acc, false);
+                    load(b1);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[i] += acc[0][i] + acc[1][i];
+                }
+                finish(tile);
             }
         }
     }
@@ -364,56 +433,63 @@ __global__ void __launch_bounds__(kGvThreads) linear_gemv_kernel(const __grid_co
 }
 
 // Shared memory besides the staged rows: partial tiles, scales, the list of groups.
-size_t other_smem(const FusedLinearArgs &f, int nt) {
-    return sizeof(float) * 2 * kGvWarps * 8 * nt * kGvRedPitch + 8 * 8 * nt + (f.offsets ? sizeof(int) * f.groups : 0);
-}
-
-template <int NT, int TYPE>
-void launch(GemvArgs &a, int sm_count, cudaStream_t stream) {
-    const size_t smem = (size_t)a.pass_cols * a.token_stride + other_smem(a.f, NT);
-    check_cuda(cudaFuncSetAttribute(linear_gemv_kernel<NT, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(smem)),
-               "cudaFuncSetAttribute(linear_gemv_kernel)");
-    int per_sm = 0;
-    check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, linear_gemv_kernel<NT, TYPE>, kGvThreads, smem),
-               "cudaOccupancyMaxActiveBlocksPerMultiprocessor(linear_gemv_kernel)");
-    const long long work = (long long)a.units * (a.f.offsets ? std::min(a.f.groups, a.f.vectors) : 1);
-    const int grid = static_cast<int>(std::max<long long>(1, std::min<long long>(work, (long long)sm_count * std::max(1, per_sm))));
-    linear_gemv_kernel<NT, TYPE><<<grid, kGvThreads, smem, stream>>>(a);
-    check_cuda(cudaGetLastError(), "linear_gemv_kernel");
+size_t other_smem(const FusedLinearArgs &f) {
+    return sizeof(float) * 2 * kGvWarps * kGvCols * kGvRedPitch + 8 * kGvCols + (f.offsets ? sizeof(int) * f.groups : 0);
 }
 
 template <int TYPE>
-void launch_type(GemvArgs &a, int nt, int sm_count, cudaStream_t stream) {
-    if (nt == 1) launch<1, TYPE>(a, sm_count, stream);
-    else if (nt == 2) launch<2, TYPE>(a, sm_count, stream);
-    else launch<4, TYPE>(a, sm_count, stream);
+void launch(GemvArgs &a, int sm_count, cudaStream_t stream) {
+    const size_t smem = (size_t)a.pass_cols * a.token_stride + other_smem(a.f);
+    check_cuda(cudaFuncSetAttribute(linear_gemv_kernel<TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    static_cast<int>(smem)),
+               "cudaFuncSetAttribute(linear_gemv_kernel)");
+    int per_sm = 0;
+    check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, linear_gemv_kernel<TYPE>, kGvThreads, smem),
+               "cudaOccupancyMaxActiveBlocksPerMultiprocessor(linear_gemv_kernel)");
+    const long long teams = kGvWarps / a.warps_k;
+    const long long work = ((long long)a.tiles * (a.f.offsets ? std::min(a.f.groups, a.f.vectors) : 1) + teams - 1) / teams;
+    const long long grid = std::min(work, (long long)sm_count * std::max(1, per_sm));
+    linear_gemv_kernel<TYPE><<<static_cast<int>(std::max<long long>(1, grid)), kGvThreads, smem, stream>>>(a);
+    check_cuda(cudaGetLastError(), "linear_gemv_kernel");
+}
+
+// Shared memory of a staged MMA column.
+int column_bytes(int cols) { return (cols + 255) / 256 * kGvStagedChunk + 16; }
+
+// Rows of x whose MMA columns fit shared memory.
+int staged_rows(const FusedLinearArgs &f) {
+    return static_cast<int>((kGvSmem - other_smem(f)) / column_bytes(f.cols)) / (f.type == NVFP4_TYPE_F32 ? 2 : 1);
 }
 
 }  // namespace
 
+// One group of eight MMA columns: eight rows of x, four of FP32 (high and low halves). Measured at 2048 x 16384 weights:
+// 8 rows 15.0 us, 12 rows 19.7 us, against 14.4 us for the tensor-memory kernel at any count up to 64; at 2048 x 2048
+// 9.0 and 11.6 against 13.3 us. Groups of rows whose counts are on the device go by their average: 256 groups of 1024
+// rows run 76 us at three rows a group and 100 us at four, against 113 us; 32 groups 27 and 33 us against 21 us.
+bool linear_gemv_serves(const FusedLinearArgs &f) {
+    const int per_row = f.type == NVFP4_TYPE_F32 ? 2 : 1;
+    return staged_rows(f) >= 1 && (f.offsets ? (long long)f.vectors * per_row <= 3LL * f.groups : f.vectors * per_row <= 8);
+}
+
 void launch_linear_gemv(const FusedLinearArgs &f, int sm_count, cudaStream_t stream) {
     GemvArgs a{};
     a.f = f;
-    a.chunks = (f.cols + 127) / 128;
+    a.chunks = (f.cols + 255) / 256;
     a.tiles = f.gated ? (f.out_rows + 7) / 8 : (f.rows + 15) / 16;
-    a.token_stride = act_tile_stride_bytes(a.chunks * 128);
+    a.token_stride = column_bytes(f.cols);
     const int per_row = f.type == NVFP4_TYPE_F32 ? 2 : 1;
-    // Columns of the MMAs: enough for the call's rows, at most 32; as many staged rows as shared memory holds.
-    auto fit = [&](int nt) { return static_cast<int>((kGvSmem - other_smem(f, nt)) / a.token_stride) / per_row; };
-    const int want = f.offsets ? std::max(1, (f.vectors + f.groups - 1) / f.groups * 2) : f.vectors;
-    int nt = 1;
-    while (nt < 4 && 8 * nt / per_row < want && fit(2 * nt) > 8 * nt / per_row) nt *= 2;
-    a.pass_rows = std::max(1, std::min({8 * nt / per_row, fit(nt), f.vectors}));
+    // Groups may have more rows than their average: further rows in further passes. (MMA columns for 16 rows made every
+    // pass slower: a batch of 32 tokens over 256 groups 91 against 54 us.)
+    a.pass_rows = std::max(1, std::min({8 / per_row, staged_rows(f), f.vectors}));
     a.pass_cols = a.pass_rows * per_row;
-    // Each warp its own tile when that fills the GPU four times over; else the warps of a CTA split K.
+    // As few warps share a tile as leave every team (of two CTAs on an SM) eight tiles to even out their times.
     const long long tiles = (long long)a.tiles * (f.offsets ? std::min(f.groups, f.vectors) : 1);
-    a.warps_k = kGvWarps;
-    while (a.warps_k > 1 && (a.warps_k > a.chunks || tiles * a.warps_k > (long long)sm_count * 64)) a.warps_k >>= 1;
-    a.units = (a.tiles + kGvWarps / a.warps_k - 1) / (kGvWarps / a.warps_k);
-    if (f.type == NVFP4_TYPE_BF16) launch_type<NVFP4_TYPE_BF16>(a, nt, sm_count, stream);
-    else if (f.type == NVFP4_TYPE_F16) launch_type<NVFP4_TYPE_F16>(a, nt, sm_count, stream);
-    else launch_type<NVFP4_TYPE_F32>(a, nt, sm_count, stream);
+    a.warps_k = 1;
+    while (a.warps_k < kGvWarps && 2 * a.warps_k <= a.chunks && tiles * a.warps_k < (long long)sm_count * 16 * 4) a.warps_k *= 2;
+    if (f.type == NVFP4_TYPE_BF16) launch<NVFP4_TYPE_BF16>(a, sm_count, stream);
+    else if (f.type == NVFP4_TYPE_F16) launch<NVFP4_TYPE_F16>(a, sm_count, stream);
+    else launch<NVFP4_TYPE_F32>(a, sm_count, stream);
 }
 
 }  // namespace nvfp4

@@ -12,7 +12,7 @@ struct nvfp4_matrix {
     int groups = 1;        // weight matrices of the same shape, one after the other
     int rows = 0;          // per group
     int cols = 0;
-    int packed_pitch = 0;  // bytes per packed row (multiple of 16)
+    int packed_pitch = 0;  // bytes per packed row (multiple of 32: one load of a lane)
     int scale_pitch = 0;   // bytes per scale row (multiple of 16)
     uint8_t *packed = nullptr;   // [groups * rows][packed_pitch]
     uint8_t *scales = nullptr;   // [groups * rows][scale_pitch]
@@ -38,6 +38,8 @@ struct nvfp4_matrix {
 namespace nvfp4 {
 
 constexpr int kLinMaxCols = 49152;
+
+inline int packed_pitch_of(int cols) { return (cols / 2 + 31) / 32 * 32; }
 
 // The tensor maps of a matrix whose arrays are allocated.
 inline void make_matrix_maps(nvfp4_matrix &m) {
