@@ -12,9 +12,9 @@
 // every lane quarter.
 //
 // Warps: 0 producer of x and 2 of weights (TMA), 1 MMA issuer, 4-15 conversion
-// (three warpgroups, every third 64 columns each), 16-23 epilogue (two
+// (three warpgroups, every third step of 128 columns each), 16-23 epilogue (two
 // warpgroups, every other 32 columns each). Tensor memory: two accumulators of
-// 160 columns, and three decoded steps of 64. The epilogue turns 32 columns at
+// 160 columns and three decoded steps of 64, or of 64 columns and six. The epilogue turns 32 columns at
 // a time through shared memory, so that a lane has four consecutive outputs of
 // one row of x: bias in registers, residual and stores as vectors.
 //
@@ -44,29 +44,34 @@ namespace {
 constexpr int kGmConvWarp0 = 4, kGmConvGroups = 3, kGmEpiWarp0 = kGmConvWarp0 + 4 * kGmConvGroups;
 constexpr int kGmEpiGroups = 2;
 constexpr int kGmThreads = 32 * (kGmEpiWarp0 + 4 * kGmEpiGroups);
-constexpr int kGmStages = 3;                        // 128-column steps in flight
-constexpr int kGmMaxN = 160;
-constexpr int kGmMaxN32 = 64;                       // of split FP32 x: one 32-column piece per epilogue warpgroup
-constexpr int kGmSegment32 = 2;                     // its steps per accumulator
-constexpr int kGmHalfB = kGmMaxN / 2 * 128;         // a CTA's half of x's rows in a tile, 64 columns of them
-constexpr int kGmStageB = 2 * kGmHalfB;
-constexpr int kGmRawStages = 3;                     // 256 columns of packed weights each
-constexpr int kGmRawBytes = 128 * 128;
+constexpr int kGmLargeN = 160;                      // rows of x per tile
+constexpr int kGmSmallN = 64;                       // of calls with few, and of split FP32 x (32 per epilogue warpgroup)
+constexpr int kGmSegment32 = 2;                     // steps per accumulator of split FP32 x
+constexpr int kGmRawBytes = 128 * 128;              // 256 columns of packed weights
 constexpr int kGmRawScales = 128 * 16;
 constexpr int kGmRaw = kGmRawBytes + kGmRawScales;
 constexpr int kGmEpiPitch = 148;                    // floats per row of x in the epilogue's turn
 constexpr int kGmEpiBytes = 32 * kGmEpiPitch * 4;
-constexpr int kGmColA = 2 * kGmMaxN;                // tensor-memory column of the first decoded step
-constexpr int kGmOffB = 0;
-constexpr int kGmOffRaw = kGmOffB + kGmStages * kGmStageB;
-constexpr int kGmOffEpi = kGmOffRaw + kGmRawStages * kGmRaw;
-constexpr int kGmOffBars = kGmOffEpi + kGmEpiGroups * kGmEpiBytes;
-constexpr int kGmBars = 2 * kGmStages + 2 * kGmRawStages + 2 + 2 + 1;
-constexpr int kGmOffTiles = kGmOffBars + kGmBars * 8 + 24;
-constexpr size_t kGmSmem = 1024 + kGmOffTiles + sizeof(int) * (kLinMaxGroups + 1);
-static_assert(kGmOffTiles % 4 == 0 && kGmSmem <= 232448, "shared memory overflow");
-static_assert(kGmColA + 64 * kGmStages <= 512, "tensor memory overflow");
-static_assert(kGmRawBytes % 1024 == 0 && kGmOffRaw % 1024 == 0 && kGmRaw % 1024 == 0, "swizzled tiles need 1024-byte alignment");
+
+// Tiles of up to N rows of x: tensor memory holds two accumulators of N columns and decoded weights in the rest, so
+// small tiles have six 128-column steps in flight, large ones three.
+template <int N, int TERMS>
+struct Shape {
+    static constexpr int kStages = (512 - 2 * N) / 64;
+    static constexpr int kHalfB = TERMS * N / 2 * 128;  // a CTA's half of x's rows in a tile, 64 columns of them
+    static constexpr int kStageB = 2 * kHalfB;
+    static constexpr int kRawStages = TERMS == 1 ? 6 : 4;  // 18 KB of weights each, as many as fit
+    static constexpr int kColA = 2 * N;              // tensor-memory column of the first decoded step
+    static constexpr int kOffRaw = kStages * kStageB;
+    static constexpr int kOffEpi = kOffRaw + kRawStages * kGmRaw;
+    static constexpr int kOffBars = kOffEpi + kGmEpiGroups * kGmEpiBytes;
+    static constexpr int kBars = 2 * kStages + 2 * kRawStages + 2 + 2 + 1;
+    static constexpr int kOffTiles = kOffBars + kBars * 8 + 24;
+    static constexpr size_t kSmem = 1024 + kOffTiles + sizeof(int) * (kLinMaxGroups + 1);
+    static_assert(kOffTiles % 4 == 0 && kSmem <= 232448, "shared memory overflow");
+    static_assert(kColA + 64 * kStages <= 512, "tensor memory overflow");
+    static_assert(kHalfB % 1024 == 0 && kOffRaw % 1024 == 0 && kGmRaw % 1024 == 0, "swizzled tiles need 1024-byte alignment");
+};
 
 enum GemmWaitSite : int {
     kSiteFusedEmpty = 71,
@@ -234,26 +239,27 @@ __device__ __forceinline__ void finish_page(const GemmArgs &a, const float *page
 }
 
 // TYPE: of x, residual and out; FP32 x arrives as FP16 parts.
-template <int TYPE>
+template <int TYPE, int N>
 __global__ void __launch_bounds__(kGmThreads, 1)
     linear_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_s,
                        const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ GemmArgs a) {
     constexpr bool kBf16 = TYPE == NVFP4_TYPE_BF16;
     constexpr int kTerms = TYPE == NVFP4_TYPE_F32 ? 2 : 1;
-    constexpr int S = kGmStages, R = kGmRawStages;
+    using Z = Shape<N, kTerms>;
+    constexpr int S = Z::kStages, R = Z::kRawStages;
     extern __shared__ uint8_t gm_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(gm_smem_raw) + 1023) & ~uintptr_t(1023));
     const FusedLinearArgs &f = a.f;
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + kGmOffBars);    // [S] rows of x have landed, weights are decoded (four warps); even CTA: and the odd one's have
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + Z::kOffBars);    // [S] rows of x have landed, weights are decoded (four warps); even CTA: and the odd one's have
     uint64_t *empty = full + S;                                          // [S] the step's MMAs are done with both
     uint64_t *raw_full = empty + S;                                      // [R] packed weights and scales have landed
-    uint64_t *raw_empty = raw_full + R;                                  // [R] (every conversion warp)
+    uint64_t *raw_empty = raw_full + R;                                  // [R] (four conversion warps for each of its two steps)
     uint64_t *acc_full = raw_empty + R;                                  // [2]
     uint64_t *acc_empty = acc_full + 2;                                  // [2] (every epilogue warp of both CTAs; even CTA)
     uint64_t *drain = acc_empty + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     int *acc_ok = reinterpret_cast<int *>(tmem_slot + 1);                // [epilogue warpgroups]
-    int *upto = reinterpret_cast<int *>(smem + kGmOffTiles);             // [groups + 1] x tiles of the groups before
+    int *upto = reinterpret_cast<int *>(smem + Z::kOffTiles);             // [groups + 1] x tiles of the groups before
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int *err = f.err;
     const uint32_t rank = cluster_rank();
@@ -261,12 +267,12 @@ __global__ void __launch_bounds__(kGmThreads, 1)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i) {
-            mbar_init(full + i, 1 + 8 + (rank == 0 ? 1 : 0));
+            mbar_init(full + i, 1 + 4 + (rank == 0 ? 1 : 0));
             mbar_init(empty + i, 1);
         }
         for (int i = 0; i < R; ++i) {
             mbar_init(raw_full + i, 1);
-            mbar_init(raw_empty + i, 4 * kGmConvGroups);
+            mbar_init(raw_empty + i, 2 * 4);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(acc_full + i, 1);
@@ -328,15 +334,15 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                     ok = false;
                     break;
                 }
-                uint8_t *b = smem + kGmOffB + st * kGmStageB;
+                uint8_t *b = smem + st * Z::kStageB;
                 if (tc::elect_one()) {
                     mbar_arrive_expect_tx(full + st, 2 * kTerms * boxes * a.box_rows * 128);
                     for (int j = 0; j < kTerms; ++j)
                         for (int x = 0; x < boxes; ++x) {
-                            uint8_t *to = b + (j * (kGmMaxN32 / 2) + x * a.box_rows) * 128;
+                            uint8_t *to = b + (j * (kGmSmallN / 2) + x * a.box_rows) * 128;
                             const int row = j * f.vectors + row0 + x * a.box_rows;
                             tma_load_2d(to, &tm_x, full + st, ks * 256, row);
-                            tma_load_2d(to + kGmHalfB, &tm_x, full + st, ks * 256 + 128, row);
+                            tma_load_2d(to + Z::kHalfB, &tm_x, full + st, ks * 256 + 128, row);
                         }
                 }
                 __syncwarp();
@@ -359,7 +365,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                     ok = false;
                     break;
                 }
-                uint8_t *raw = smem + kGmOffRaw + st * kGmRaw;
+                uint8_t *raw = smem + Z::kOffRaw + st * kGmRaw;
                 if (tc::elect_one()) {
                     mbar_arrive_expect_tx(raw_full + st, kGmRaw);
                     tma_load_2d(raw, &tm_w, raw_full + st, rs * 128, w0);
@@ -376,7 +382,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
     } else if (warp == 1) {
         // ---------------------------------------------------------- MMA
         // Everything an instruction takes is the same in every lane and known to be (reductions, loop counters).
-        const uint64_t desc = tc::smem_desc_sw128(smem_u32(smem) + kGmOffB);  // its address field cannot overflow
+        const uint64_t desc = tc::smem_desc_sw128(smem_u32(smem));  // its address field cannot overflow
         const int last = __reduce_max_sync(0xffffffffu, items);
         uint32_t st = 0, ph = 0;
         bool ok = true;
@@ -401,7 +407,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                 const uint32_t n = __reduce_max_sync(0xffffffffu, tile_of(a, upto, item).n);
                 const uint32_t idesc = tc::idesc_16bit_pair((n + 15) & ~15u, kBf16 ? 1u : 0u);
                 for (int left = a.k_steps; left > 0 && ok; left -= a.segment, ++use) {
-                    const uint32_t buf = use & 1, acc = tmem + buf * kGmMaxN;
+                    const uint32_t buf = use & 1, acc = tmem + buf * N;
                     if (use > 1 && !wait_warp(acc_empty + buf, ((use >> 1) - 1) & 1u, err, kSiteFusedAccEmpty)) {
                         ok = false;
                         break;
@@ -424,8 +430,8 @@ __global__ void __launch_bounds__(kGmThreads, 1)
 #pragma unroll
                                     for (int i = 0; i < 8; ++i)
                                         tc::mma_16bit_ts_pair(
-                                            acc, tmem + kGmColA + 64 * stage + 8 * i,
-                                            desc + ((stage * kGmStageB + (i >> 2) * kGmHalfB + j * (kGmMaxN32 / 2) * 128 +
+                                            acc, tmem + Z::kColA + 64 * stage + 8 * i,
+                                            desc + ((stage * Z::kStageB + (i >> 2) * Z::kHalfB + j * (kGmSmallN / 2) * 128 +
                                                      32 * (i & 3)) >> 4),
                                             idesc, (j | i) != 0 ? 1u : more);
                                 tc::commit_pair(empty + stage);
@@ -451,30 +457,33 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         __syncwarp();
     } else if (warp >= kGmConvWarp0 && warp < kGmEpiWarp0) {
         // --------------------------------------------------- conversion
-        const uint32_t mine = (warp - kGmConvWarp0) >> 2;  // half steps it with it % groups == mine
+        const int mine = (warp - kGmConvWarp0) >> 2;  // the warpgroup's first step
         const int quarter = warp & 3;
         // Row of the raw tile that this lane decodes into its tensor-memory lane.
         const int row = f.gated ? (lane & 15) + 16 * quarter + (lane >= 16 ? 64 : 0) : 32 * quarter + lane;
-        const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16) + kGmColA;
-        uint32_t it = 0, rt = 0, next = mine;
+        const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16) + Z::kColA;
+        uint32_t it = 0, rt = 0;  // steps and raw stages of the tiles before
+        int ks = mine;
         bool ok = true;
         for (int item = pair; item < items && ok; item += pairs) {
-            for (int ks0 = 0; ks0 < a.k_steps && ok; ks0 += 2, ++rt) {
-                const int rs = rt % R;
-                if (!wait_warp(raw_full + rs, (rt / R) & 1u, err, kSiteFusedRawFull)) {
+            for (; ks < a.k_steps; ks += kGmConvGroups) {
+                const uint32_t step = it + ks, raw_no = rt + (ks >> 1);
+                const int st = step % S, rs = raw_no % R;
+                if (!wait_warp(raw_full + rs, (raw_no / R) & 1u, err, kSiteFusedRawFull)) {
                     ok = false;
                     break;
                 }
-                const uint8_t *raw = smem + kGmOffRaw + rs * kGmRaw;
-                const uint32_t end = it + 2 * min(2, a.k_steps - ks0);
-                for (; next < end; next += kGmConvGroups) {
-                    const int j = next - it;
-                    const uint32_t word = *reinterpret_cast<const uint32_t *>(raw + kGmRawBytes + row * 16 + 4 * j);
-                    const uint4 q0 = *reinterpret_cast<const uint4 *>(raw + row * 128 + (((2 * j) ^ (row & 7)) << 4));
-                    const uint4 q1 = *reinterpret_cast<const uint4 *>(raw + row * 128 + (((2 * j + 1) ^ (row & 7)) << 4));
-                    uint32_t r[32];
+                const uint8_t *raw = smem + Z::kOffRaw + rs * kGmRaw;
+                const uint2 sc = *reinterpret_cast<const uint2 *>(raw + kGmRawBytes + row * 16 + 8 * (ks & 1));
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int unit = 4 * (ks & 1) + 2 * half;  // 16-byte unit of the row's 128
+                    const uint4 q0 = *reinterpret_cast<const uint4 *>(raw + row * 128 + ((unit ^ (row & 7)) << 4));
+                    const uint4 q1 = *reinterpret_cast<const uint4 *>(raw + row * 128 + (((unit + 1) ^ (row & 7)) << 4));
+                    const uint32_t word = half ? sc.y : sc.x;
                     const uint32_t s01 = e4m3x2_to_f16x2((uint16_t)word), s23 = e4m3x2_to_f16x2((uint16_t)(word >> 16));
                     const uint32_t s0 = f16x2_lo_lo(s01), s1 = f16x2_hi_hi(s01), s2 = f16x2_lo_lo(s23), s3 = f16x2_hi_hi(s23);
+                    uint32_t r[32];
                     decode8<kBf16>(q0.x, s0, r);
                     decode8<kBf16>(q0.y, s0, r + 4);
                     decode8<kBf16>(q0.z, s1, r + 8);
@@ -483,28 +492,36 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                     decode8<kBf16>(q1.y, s2, r + 20);
                     decode8<kBf16>(q1.z, s3, r + 24);
                     decode8<kBf16>(q1.w, s3, r + 28);
-                    const int st = (next >> 1) % S;
-                    if (!wait_warp(empty + st, (((next >> 1) / S) & 1u) ^ 1u, err, kSiteFusedEmpty)) {
-                        ok = false;
-                        break;
+                    if (half == 0) {
+                        if (!wait_warp(empty + st, ((step / S) & 1u) ^ 1u, err, kSiteFusedEmpty)) {
+                            ok = false;
+                            break;
+                        }
+                        tc::fence_after_sync();
                     }
-                    tc::fence_after_sync();
-                    tc::st_32x32b_x32(lanes + 64 * st + 32 * (next & 1), r);
-                    tc::wait_st();
-                    tc::fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(full + st);
+                    tc::st_32x32b_x32(lanes + 64 * st + 32 * half, r);
                 }
+                if (!ok) break;
+                // The raw stage may be refilled; one that holds a row's last, odd step has no second reader.
                 __syncwarp();
-                if (lane == 0) mbar_arrive(raw_empty + rs);
-                it = end;
+                if (lane == 0) {
+                    mbar_arrive(raw_empty + rs);
+                    if ((ks & 1) == 0 && ks + 1 == a.k_steps) mbar_arrive(raw_empty + rs);
+                }
+                tc::wait_st();
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full + st);
             }
+            ks -= a.k_steps;
+            it += a.k_steps;
+            rt += a.raw_steps;
         }
     } else if (warp >= kGmEpiWarp0) {
         // ----------------------------------------------------- epilogue
         const int piece = (warp - kGmEpiWarp0) >> 2, quarter = warp & 3;
         const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
-        float *page = reinterpret_cast<float *>(smem + kGmOffEpi + piece * kGmEpiBytes);
+        float *page = reinterpret_cast<float *>(smem + Z::kOffEpi + piece * kGmEpiBytes);
         // Place of this lane's weight row in a turned row of x: gate rows first, the up rows 80 floats on.
         const int place = !f.gated ? 32 * quarter + lane : lane < 16 ? 16 * quarter + lane : 80 + 16 * quarter + lane - 16;
         // Outputs of this lane after the turn: four, of one row of x (with a gate 16 lanes cover a row).
@@ -564,7 +581,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                         break;
                     }
                     uint32_t r[32];
-                    tc::ld_32x32b_x32(lanes + (use & 1) * kGmMaxN + 32 * piece, r);
+                    tc::ld_32x32b_x32(lanes + (use & 1) * N + 32 * piece, r);
                     tc::wait_ld();
                     release();
 #pragma unroll
@@ -581,7 +598,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                 int c0 = 32 * piece;
                 for (; c0 < t.n; c0 += 32 * kGmEpiGroups) {
                     uint32_t r[32];
-                    tc::ld_32x32b_x32(lanes + (use & 1) * kGmMaxN + c0, r);
+                    tc::ld_32x32b_x32(lanes + (use & 1) * N + c0, r);
                     tc::wait_ld();
                     if (c0 + 32 * kGmEpiGroups >= t.n) release();
 #pragma unroll
@@ -661,16 +678,16 @@ size_t parts_bytes(int type, int vectors, int cols) {
     return ((size_t)vectors * cols * (type == NVFP4_TYPE_F32 ? 4 : 2) + 255) & ~size_t(255);
 }
 
-template <int TYPE>
+template <int TYPE, int N>
 void launch(const GemmArgs &g, const nvfp4_matrix &matrix, const CUtensorMap &map_x, int grid, bool dependent,
             cudaStream_t stream) {
-    check_cuda(cudaFuncSetAttribute(linear_gemm_kernel<TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(kGmSmem)),
+    check_cuda(cudaFuncSetAttribute(linear_gemm_kernel<TYPE, N>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    static_cast<int>(Shape<N, TYPE == NVFP4_TYPE_F32 ? 2 : 1>::kSmem)),
                "cudaFuncSetAttribute(linear_gemm_kernel)");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kGmThreads);
-    cfg.dynamicSmemBytes = kGmSmem;
+    cfg.dynamicSmemBytes = Shape<N, TYPE == NVFP4_TYPE_F32 ? 2 : 1>::kSmem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -680,7 +697,7 @@ void launch(const GemmArgs &g, const nvfp4_matrix &matrix, const CUtensorMap &ma
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = dependent ? 2 : 1;
-    check_cuda(cudaLaunchKernelEx(&cfg, linear_gemm_kernel<TYPE>, matrix.map_w, matrix.map_s, map_x, g),
+    check_cuda(cudaLaunchKernelEx(&cfg, linear_gemm_kernel<TYPE, N>, matrix.map_w, matrix.map_s, map_x, g),
                "linear_gemm_kernel");
 }
 
@@ -696,16 +713,15 @@ void launch_linear_gemm(const FusedLinearArgs &f, const nvfp4_matrix &matrix, vo
     GemmArgs g{};
     g.f = f;
     const int terms = f.type == NVFP4_TYPE_F32 ? 2 : 1;  // 16-bit parts of x
-    g.max_n = f.type == NVFP4_TYPE_F32 ? kGmMaxN32 : kGmMaxN;
+    const bool small = f.type == NVFP4_TYPE_F32 || (f.offsets ? (long long)f.vectors <= 32LL * f.groups : f.vectors <= kGmSmallN);
+    g.max_n = small ? kGmSmallN : kGmLargeN;
     g.m_pairs = f.gated ? (f.out_rows + 127) / 128 : (f.rows + 255) / 256;
     g.k_steps = (f.cols + 127) / 128;
     g.raw_steps = (f.cols + 255) / 256;
     g.segment = f.type == NVFP4_TYPE_F32 ? kGmSegment32 : g.k_steps;
-    // One box for half of the even tiles of a single group; 16 rows for ranges known on the
-    // device.
+    // One box for half of the even tiles of a single group; 16 rows for ranges known on the device.
     const int tiles = (f.vectors + g.max_n - 1) / g.max_n;
-    g.box_rows = f.offsets ? ((long long)f.vectors <= 32LL * f.groups || f.type == NVFP4_TYPE_F32 ? 16 : 16)
-                           : ((f.vectors + tiles - 1) / tiles + 15) / 16 * 8;
+    g.box_rows = f.offsets ? 16 : ((f.vectors + tiles - 1) / tiles + 15) / 16 * 8;
     const int e = f.type == NVFP4_TYPE_F32 ? 4 : 2;
     auto vectors_of_4 = [&](const void *p, long long stride) {
         return (reinterpret_cast<uintptr_t>(p) % (4 * e)) == 0 && stride % 4 == 0 ? 1 : 0;
@@ -739,9 +755,14 @@ void launch_linear_gemm(const FusedLinearArgs &f, const nvfp4_matrix &matrix, vo
     // Items the call can have: every group may end inside a tile.
     const long long x_tiles_most = tiles + (f.offsets ? std::min(f.groups, f.vectors) : 0);
     const int grid = 2 * static_cast<int>(std::min<long long>(sm_count / 2, x_tiles_most * g.m_pairs));
-    if (f.type == NVFP4_TYPE_BF16) launch<NVFP4_TYPE_BF16>(g, matrix, map_x, grid, !direct, stream);
-    else if (f.type == NVFP4_TYPE_F16) launch<NVFP4_TYPE_F16>(g, matrix, map_x, grid, !direct, stream);
-    else launch<NVFP4_TYPE_F32>(g, matrix, map_x, grid, !direct, stream);
+    if (f.type == NVFP4_TYPE_F32)
+        launch<NVFP4_TYPE_F32, kGmSmallN>(g, matrix, map_x, grid, !direct, stream);
+    else if (f.type == NVFP4_TYPE_BF16)
+        small ? launch<NVFP4_TYPE_BF16, kGmSmallN>(g, matrix, map_x, grid, !direct, stream)
+              : launch<NVFP4_TYPE_BF16, kGmLargeN>(g, matrix, map_x, grid, !direct, stream);
+    else
+        small ? launch<NVFP4_TYPE_F16, kGmSmallN>(g, matrix, map_x, grid, !direct, stream)
+              : launch<NVFP4_TYPE_F16, kGmLargeN>(g, matrix, map_x, grid, !direct, stream);
 }
 
 }  // namespace nvfp4
