@@ -206,36 +206,60 @@ __device__ __forceinline__ void store4(void *p, size_t at, bool wide, int valid,
         if (i < valid) store_from_f32(p, TYPE, at + i, v[i]);
 }
 
-// A turned page of up to 32 rows of x: scale, bias, activation, gate, residual, store. Lane: four outputs from `out0`.
-template <int TYPE, int ACT>
-__device__ __forceinline__ void finish_page(const GemmArgs &a, const float *page, int row0, int n, int first, int step,
-                                            int col, int out0, int valid, float inv, const float (&bias)[4],
+// A turned page of up to 32 rows of x: scale, bias, activation, gate, residual, store. A lane has four outputs (from
+// `out0`, `valid` of them) of every 4th row from `first` on, with a gate of every 8th; all of its shared-memory reads
+// are made before the first store.
+template <int TYPE, int ACT, bool GATED>
+__device__ __forceinline__ void finish_page(const GemmArgs &a, const float *page, int row0, int n, int first, int col,
+                                            int out0, int valid, float inv, const float (&bias)[4],
                                             const float (&bias_up)[4]) {
+    constexpr int kStep = GATED ? 8 : 4, kRows = 32 / kStep;
     const FusedLinearArgs &f = a.f;
     if (valid <= 0) return;
-#pragma unroll 4
-    for (int v = first; v < n; v += step) {
-        const long long row = (long long)row0 + v;
-        const float scale = a.row_scale ? inv * __ldcg(a.row_scale + row) : inv;
-        const float4 zg = *reinterpret_cast<const float4 *>(page + v * kGmEpiPitch + col);
-        float z[4] = {zg.x, zg.y, zg.z, zg.w};
+    float4 z[kRows], up[GATED ? kRows : 1];
+    float scale[kRows];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) z[i] = activate<ACT>(fmaf(z[i], scale, bias[i]));
-        if (f.gated) {
-            const float4 zu = *reinterpret_cast<const float4 *>(page + v * kGmEpiPitch + 80 + col);
-            z[0] *= fmaf(zu.x, scale, bias_up[0]);
-            z[1] *= fmaf(zu.y, scale, bias_up[1]);
-            z[2] *= fmaf(zu.z, scale, bias_up[2]);
-            z[3] *= fmaf(zu.w, scale, bias_up[3]);
-        }
-        if (f.residual) {
-            float res[4];
-            load4<TYPE>(f.residual, (size_t)(row * f.residual_stride + out0), a.wide_res, valid, res);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) z[i] += res[i];
-        }
-        store4<TYPE>(f.out, (size_t)(row * f.out_stride + out0), a.wide_out, valid, z);
+    for (int i = 0; i < kRows; ++i) {
+        const int v = first + i * kStep;
+        z[i] = *reinterpret_cast<const float4 *>(page + v * kGmEpiPitch + col);
+        if constexpr (GATED) up[i] = *reinterpret_cast<const float4 *>(page + v * kGmEpiPitch + 80 + col);
+        scale[i] = inv;
+        if (TYPE == NVFP4_TYPE_F32 && v < n) scale[i] = inv * __ldcg(a.row_scale + row0 + v);
     }
+    constexpr int kBytes = TYPE == NVFP4_TYPE_F32 ? 4 : 2;
+    uint8_t *out = static_cast<uint8_t *>(f.out) + ((row0 + first) * f.out_stride + out0) * kBytes;
+    const uint8_t *res = static_cast<const uint8_t *>(f.residual) + ((row0 + first) * f.residual_stride + out0) * kBytes;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        if (first + i * kStep < n) {
+            float y[4] = {z[i].x, z[i].y, z[i].z, z[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = activate<ACT>(fmaf(y[e], scale[i], bias[e]));
+            if constexpr (GATED) {
+                y[0] *= fmaf(up[i].x, scale[i], bias_up[0]);
+                y[1] *= fmaf(up[i].y, scale[i], bias_up[1]);
+                y[2] *= fmaf(up[i].z, scale[i], bias_up[2]);
+                y[3] *= fmaf(up[i].w, scale[i], bias_up[3]);
+            }
+            if (f.residual) {
+                float r[4];
+                load4<TYPE>(res, 0, a.wide_res, valid, r);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] += r[e];
+            }
+            store4<TYPE>(out, 0, a.wide_out, valid, y);
+        }
+        out += kStep * f.out_stride * kBytes;
+        res += kStep * f.residual_stride * kBytes;
+    }
+}
+
+template <int TYPE, int ACT>
+__device__ __forceinline__ void finish_page(const GemmArgs &a, const float *page, int row0, int n, int first, int col,
+                                            int out0, int valid, float inv, const float (&bias)[4],
+                                            const float (&bias_up)[4]) {
+    if (a.f.gated) finish_page<TYPE, ACT, true>(a, page, row0, n, first, col, out0, valid, inv, bias, bias_up);
+    else finish_page<TYPE, ACT, false>(a, page, row0, n, first, col, out0, valid, inv, bias, bias_up);
 }
 
 // TYPE: of x, residual and out; FP32 x arrives as FP16 parts.
@@ -527,7 +551,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         // Outputs of this lane after the turn: four, of one row of x (with a gate 16 lanes cover a row).
         const int lanes_row = f.gated ? 16 : 32;
         const int col = 4 * (lane & (lanes_row - 1));
-        const int vec0 = quarter * (f.gated ? 2 : 1) + (f.gated ? lane >> 4 : 0), vec_step = f.gated ? 8 : 4;
+        const int vec0 = quarter * (f.gated ? 2 : 1) + (f.gated ? lane >> 4 : 0);
         const int tile_rows = f.gated ? 64 : 128;
         int use = 0;
         // One thread waits, so that the four warps leave at the same place after a failure.
@@ -563,11 +587,11 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                 named_barrier(1 + piece, 128);
                 const int row0 = t.row0 + c0, n = min(32, t.n - c0);
                 switch (f.act) {
-                    case NVFP4_ACT_RELU: finish_page<TYPE, NVFP4_ACT_RELU>(a, page, row0, n, vec0, vec_step, col, out0, valid, inv, bias, bias_up); break;
-                    case NVFP4_ACT_SILU: finish_page<TYPE, NVFP4_ACT_SILU>(a, page, row0, n, vec0, vec_step, col, out0, valid, inv, bias, bias_up); break;
-                    case NVFP4_ACT_GELU: finish_page<TYPE, NVFP4_ACT_GELU>(a, page, row0, n, vec0, vec_step, col, out0, valid, inv, bias, bias_up); break;
-                    case NVFP4_ACT_GELU_TANH: finish_page<TYPE, NVFP4_ACT_GELU_TANH>(a, page, row0, n, vec0, vec_step, col, out0, valid, inv, bias, bias_up); break;
-                    default: finish_page<TYPE, NVFP4_ACT_NONE>(a, page, row0, n, vec0, vec_step, col, out0, valid, inv, bias, bias_up);
+                    case NVFP4_ACT_RELU: finish_page<TYPE, NVFP4_ACT_RELU>(a, page, row0, n, vec0, col, out0, valid, inv, bias, bias_up); break;
+                    case NVFP4_ACT_SILU: finish_page<TYPE, NVFP4_ACT_SILU>(a, page, row0, n, vec0, col, out0, valid, inv, bias, bias_up); break;
+                    case NVFP4_ACT_GELU: finish_page<TYPE, NVFP4_ACT_GELU>(a, page, row0, n, vec0, col, out0, valid, inv, bias, bias_up); break;
+                    case NVFP4_ACT_GELU_TANH: finish_page<TYPE, NVFP4_ACT_GELU_TANH>(a, page, row0, n, vec0, col, out0, valid, inv, bias, bias_up); break;
+                    default: finish_page<TYPE, NVFP4_ACT_NONE>(a, page, row0, n, vec0, col, out0, valid, inv, bias, bias_up);
                 }
                 named_barrier(1 + piece, 128);
             };
