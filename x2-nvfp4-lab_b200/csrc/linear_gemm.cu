@@ -13,7 +13,7 @@
 //
 // Warps: 0 producer of x and 2 of weights (TMA), 1 MMA issuer, 4-15 conversion
 // (three warpgroups, every third step of 128 columns each), 16-23 epilogue (two
-// warpgroups, every other 32 columns each). Tensor memory: two accumulators of
+// warpgroups). Tensor memory: two accumulators of
 // 160 columns and three decoded steps of 64, or of 64 columns and six. The epilogue turns 32 columns at
 // a time through shared memory, so that a lane has four consecutive outputs of
 // one row of x: bias in registers, residual and stores as vectors.
@@ -563,13 +563,24 @@ __global__ void __launch_bounds__(kGmThreads, 1)
             tc::fence_after_sync();
             return is;
         };
+        // With more tiles than pairs the warpgroups take whole tiles in turn (each its accumulator; what one waits for at
+        // the start of a tile hides behind the other's work), else every other 32 columns of the one tile. FP32 always
+        // does the latter: its sums are in registers.
+        const bool whole = TYPE != NVFP4_TYPE_F32 && items > pairs;
         auto release = [&]() {
             tc::fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive_at(acc_empty + (use & 1), 0);
+            if (lane == 0) {
+                mbar_arrive_at(acc_empty + (use & 1), 0);
+                if (whole) mbar_arrive_at(acc_empty + (use & 1), 0);  // for the other warpgroup
+            }
         };
         bool ok = true;
         for (int item = pair; item < items && ok; item += pairs) {
+            if (whole && (use & 1) != piece) {
+                ++use;
+                continue;
+            }
             const Tile t = tile_of(a, upto, item);
             const int out0 = t.m * tile_rows + col, valid = min(4, f.out_rows - out0);
             const float inv = f.inv_globals ? __ldg(f.inv_globals + t.group) : f.inv_global;
@@ -619,17 +630,17 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                 }
             } else {
                 if (!filled()) break;
-                int c0 = 32 * piece;
-                for (; c0 < t.n; c0 += 32 * kGmEpiGroups) {
+                const int step = whole ? 32 : 32 * kGmEpiGroups, c_first = whole ? 0 : 32 * piece;
+                for (int c0 = c_first; c0 < t.n; c0 += step) {
                     uint32_t r[32];
                     tc::ld_32x32b_x32(lanes + (use & 1) * N + c0, r);
                     tc::wait_ld();
-                    if (c0 + 32 * kGmEpiGroups >= t.n) release();
+                    if (c0 + step >= t.n) release();
 #pragma unroll
                     for (int i = 0; i < 32; ++i) page[i * kGmEpiPitch + place] = __uint_as_float(r[i]);
                     finish(c0);
                 }
-                if (32 * piece >= t.n) release();
+                if (c_first >= t.n) release();
                 ++use;
             }
         }
