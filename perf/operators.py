@@ -294,7 +294,7 @@ def run(s):
 
 
 def _own(s):
-    rt = _runtime
+    rt = _library()
     act = None if s.get("act") == "none" else s.get("act")
     if s["op"] == "linear":
         return rt.linear_fused(s["matrix"], s["x"], bias=s["bias_rows"], activation=act, residual=s["residual_rows"])
