@@ -436,13 +436,6 @@ NVFP4_API nvfp4_status nvfp4_linear_grouped(
 
 /* ------------------------------------------------- rows sorted by expert */
 
-/* additive: bytes of device workspace nvfp4_expert_sort needs (0 for few
- * picks). */
-NVFP4_API size_t nvfp4_expert_sort_workspace_bytes(
-    int tokens,
-    int topk,
-    int experts);
-
 /* additive: token rows copied to their experts' places. x [tokens, hidden] of
  * `type` (row stride in elements), ids [tokens, topk] of 4 or 8 bytes (row
  * stride in elements); an id outside [0, experts) drops its pick. Outputs
@@ -455,9 +448,8 @@ NVFP4_API size_t nvfp4_expert_sort_workspace_bytes(
  *   inverse  int32 [tokens, topk]: the row of each pick, -1 for a dropped one
  *   offsets  int32 [experts + 1]: each expert's first row, then the number of
  *            rows in use
- * topk <= 64, experts <= 1024, tokens * topk below 2^31 - 2048. Enqueued on `stream`
- * (NULL: the runtime's stream); the workspace must not be shared by calls
- * that overlap. */
+ * topk <= 64, experts <= 1024, tokens * topk below 2^31 - 16384. Enqueued on
+ * `stream` (NULL: the runtime's stream); needs no workspace. */
 NVFP4_API nvfp4_status nvfp4_expert_sort(
     nvfp4_runtime * runtime,
     const void * x,
@@ -474,8 +466,6 @@ NVFP4_API nvfp4_status nvfp4_expert_sort(
     int32_t * perm,
     int32_t * inverse,
     int32_t * offsets,
-    void * workspace,
-    size_t workspace_bytes,
     void * stream);
 
 /* additive: out[t] = residual[t] + sum_k weights[t, k] * rows[inverse[t, k]],

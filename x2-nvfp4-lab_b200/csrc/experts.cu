@@ -26,9 +26,10 @@ constexpr int kExThreads = 256;
 constexpr int kExMaxTopk = 64;
 constexpr int kExMaxExperts = 1024;
 constexpr int kExWarps = kExThreads / 32;
+constexpr int kExRows = 8;  // picks of a token that a thread handles together
 // Picks whose ranks one launch finds by comparing every pick with every other (a warp per pick): each CTA does it for
 // its own token from a shared-memory copy of the ids, so nothing waits on another launch.
-constexpr int kExSmallPicks = 1024;
+constexpr int kExSmallPicks = 4096;
 
 // Row of a pick: -1 for a dropped one, and for a number that no sort of this many picks writes.
 __device__ __forceinline__ int row_of(const int *inverse, long long pick, int picks) {
@@ -39,8 +40,11 @@ __device__ __forceinline__ int row_of(const int *inverse, long long pick, int pi
 // Expert of a pick, `experts` where the id names none.
 __device__ __forceinline__ int pick_key(const void *ids, int wide, long long ids_stride, int topk, int pick,
                                         int experts) {
-    const int t = pick / topk, k = pick - t * topk;
-    const long long at = (long long)t * ids_stride + k;
+    long long at = pick;
+    if (ids_stride != topk) {
+        const int t = pick / topk;
+        at = (long long)t * ids_stride + (pick - t * topk);
+    }
     const long long id = wide ? static_cast<const long long *>(ids)[at] : (long long)static_cast<const int *>(ids)[at];
     return id >= 0 && id < experts ? (int)id : experts;
 }
@@ -132,13 +136,12 @@ struct SortArgs {
     int *perm;
     int *inverse;
     int *offsets;
-    int *table;            // [blocks][experts + 1] picks per block and expert
     long long x_stride;    // bytes
     long long ids_stride;  // elements
     int ids_wide;
     int tokens, topk, experts, picks;
     int row_bytes;
-    int blocks, per_block;  // of the counting launches
+    int per_warp;           // picks a warp ranks, a multiple of 32
     int group;              // threads that share a token in the copy launch
 };
 
@@ -208,55 +211,79 @@ __global__ void __launch_bounds__(kExThreads) expert_sort_small_kernel(SortArgs 
     }
 }
 
-// Many picks, first launch: each block's picks per expert.
-__global__ void __launch_bounds__(kExThreads) expert_count_kernel(SortArgs a) {
-    __shared__ int count[kExMaxExperts + 1];
-    pdl_launch_dependents();
-    for (int e = threadIdx.x; e <= a.experts; e += kExThreads) count[e] = 0;
-    __syncthreads();
-    const int first = blockIdx.x * a.per_block, last = min(first + a.per_block, a.picks);
-    for (int i = first + threadIdx.x; i < last; i += kExThreads)
-        atomicAdd(&count[pick_key(a.ids, a.ids_wide, a.ids_stride, a.topk, i, a.experts)], 1);
-    __syncthreads();
-    for (int e = threadIdx.x; e <= a.experts; e += kExThreads)
-        a.table[(long long)blockIdx.x * (a.experts + 1) + e] = count[e];
+constexpr int kRankCtas = 8, kRankThreads = 1024, kRankWarps = kRankThreads / 32;
+constexpr int kRankKeys = 8;  // picks a lane holds at a time
+
+// Lanes of the warp with this lane's key, a ballot per bit (match.any takes about 80 cycles an SM for each warp).
+__device__ __forceinline__ unsigned lanes_with(int key, int bits) {
+    unsigned same = 0xffffffffu;
+    for (int b = 0; b < bits; ++b) {
+        const bool one = (key >> b) & 1;
+        const unsigned ones = __ballot_sync(0xffffffffu, one);
+        same &= one ? ones : ~ones;
+    }
+    return same;
 }
 
-// Second launch: every block sums the table's columns for its own starting rows (the table is small and in L2), then
-// ranks its picks in order: a warp takes 32 at a time, equal ids rank by lane, the warps' counts by warp.
-__global__ void __launch_bounds__(kExThreads) expert_place_kernel(SortArgs a) {
-    extern __shared__ int place_smem[];
-    int *base = place_smem;                 // [experts + 1] row of the block's next pick of that expert
-    int *counts = place_smem + a.experts + 1;  // [warps][experts + 1]
-    __shared__ int warp_sum[kExWarps];
+// Many picks, first launch: one cluster ranks them all. A warp owns consecutive picks and counts them; the warps' counts
+// add up in the CTA, the CTAs' through distributed shared memory; then every warp walks its picks again, 32 at a time,
+// and places them in order.
+__global__ void __launch_bounds__(kRankThreads, 1) expert_rank_kernel(SortArgs a) {
+    extern __shared__ int rank_smem[];
     const int n = a.experts + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int i = threadIdx.x; i < kExWarps * n; i += kExThreads) counts[i] = 0;
-    __syncthreads();
-    // The picks of a warp are consecutive, so counting needs no other launch's results.
-    const int per_warp = a.per_block / kExWarps;
-    const int first = blockIdx.x * a.per_block + warp * per_warp, last = min(first + per_warp, a.picks);
-    int *mine = counts + warp * n;
-    for (int i = first; i < last; i += 32) {
-        const int key = i + lane < last ? pick_key(a.ids, a.ids_wide, a.ids_stride, a.topk, i + lane, a.experts) : -1;
-        const unsigned same = __match_any_sync(0xffffffffu, key);
-        if (key >= 0 && lane == __ffs(same) - 1) mine[key] += __popc(same);
-        __syncwarp();
-    }
-    pdl_wait();
+    const int cta = (int)cluster_rank();
+    int *block = rank_smem;       // [experts + 1] picks of this CTA, read by the others
+    int *base = block + n;        // [experts + 1] first row of this CTA's picks
+    int *counts = base + n;       // [warps][experts + 1] a warp's picks, then the place of its next one
+    __shared__ int warp_sum[kRankWarps];
     pdl_launch_dependents();
-    const int per = (n + kExThreads - 1) / kExThreads;
-    const int e0 = min(threadIdx.x * per, n), e1 = min(e0 + per, n);
+    for (int i = threadIdx.x; i < kRankWarps * n; i += kRankThreads) counts[i] = 0;
+    __syncthreads();
+    const long long first = (long long)(cta * kRankWarps + warp) * a.per_warp;
+    const long long last = min(first + a.per_warp, (long long)a.picks);
+    int *mine = counts + warp * n;
+    const int bits = 32 - __clz(n);
+    int key[kRankKeys];
+    auto load_keys = [&](long long i) {
+#pragma unroll
+        for (int u = 0; u < kRankKeys; ++u) {
+            const long long pick = i + 32 * u + lane;
+            key[u] = pick < last ? pick_key(a.ids, a.ids_wide, a.ids_stride, a.topk, (int)pick, a.experts) : -1;
+        }
+    };
+    for (long long i = first; i < last; i += 32 * kRankKeys) {
+        load_keys(i);
+#pragma unroll
+        for (int u = 0; u < kRankKeys; ++u) {
+            if (key[u] >= 0) atomicAdd(mine + key[u], 1);
+        }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < n; e += kRankThreads) {
+        int run = 0;
+#pragma unroll 8
+        for (int w = 0; w < kRankWarps; ++w) {
+            const int c = counts[w * n + e];
+            counts[w * n + e] = run;
+            run += c;
+        }
+        block[e] = run;
+    }
+    cluster_sync();
+    // A thread's experts are consecutive (one, or two past 1023), so that the sum over earlier experts is a scan.
+    const int per = (n + kRankThreads - 1) / kRankThreads;
+    const int e0 = min((int)threadIdx.x * per, n), e1 = min(e0 + per, n);
     int own = 0;
     for (int e = e0; e < e1; ++e) {
-        int before = 0, total = 0;
-#pragma unroll 8
-        for (int b = 0; b < a.blocks; ++b) {
-            const int c = __ldcg(a.table + (long long)b * n + e);
-            before += b < (int)blockIdx.x ? c : 0;
-            total += c;
+        int before = 0, all = 0;
+#pragma unroll
+        for (int r = 0; r < kRankCtas; ++r) {
+            const int c = load_cluster(block + e, r);
+            before += r < cta ? c : 0;
+            all += c;
         }
-        base[e] = own + before;  // the sum over earlier experts is added below
-        own += total;
+        base[e] = own + before;
+        own += all;
     }
     int upto = own;
 #pragma unroll
@@ -270,33 +297,32 @@ __global__ void __launch_bounds__(kExThreads) expert_place_kernel(SortArgs a) {
     for (int w = 0; w < warp; ++w) start += warp_sum[w];
     for (int e = e0; e < e1; ++e) {
         base[e] += start;
-        if (blockIdx.x == 0) a.offsets[e] = base[e];  // block 0 has no picks before it
-        int run = base[e];
-#pragma unroll
-        for (int w = 0; w < kExWarps; ++w) {
-            const int c = counts[w * n + e];
-            counts[w * n + e] = run;
-            run += c;
-        }
+        if (cta == 0) a.offsets[e] = base[e];  // no CTA's picks come before the first one's
     }
     __syncthreads();
-    for (int i = first; i < last; i += 32) {
-        const int pick = i + lane;
-        const int key = pick < last ? pick_key(a.ids, a.ids_wide, a.ids_stride, a.topk, pick, a.experts) : -1;
-        const unsigned same = __match_any_sync(0xffffffffu, key);
-        const int row = key >= 0 ? mine[key] + __popc(same & ((1u << lane) - 1u)) : 0;
-        __syncwarp();
-        if (key >= 0) {
-            const bool used = key < a.experts;
-            a.inverse[pick] = used ? row : -1;
-            a.perm[row] = used ? pick : -1;
-            if (lane == __ffs(same) - 1) mine[key] += __popc(same);
+    for (long long i = first; i < last; i += 32 * kRankKeys) {
+        if (a.per_warp > 32 * kRankKeys) load_keys(i);  // else they are still in registers
+#pragma unroll
+        for (int u = 0; u < kRankKeys; ++u) {
+            if (i + 32 * u >= last) break;
+            // Picks past the last have a key of their own.
+            const unsigned same = lanes_with(key[u] >= 0 ? key[u] : n, bits);
+            const int row = key[u] >= 0 ? base[key[u]] + mine[key[u]] + __popc(same & ((1u << lane) - 1u)) : 0;
+            __syncwarp();
+            if (key[u] >= 0) {
+                const int pick = (int)(i + 32 * u) + lane;
+                const bool used = key[u] < a.experts;
+                a.inverse[pick] = used ? row : -1;
+                a.perm[row] = used ? pick : -1;
+                if (lane == __ffs(same) - 1) mine[key[u]] += __popc(same);
+            }
+            __syncwarp();
         }
-        __syncwarp();
     }
+    cluster_sync();  // no CTA leaves while another may read its counts
 }
 
-// Third launch: each token's row to its picks' rows, and zeros to the rows past the last expert's. A group of
+// Second launch: each token's row to its picks' rows, and zeros to the rows past the last expert's. A group of
 // threads owns a token.
 template <int B>
 __global__ void __launch_bounds__(kExThreads) expert_copy_kernel(SortArgs a) {
@@ -308,14 +334,19 @@ __global__ void __launch_bounds__(kExThreads) expert_copy_kernel(SortArgs a) {
     const V *src = reinterpret_cast<const V *>(a.x + (long long)t * a.x_stride);
     V val = lane < nvec ? src[lane] : zero_vec<V>();  // x depends on no earlier launch of this call
     pdl_wait();
-    const int used = a.offsets[a.experts];
-    for (int v = lane; v < nvec; v += a.group) {
-        if (v != lane) val = src[v];
-        for (int k = 0; k < a.topk; ++k) {
-            const int p = __ldg(a.inverse + (long long)t * a.topk + k);
-            if (p >= 0) reinterpret_cast<V *>(a.rows + (long long)p * a.row_bytes)[v] = val;
-            const int r = t * a.topk + k;
-            if (r >= used) reinterpret_cast<V *>(a.rows + (long long)r * a.row_bytes)[v] = zero_vec<V>();
+    const int used = __ldcg(a.offsets + a.experts);
+    for (int k0 = 0; k0 < a.topk; k0 += kExRows) {
+        int p[kExRows];
+#pragma unroll
+        for (int j = 0; j < kExRows; ++j) p[j] = k0 + j < a.topk ? __ldcg(a.inverse + (long long)t * a.topk + k0 + j) : -1;
+        for (int v = lane; v < nvec; v += a.group) {
+            if (v != lane || k0 > 0) val = src[v];
+#pragma unroll
+            for (int j = 0; j < kExRows; ++j) {
+                if (p[j] >= 0) reinterpret_cast<V *>(a.rows + (long long)p[j] * a.row_bytes)[v] = val;
+                const int r = t * a.topk + k0 + j;
+                if (k0 + j < a.topk && r >= used) reinterpret_cast<V *>(a.rows + (long long)r * a.row_bytes)[v] = zero_vec<V>();
+            }
         }
     }
 }
@@ -339,8 +370,6 @@ struct ReturnArgs {
     int group;
 };
 
-// K rows at a time in flight per thread.
-constexpr int kExRows = 8;
 
 template <int TYPE, int B>
 __global__ void __launch_bounds__(kExThreads) expert_return_kernel(ReturnArgs a) {
@@ -497,14 +526,6 @@ void launch(void (*kernel)(Args), int grid, size_t smem, cudaStream_t stream, bo
     check_cuda(cudaLaunchKernelEx(&cfg, kernel, args), name);
 }
 
-// Blocks of the counting launches and the picks of each (a multiple of the CTA, so that a warp's are consecutive).
-void sort_blocks(long long picks, int *blocks, int *per_block) {
-    const long long want = std::min<long long>(std::max<long long>((picks + 2047) / 2048, 1), 128);
-    const long long per = ((picks + want - 1) / want + kExThreads - 1) / kExThreads * kExThreads;
-    *per_block = static_cast<int>(per);
-    *blocks = static_cast<int>((picks + per - 1) / per);
-}
-
 template <int B>
 void launch_sort(SortArgs &a, cudaStream_t s) {
     a.group = group_of(a.row_bytes / B);
@@ -512,9 +533,22 @@ void launch_sort(SortArgs &a, cudaStream_t s) {
         launch(expert_sort_small_kernel<B>, a.tokens + 1, 0, s, false, a, "expert_sort_small_kernel");
         return;
     }
-    launch(expert_count_kernel, a.blocks, 0, s, false, a, "expert_count_kernel");
-    launch(expert_place_kernel, a.blocks, sizeof(int) * (kExWarps + 1) * (a.experts + 1), s, true, a,
-           "expert_place_kernel");
+    const size_t smem = sizeof(int) * (kRankWarps + 2) * (a.experts + 1);
+    check_cuda(cudaFuncSetAttribute(expert_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    static_cast<int>(sizeof(int) * (kRankWarps + 2) * (kExMaxExperts + 1))),
+               "cudaFuncSetAttribute(expert_rank_kernel)");
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(kRankCtas);
+    cfg.blockDim = dim3(kRankThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kRankCtas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    check_cuda(cudaLaunchKernelEx(&cfg, expert_rank_kernel, a), "expert_rank_kernel");
     const int per_cta = kExThreads / a.group;
     launch(expert_copy_kernel<B>, (a.tokens + per_cta - 1) / per_cta, 0, s, true, a, "expert_copy_kernel");
 }
@@ -549,7 +583,7 @@ void run_return(ReturnArgs &a, int type, int vec, bool backward, cudaStream_t s)
 
 bool valid_sizes(int type, int tokens, int topk, int hidden) {
     return valid_type(type) && tokens > 0 && topk > 0 && topk <= kExMaxTopk && hidden > 0 && hidden <= (1 << 24) &&
-           static_cast<long long>(tokens) * topk < INT_MAX - kExThreads * kExWarps;
+           static_cast<long long>(tokens) * topk < INT_MAX - 16384;
 }
 
 }  // namespace
@@ -557,27 +591,14 @@ bool valid_sizes(int type, int tokens, int topk, int hidden) {
 
 using namespace nvfp4;
 
-extern "C" NVFP4_API size_t nvfp4_expert_sort_workspace_bytes(int tokens, int topk, int experts) {
-    if (tokens <= 0 || topk <= 0 || experts <= 0) return 0;
-    const long long picks = static_cast<long long>(tokens) * topk;
-    if (picks <= kExSmallPicks) return 0;
-    int blocks = 0, per_block = 0;
-    sort_blocks(picks, &blocks, &per_block);
-    return sizeof(int) * static_cast<size_t>(blocks) * (static_cast<size_t>(experts) + 1);
-}
-
 extern "C" NVFP4_API nvfp4_status nvfp4_expert_sort(nvfp4_runtime *runtime, const void *x, int type, int64_t x_stride,
                                                     int tokens, int hidden, const void *ids, int ids_bytes,
                                                     int64_t ids_stride, int topk, int experts, void *rows,
-                                                    int32_t *perm, int32_t *inverse, int32_t *offsets,
-                                                    void *workspace, size_t workspace_bytes, void *stream) {
+                                                    int32_t *perm, int32_t *inverse, int32_t *offsets, void *stream) {
     if (!runtime || !x || !ids || !rows || !perm || !inverse || !offsets || !valid_sizes(type, tokens, topk, hidden) ||
         (ids_bytes != 4 && ids_bytes != 8) || ids_stride < 0 || x_stride < 0)
         return fail_invalid("invalid expert sort arguments");
     if (experts < 1 || experts > kExMaxExperts) return fail_invalid("the expert sort supports 1 to 1024 experts");
-    const size_t need = nvfp4_expert_sort_workspace_bytes(tokens, topk, experts);
-    if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3u)))
-        return fail_invalid("the expert sort's workspace is too small (nvfp4_expert_sort_workspace_bytes)");
     try {
         const device_scope scope(runtime);
         check_on_device(runtime, {x, ids, rows}, "expert sort");
@@ -588,7 +609,6 @@ extern "C" NVFP4_API nvfp4_status nvfp4_expert_sort(nvfp4_runtime *runtime, cons
         a.perm = perm;
         a.inverse = inverse;
         a.offsets = offsets;
-        a.table = static_cast<int *>(workspace);
         a.x_stride = x_stride * type_bytes(type);
         a.ids_stride = ids_stride;
         a.ids_wide = ids_bytes == 8;
@@ -597,7 +617,7 @@ extern "C" NVFP4_API nvfp4_status nvfp4_expert_sort(nvfp4_runtime *runtime, cons
         a.experts = experts;
         a.picks = tokens * topk;
         a.row_bytes = hidden * type_bytes(type);
-        sort_blocks(a.picks, &a.blocks, &a.per_block);
+        a.per_warp = ((a.picks + kRankCtas * kRankWarps - 1) / (kRankCtas * kRankWarps) + 31) / 32 * 32;
         const int vec = vector_bytes({place_of(x), place_of(rows), static_cast<unsigned long long>(a.x_stride),
                                       static_cast<unsigned long long>(a.row_bytes)});
         std::lock_guard<std::mutex> lock(runtime->queue_mutex);

@@ -78,6 +78,19 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// The 32-bit word at `p`'s place in the shared memory of the cluster's CTA `rank`.
+__device__ __forceinline__ int load_cluster(const int *p, uint32_t rank) {
+    int v;
+    asm volatile(
+        "{\n\t.reg .b32 remote;\n\t"
+        "mapa.shared::cluster.u32 remote, %1, %2;\n\t"
+        "ld.shared::cluster.b32 %0, [remote];\n\t}"
+        : "=r"(v)
+        : "r"(smem_u32(p)), "r"(rank)
+        : "memory");
+    return v;
+}
+
 // Arrive on the barrier at `bar`'s offset in the cluster's CTA `rank`.
 __device__ __forceinline__ void mbar_arrive_at(uint64_t *bar, uint32_t rank) {
     asm volatile(

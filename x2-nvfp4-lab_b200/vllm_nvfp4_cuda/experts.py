@@ -73,14 +73,11 @@ def _sort(rt, x, ids, experts):
         offsets.zero_()
         return rows, perm, inverse, offsets
     x, ids = _rows_of(x), _rows_of(ids)
-    size = rt.lib.nvfp4_expert_sort_workspace_bytes(tokens, topk, experts)
-    workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     rt._check(
         rt.lib.nvfp4_expert_sort(
             rt.handle, x.data_ptr(), TYPES[x.dtype], _row_stride(x), tokens, hidden, ids.data_ptr(),
             ids.element_size(), _row_stride(ids), topk, experts, rows.data_ptr(), perm.data_ptr(),
-            inverse.data_ptr(), offsets.data_ptr(), workspace.data_ptr() if size else None, size,
-            _handle(x.device)),
+            inverse.data_ptr(), offsets.data_ptr(), _handle(x.device)),
         "nvfp4_expert_sort")
     return rows, perm, inverse, offsets
 

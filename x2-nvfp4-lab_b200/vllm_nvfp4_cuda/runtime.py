@@ -197,10 +197,9 @@ _SIGNATURES: dict[str, tuple[list, object]] = {
     "nvfp4_linear_grouped": (
         [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
          C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p], C.c_int),
-    "nvfp4_expert_sort_workspace_bytes": ([C.c_int, C.c_int, C.c_int], C.c_size_t),
     "nvfp4_expert_sort": (
         [C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_int,
-         C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p], C.c_int),
+         C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
     "nvfp4_expert_return": (
         [C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int,
          C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_void_p], C.c_int),
