@@ -527,16 +527,16 @@ void launch(void (*kernel)(Args), int grid, size_t smem, cudaStream_t stream, bo
 }
 
 template <int B>
-void launch_sort(SortArgs &a, cudaStream_t s) {
+void launch_sort(SortArgs &a, int device, cudaStream_t s) {
     a.group = group_of(a.row_bytes / B);
     if (a.picks <= kExSmallPicks) {
         launch(expert_sort_small_kernel<B>, a.tokens + 1, 0, s, false, a, "expert_sort_small_kernel");
         return;
     }
     const size_t smem = sizeof(int) * (kRankWarps + 2) * (a.experts + 1);
-    check_cuda(cudaFuncSetAttribute(expert_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(sizeof(int) * (kRankWarps + 2) * (kExMaxExperts + 1))),
-               "cudaFuncSetAttribute(expert_rank_kernel)");
+    static std::atomic<uint64_t> done{0};
+    allow_shared_memory(expert_rank_kernel, sizeof(int) * (kRankWarps + 2) * (kExMaxExperts + 1), done, device,
+                        "cudaFuncSetAttribute(expert_rank_kernel)");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(kRankCtas);
     cfg.blockDim = dim3(kRankThreads);
@@ -623,10 +623,10 @@ extern "C" NVFP4_API nvfp4_status nvfp4_expert_sort(nvfp4_runtime *runtime, cons
         std::lock_guard<std::mutex> lock(runtime->queue_mutex);
         runtime->direct_call(static_cast<cudaStream_t>(stream), [&](cudaStream_t os) {
             runtime->profiled_kernel("expert_sort", os, [&](cudaStream_t s) {
-                if (vec == 16) launch_sort<16>(a, s);
-                else if (vec == 8) launch_sort<8>(a, s);
-                else if (vec == 4) launch_sort<4>(a, s);
-                else if (vec == 2) launch_sort<2>(a, s);
+                if (vec == 16) launch_sort<16>(a, runtime->device, s);
+                else if (vec == 8) launch_sort<8>(a, runtime->device, s);
+                else if (vec == 4) launch_sort<4>(a, runtime->device, s);
+                else if (vec == 2) launch_sort<2>(a, runtime->device, s);
                 else throw invalid_argument_error("expert sort: rows must be aligned to their elements");
             });
         });

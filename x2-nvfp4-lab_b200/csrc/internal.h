@@ -5,6 +5,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <chrono>
 #include <cstdint>
 #include <initializer_list>
@@ -136,6 +137,15 @@ class device_scope {
   private:
     int back_ = -1;
 };
+
+// Raises a kernel's dynamic shared-memory limit once per device (`done`: one flag word per kernel).
+template <typename Kernel>
+void allow_shared_memory(Kernel kernel, size_t bytes, std::atomic<uint64_t> &done, int device, const char *name) {
+    const uint64_t bit = device < 64 ? uint64_t{1} << device : 0;
+    if (bit && (done.load(std::memory_order_acquire) & bit)) return;
+    check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)), name);
+    done.fetch_or(bit, std::memory_order_acq_rel);
+}
 
 // Throws when one of `pointers` (NULL skipped) is device memory of another GPU than the runtime's.
 void check_on_device(const nvfp4_runtime *runtime, std::initializer_list<const void *> pointers, const char *operation);

@@ -89,7 +89,7 @@ nvfp4_status run_fused(nvfp4_runtime *runtime, const nvfp4_matrix *matrix, const
         std::lock_guard<std::mutex> lock(runtime->queue_mutex);
         runtime->direct_call(static_cast<cudaStream_t>(stream), [&](cudaStream_t os) {
             runtime->profiled_kernel(operation, os, [&](cudaStream_t s) {
-                if (few) launch_linear_gemv(a, runtime->sm_count, s);
+                if (few) launch_linear_gemv(a, runtime->device, runtime->sm_count, s);
                 else launch_linear_gemm(a, *matrix, workspace, runtime->sm_count, s);
             });
         });

@@ -111,7 +111,7 @@ __device__ __forceinline__ void zero_other_rows(const FusedLinearArgs &a) {
 
 // Whether the few-row kernel takes the call (x and out need not be set).
 bool linear_gemv_serves(const FusedLinearArgs &a);
-void launch_linear_gemv(const FusedLinearArgs &a, int sm_count, cudaStream_t stream);
+void launch_linear_gemv(const FusedLinearArgs &a, int device, int sm_count, cudaStream_t stream);
 
 // Device workspace of launch_linear_gemm for this call: 0 when the kernel can
 // read x where it lies.

@@ -716,9 +716,9 @@ size_t parts_bytes(int type, int vectors, int cols) {
 template <int TYPE, int N>
 void launch(const GemmArgs &g, const nvfp4_matrix &matrix, const CUtensorMap &map_x, int grid, bool dependent,
             cudaStream_t stream) {
-    check_cuda(cudaFuncSetAttribute(linear_gemm_kernel<TYPE, N>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(Shape<N, TYPE == NVFP4_TYPE_F32 ? 2 : 1>::kSmem)),
-               "cudaFuncSetAttribute(linear_gemm_kernel)");
+    static std::atomic<uint64_t> done{0};
+    allow_shared_memory(linear_gemm_kernel<TYPE, N>, Shape<N, TYPE == NVFP4_TYPE_F32 ? 2 : 1>::kSmem, done,
+                        matrix.runtime->device, "cudaFuncSetAttribute(linear_gemm_kernel)");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kGmThreads);

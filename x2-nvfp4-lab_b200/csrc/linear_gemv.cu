@@ -36,7 +36,8 @@ constexpr int kGvThreads = 256;
 constexpr int kGvWarps = kGvThreads / 32;
 constexpr int kGvCols = 8;                          // columns of an MMA: rows of x, or halves of FP32 rows
 constexpr int kGvRedPitch = 20;                    // floats per column of a partial tile: conflict-free stores
-constexpr size_t kGvSmem = 232448;                 // shared memory of a CTA
+constexpr size_t kGvSmem = 232384;                 // dynamic shared memory of a CTA (64 bytes are static)
+constexpr size_t kGvSmemSm = 233472;               // and of an SM, of which every CTA takes 1 KB more
 
 struct GemvArgs {
     FusedLinearArgs f;
@@ -438,17 +439,15 @@ size_t other_smem(const FusedLinearArgs &f) {
 }
 
 template <int TYPE>
-void launch(GemvArgs &a, int sm_count, cudaStream_t stream) {
+void launch(GemvArgs &a, int device, int sm_count, cudaStream_t stream) {
     const size_t smem = (size_t)a.pass_cols * a.token_stride + other_smem(a.f);
-    check_cuda(cudaFuncSetAttribute(linear_gemv_kernel<TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(smem)),
-               "cudaFuncSetAttribute(linear_gemv_kernel)");
-    int per_sm = 0;
-    check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, linear_gemv_kernel<TYPE>, kGvThreads, smem),
-               "cudaOccupancyMaxActiveBlocksPerMultiprocessor(linear_gemv_kernel)");
+    static std::atomic<uint64_t> done{0};
+    allow_shared_memory(linear_gemv_kernel<TYPE>, kGvSmem, done, device, "cudaFuncSetAttribute(linear_gemv_kernel)");
+    // Two CTAs on an SM (the kernel's registers) where their shared memory fits.
+    const int per_sm = 2 * (smem + 1024) <= kGvSmemSm ? 2 : 1;
     const long long teams = kGvWarps / a.warps_k;
     const long long work = ((long long)a.tiles * (a.f.offsets ? std::min(a.f.groups, a.f.vectors) : 1) + teams - 1) / teams;
-    const long long grid = std::min(work, (long long)sm_count * std::max(1, per_sm));
+    const long long grid = std::min(work, (long long)sm_count * per_sm);
     linear_gemv_kernel<TYPE><<<static_cast<int>(std::max<long long>(1, grid)), kGvThreads, smem, stream>>>(a);
     check_cuda(cudaGetLastError(), "linear_gemv_kernel");
 }
@@ -472,7 +471,7 @@ bool linear_gemv_serves(const FusedLinearArgs &f) {
     return staged_rows(f) >= 1 && (f.offsets ? (long long)f.vectors * per_row <= 3LL * f.groups : f.vectors * per_row <= 8);
 }
 
-void launch_linear_gemv(const FusedLinearArgs &f, int sm_count, cudaStream_t stream) {
+void launch_linear_gemv(const FusedLinearArgs &f, int device, int sm_count, cudaStream_t stream) {
     GemvArgs a{};
     a.f = f;
     a.chunks = (f.cols + 255) / 256;
@@ -487,9 +486,9 @@ void launch_linear_gemv(const FusedLinearArgs &f, int sm_count, cudaStream_t str
     const long long tiles = (long long)a.tiles * (f.offsets ? std::min(f.groups, f.vectors) : 1);
     a.warps_k = 1;
     while (a.warps_k < kGvWarps && 2 * a.warps_k <= a.chunks && tiles * a.warps_k < (long long)sm_count * 16 * 4) a.warps_k *= 2;
-    if (f.type == NVFP4_TYPE_BF16) launch<NVFP4_TYPE_BF16>(a, sm_count, stream);
-    else if (f.type == NVFP4_TYPE_F16) launch<NVFP4_TYPE_F16>(a, sm_count, stream);
-    else launch<NVFP4_TYPE_F32>(a, sm_count, stream);
+    if (f.type == NVFP4_TYPE_BF16) launch<NVFP4_TYPE_BF16>(a, device, sm_count, stream);
+    else if (f.type == NVFP4_TYPE_F16) launch<NVFP4_TYPE_F16>(a, device, sm_count, stream);
+    else launch<NVFP4_TYPE_F32>(a, device, sm_count, stream);
 }
 
 }  // namespace nvfp4

@@ -12,19 +12,18 @@ lab has no counterpart.
 
 from __future__ import annotations
 
-from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
-from .runtime import _stream_handle
+from .runtime import CUDA_STREAM_LEGACY
 
 # Element types of the C ABI (NVFP4_TYPE_*).
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_TOPK, MAX_EXPERTS = 64, 1024
 
 
-@dataclass(frozen=True)
-class ExpertOrder:
+class ExpertOrder(NamedTuple):
     """Where ``expert_sort`` put the picks (int32 CUDA tensors)."""
 
     perm: torch.Tensor     # [T*K] flat pick token*K + k of each row, -1 past the last expert's rows
@@ -55,8 +54,10 @@ def on_stream(stream, tensors, call):
     return result
 
 
-def _handle(device) -> object:
-    return _stream_handle(torch.cuda.current_stream(device))
+def stream_of(device) -> int:
+    """torch's current stream on ``device`` as the C ABI takes it (its default stream has handle 0, which the ABI would
+    read as the runtime's own)."""
+    return torch._C._cuda_getCurrentRawStream(device.index) or CUDA_STREAM_LEGACY
 
 
 # ------------------------------------------------------------------ one call each
@@ -77,7 +78,7 @@ def _sort(rt, x, ids, experts):
         rt.lib.nvfp4_expert_sort(
             rt.handle, x.data_ptr(), TYPES[x.dtype], _row_stride(x), tokens, hidden, ids.data_ptr(),
             ids.element_size(), _row_stride(ids), topk, experts, rows.data_ptr(), perm.data_ptr(),
-            inverse.data_ptr(), offsets.data_ptr(), _handle(x.device)),
+            inverse.data_ptr(), offsets.data_ptr(), stream_of(x.device)),
         "nvfp4_expert_sort")
     return rows, perm, inverse, offsets
 
@@ -101,7 +102,7 @@ def _return(rt, rows, inverse, weights, residual, out):
             TYPES[weights.dtype] if weights is not None else 0,
             residual.data_ptr() if residual is not None else None,
             _row_stride(residual) if residual is not None else 0, tokens, topk, hidden, out.data_ptr(),
-            _row_stride(out), _handle(rows.device)),
+            _row_stride(out), stream_of(rows.device)),
         "nvfp4_expert_return")
     return out
 
@@ -125,7 +126,7 @@ def _return_backward(rt, dout, rows, inverse, offsets, weights, experts, need_ro
             inverse.data_ptr(), offsets.data_ptr(), weights.data_ptr() if weights is not None else None,
             TYPES[weights.dtype] if weights is not None else 0, tokens, topk, hidden, experts,
             drows.data_ptr() if need_rows else None, dweights.data_ptr() if need_weights else None,
-            _handle(dout.device)),
+            stream_of(dout.device)),
         "nvfp4_expert_return_backward")
     return drows, dweights
 
@@ -135,18 +136,18 @@ def _return_backward(rt, dout, rows, inverse, offsets, weights, experts, need_ro
 
 class _ExpertSort(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, rt, ids, experts):
-        rows, perm, inverse, offsets = _sort(rt, x, ids, experts)
+    def forward(ctx, x, rt, ids, experts, record):
+        # The order goes out by the record: numbers without a gradient, which autograd need not see.
+        rows, *order = _sort(rt, x, ids, experts)
+        record.extend(order)
         ctx.rt = rt
-        ctx.save_for_backward(inverse)
-        ctx.mark_non_differentiable(perm, inverse, offsets)
-        return rows, perm, inverse, offsets
+        ctx.inverse = order[1]
+        return rows
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, drows, *_):
-        (inverse,) = ctx.saved_tensors
-        return _return(ctx.rt, drows, inverse, None, None, None), None, None, None
+    def backward(ctx, drows):
+        return _return(ctx.rt, drows, ctx.inverse, None, None, None), None, None, None, None
 
 
 class _ExpertReturn(torch.autograd.Function):
@@ -191,7 +192,8 @@ def expert_sort(rt, x, ids, experts: int, stream=None):
 
     def call():
         if x.requires_grad and torch.is_grad_enabled():
-            return _ExpertSort.apply(x, rt, ids, experts)
+            record = []
+            return _ExpertSort.apply(x, rt, ids, experts, record), *record
         return _sort(rt, x, ids, experts)
 
     rows, perm, inverse, offsets = on_stream(stream, (x, ids), call)

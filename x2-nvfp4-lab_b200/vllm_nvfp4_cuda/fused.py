@@ -9,8 +9,8 @@ from __future__ import annotations
 
 import torch
 
-from .experts import TYPES, _row_stride, _rows_of, on_stream
-from .runtime import ACTIVATIONS, _stream_handle
+from .experts import TYPES, _row_stride, _rows_of, on_stream, stream_of
+from .runtime import ACTIVATIONS
 
 
 def _require(condition, message):
@@ -57,21 +57,25 @@ def linear_fused(rt, matrix, x, bias, activation, residual, out, stream):
         _require(t is None or (tuple(t.shape) == shape and t.dtype == x.dtype),
                  f"{name} must be of x's type, [..., {width}]")
 
+    def rows2d(t, cols):
+        return _rows_of(t if t.dim() == 2 else t.reshape(-1, cols))
+
     def call():
-        x2 = _rows_of(x.reshape(-1, matrix.cols))
-        y = out if out is not None else x.new_empty(shape)
-        if out is not None:
+        x2 = rows2d(x, matrix.cols)
+        if out is None:
+            y, stride = x.new_empty(shape), width
+        else:
+            y = out
             try:
-                y2 = out.view(-1, width)
+                y2 = out if out.dim() == 2 else out.view(-1, width)
             except RuntimeError:
                 y2 = None
             _require(y2 is not None and (y2.stride(1) == 1 or width == 1)
                      and (y2.shape[0] < 2 or y2.stride(0) >= width), "out must have contiguous columns and even rows")
-        else:
-            y2 = y.view(-1, width)
+            stride = _row_stride(y2)
         if x2.shape[0] == 0:
             return y
-        r2 = _rows_of(residual.reshape(-1, width)) if residual is not None else None
+        r2 = rows2d(residual, width) if residual is not None else None
         b = bias.contiguous() if bias is not None else None
         _held, space, size = _workspace(rt, matrix, x2, 0)
         rt._check(
@@ -79,8 +83,8 @@ def linear_fused(rt, matrix, x, bias, activation, residual, out, stream):
                 rt.handle, matrix.handle, x2.data_ptr(), TYPES[x.dtype], _row_stride(x2), x2.shape[0],
                 b.data_ptr() if b is not None else None, TYPES[b.dtype] if b is not None else 0,
                 ACTIVATIONS[activation], r2.data_ptr() if r2 is not None else None,
-                _row_stride(r2) if r2 is not None else 0, y2.data_ptr(), _row_stride(y2), space, size,
-                _stream_handle(torch.cuda.current_stream(x.device))),
+                _row_stride(r2) if r2 is not None else 0, y.data_ptr(), stride, space, size,
+                stream_of(x.device)),
             "nvfp4_linear_fused")
         return y
 
@@ -110,7 +114,7 @@ def linear_grouped(rt, matrix, x, offsets, bias, activation, out, stream):
                 rt.handle, matrix.handle, x2.data_ptr(), TYPES[x.dtype], _row_stride(x2), shape[0], o.data_ptr(),
                 b.data_ptr() if b is not None else None, TYPES[b.dtype] if b is not None else 0,
                 ACTIVATIONS[activation], y.data_ptr(), _row_stride(y), 1 if out is None else 0, space, size,
-                _stream_handle(torch.cuda.current_stream(x.device))),
+                stream_of(x.device)),
             "nvfp4_linear_grouped")
         return y
 
