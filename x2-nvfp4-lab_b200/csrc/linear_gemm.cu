@@ -28,9 +28,10 @@
 // FP32 x enters as two FP16 halves, scaled per row by a power of two
 // (linear_gemv.cu has the error), split by a kernel before; x that TMA cannot
 // read (16-byte addresses and strides) is copied by the same kernel. For FP32
-// the sums move to FP32 registers of the epilogue every 256 columns: the tensor
-// core rounds its running sum towards zero, and the bias of a long chain would
-// show.
+// the sums move to FP32 registers of the epilogue every 128 columns, and the low
+// halves' products come first: the tensor core rounds its running sum towards
+// zero, and the bias of a long chain would show (5.7e-7 of the result with
+// segments of 256 columns, high halves first).
 #include "linear_fused.cuh"
 #include "tcgen05_util.cuh"
 #include "tma_util.cuh"
@@ -46,7 +47,7 @@ constexpr int kGmEpiGroups = 2;
 constexpr int kGmThreads = 32 * (kGmEpiWarp0 + 4 * kGmEpiGroups);
 constexpr int kGmLargeN = 160;                      // rows of x per tile
 constexpr int kGmSmallN = 64;                       // of calls with few, and of split FP32 x (32 per epilogue warpgroup)
-constexpr int kGmSegment32 = 2;                     // steps per accumulator of split FP32 x
+constexpr int kGmSegment32 = 1;                     // steps per accumulator of split FP32 x
 constexpr int kGmRawBytes = 128 * 128;              // 256 columns of packed weights
 constexpr int kGmRawScales = 128 * 16;
 constexpr int kGmRaw = kGmRawBytes + kGmRawScales;
@@ -450,14 +451,14 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                             tc::fence_after_sync();
                             if (tc::elect_one()) {
 #pragma unroll
-                                for (int j = 0; j < kTerms; ++j)
+                                for (int j = kTerms - 1; j >= 0; --j)  // the small halves first
 #pragma unroll
                                     for (int i = 0; i < 8; ++i)
                                         tc::mma_16bit_ts_pair(
                                             acc, tmem + Z::kColA + 64 * stage + 8 * i,
                                             desc + ((stage * Z::kStageB + (i >> 2) * Z::kHalfB + j * (kGmSmallN / 2) * 128 +
                                                      32 * (i & 3)) >> 4),
-                                            idesc, (j | i) != 0 ? 1u : more);
+                                            idesc, j != kTerms - 1 || i != 0 ? 1u : more);
                                 tc::commit_pair(empty + stage);
                             }
                             __syncwarp();
