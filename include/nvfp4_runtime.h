@@ -386,12 +386,13 @@ NVFP4_API size_t nvfp4_linear_workspace_bytes(
  * selects the runtime's stream). x [vectors, cols], residual and out
  * [vectors, rows] (rows / 2 with a gate) are of `type`, each with its own row
  * stride in elements (columns contiguous); bias [rows] has a type of its own;
- * bias and residual may be NULL, residual may be out itself. The weights'
+ * bias and residual may be NULL, residual may be out itself (else neither it
+ * nor x shares memory with out). The weights'
  * values are exact in the products, sums are FP32, and the result is rounded
  * once. BF16 and FP32 elements of x below 2^-29 of their row's largest finite
  * value may lose low bits (by less than 2^-39 of that value). No memory is
  * allocated and the matrix is only read: calls may overlap and be captured in
- * CUDA graphs. Up to 2^31 - 1 vectors. */
+ * CUDA graphs. Up to 2^30 vectors. */
 NVFP4_API nvfp4_status nvfp4_linear_fused(
     nvfp4_runtime * runtime,
     const nvfp4_matrix * matrix,
@@ -472,7 +473,8 @@ NVFP4_API nvfp4_status nvfp4_expert_sort(
  * picks with inverse -1 left out, in FP32 and the order of k, rounded once.
  * rows, residual and out are of `type` with row strides in elements; weights
  * [tokens, topk] (contiguous, a type of their own) may be NULL for ones (the
- * gradient of nvfp4_expert_sort to x), residual may be NULL. */
+ * gradient of nvfp4_expert_sort to x), residual may be NULL, or out itself;
+ * otherwise out shares no memory with what is read. */
 NVFP4_API nvfp4_status nvfp4_expert_return(
     nvfp4_runtime * runtime,
     const void * rows,

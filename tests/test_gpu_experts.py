@@ -44,9 +44,10 @@ def _plain_order(ids, experts):
     return perm, inverse.reshape(ids.shape), offsets
 
 
-# tokens x topk on both sides of the one-launch sort (1024 picks), of a counting block (2048) and of several.
+# tokens x topk on both sides of the one-CTA sort (4096 picks), with most experts and picks in each.
 SIZES = [(1, 1, 1, 8), (1, 8, 256, 2048), (3, 2, 8, 1), (7, 64, 40, 33), (128, 8, 64, 96), (129, 8, 256, 100),
-         (513, 6, 1024, 20), (700, 3, 5, 2052), (2048, 1, 3, 7), (3001, 8, 256, 24)]
+         (513, 6, 1024, 20), (700, 3, 5, 2052), (2048, 1, 3, 7), (3001, 8, 256, 24), (512, 8, 9, 4),
+         (4097, 1, 1024, 8), (600, 64, 1024, 12)]
 
 
 @pytest.mark.parametrize("how", ["all", "some", "none", "one"])
@@ -247,6 +248,30 @@ def test_streams_and_graphs(cuda_runtime):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_results_side_by_side_and_onto_the_residual(cuda_runtime):
+    """The return into the columns beside its rows, and onto its residual: the bits of the plain call."""
+    rt = cuda_runtime
+    tokens, topk, experts, hidden = 70, 2, 6, 48
+    ids = torch.from_numpy(_ids(60, tokens, topk, experts, "some")).cuda()
+    rows, order = rt.expert_sort(_normal(61, tokens, hidden), ids, experts)
+    w, residual = _normal(62, tokens, topk), _normal(63, tokens, hidden)
+    want = rt.expert_return(rows, order, w, residual)
+    both = torch.cat([rows, torch.full_like(rows, 3.0)], dim=1)
+    out = rt.expert_return(both[:, :hidden], order, w, residual, out=both[:tokens, hidden:])
+    assert torch.equal(out, want) and torch.equal(both[:, :hidden], rows) and bool((both[tokens:, hidden:] == 3).all())
+    assert rt.expert_return(rows, order, w, residual, out=residual) is residual and torch.equal(residual, want)
+
+
+def test_changed_order_is_seen_by_the_backward_pass(cuda_runtime):
+    """The order is kept for the gradients: writing to it in between is an error, not another gradient."""
+    x = _normal(64, 9, 8).requires_grad_()
+    ids = torch.from_numpy(_ids(65, 9, 2, 4, "all")).cuda()
+    rows, order = cuda_runtime.expert_sort(x, ids, 4)
+    order.inverse.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        rows.sum().backward()
+
+
 def test_refusals(cuda_runtime):
     rt = cuda_runtime
     x = torch.zeros(4, 8, device="cuda")
@@ -271,6 +296,12 @@ def test_refusals(cuda_runtime):
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {i} was taken")
+    for out in (rows[2:6], rows[:4]):  # onto rows that are still to be read
+        with pytest.raises(RuntimeError, match="overlap"):
+            rt.expert_return(rows, order, w, out=out)
+    wide = torch.zeros(5, 8, device="cuda")
+    with pytest.raises(RuntimeError, match="overlap"):
+        rt.expert_return(rows, order, w, wide[:4], out=wide[1:])
     # A gradient of a gradient is refused.
     y = x.clone().requires_grad_()
     r, _ = rt.expert_sort(y, ids, 3)

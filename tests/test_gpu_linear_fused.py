@@ -251,6 +251,67 @@ def test_streams_graphs_and_calls_at_once(cuda_runtime):
     cuda_runtime.synchronize()
 
 
+def test_grouped_streams_graphs_and_calls_at_once(cuda_runtime):
+    """The grouped form on two streams at once, and two captured calls replayed together on new rows and offsets."""
+    groups, rows, cols = 6, 136, 256
+    m, *_ = _matrix(cuda_runtime, groups, rows, cols, 24)
+    for dtype in (torch.float16, torch.float32):
+        for cuts in (([0, 1, 1, 3, 4, 4, 6], [0, 2, 2, 2, 3, 6, 6]), ([0, 90, 91, 150, 300, 300, 400],
+                                                                      [0, 0, 0, 399, 400, 400, 400])):
+            xs = [_normal(25 + i, cuts[0][-1], cols, dtype=dtype) for i in range(2)]
+            os = [torch.tensor(c, dtype=torch.int32, device="cuda") for c in cuts]
+            plain = [[cuda_runtime.linear_grouped(m, x, o, activation="gelu_mul") for o in os] for x in xs]
+            torch.cuda.synchronize()
+            streams = [torch.cuda.Stream() for _ in xs]
+            got = [cuda_runtime.linear_grouped(m, x, o, activation="gelu_mul", stream=s)
+                   for x, o, s in zip(xs, os, streams)]
+            torch.cuda.synchronize()
+            assert torch.equal(got[0], plain[0][0]) and torch.equal(got[1], plain[1][1])
+            graphs, inputs, outputs = [], [], []
+            for i in range(2):
+                inputs.append((xs[i].clone(), os[i].clone()))
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g):
+                    outputs.append(cuda_runtime.linear_grouped(m, *inputs[i], activation="gelu_mul"))
+                graphs.append(g)
+            for i in range(2):
+                inputs[i][0].copy_(xs[1 - i])
+                inputs[i][1].copy_(os[1 - i])
+            torch.cuda.synchronize()
+            for s, g in zip(streams, graphs):
+                with torch.cuda.stream(s):
+                    g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(outputs[0], plain[1][1]) and torch.equal(outputs[1], plain[0][0])
+    m.close()
+    cuda_runtime.synchronize()
+
+
+@pytest.mark.parametrize("vectors", [1, 6, 40])
+def test_results_in_the_memory_of_the_inputs(cuda_runtime, vectors):
+    """Into the columns beside x (the bits of the plain call); onto x, or across the residual's rows, is refused."""
+    rt, cols = cuda_runtime, 64
+    m, *_ = _matrix(rt, 1, 64, cols, 27)
+    for dtype in TYPES.values():
+        both = _normal(28, vectors + 1, 2 * cols, dtype=dtype)
+        x, beside = both[:vectors, :cols], both[:vectors, cols:]
+        want = rt.linear_fused(m, x, activation="relu", residual=beside)
+        with pytest.raises(RuntimeError, match="overlap"):
+            rt.linear_fused(m, x, out=x)
+        with pytest.raises(RuntimeError, match="overlap"):
+            rt.linear_fused(m, x, out=both[:vectors, cols // 2:cols // 2 + cols])
+        if vectors > 1:
+            with pytest.raises(RuntimeError, match="overlap"):
+                rt.linear_fused(m, x.clone(), residual=beside, out=both[1:, cols:])
+        assert torch.equal(rt.linear_fused(m, x, activation="relu", residual=beside, out=beside), want)
+    g, *_ = _matrix(rt, 2, 64, cols, 29)
+    x = _normal(30, 3, cols)
+    with pytest.raises(RuntimeError, match="overlap"):
+        rt.linear_grouped(g, x, torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda"), out=x)
+    m.close()
+    g.close()
+
+
 def test_refusals(cuda_runtime):
     rt = cuda_runtime
     m, *_ = _matrix(rt, 1, 65, 64, 21)

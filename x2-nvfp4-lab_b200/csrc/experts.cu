@@ -661,6 +661,13 @@ extern "C" NVFP4_API nvfp4_status nvfp4_expert_return(nvfp4_runtime *runtime, co
     if (!runtime || !rows || !inverse || !out || !valid_sizes(type, tokens, topk, hidden) ||
         (weights && !valid_type(weights_type)) || rows_stride < 0 || residual_stride < 0 || out_stride < hidden)
         return fail_invalid("invalid expert return arguments");
+    const long long row = static_cast<long long>(hidden) * type_bytes(type), picks = static_cast<long long>(tokens) * topk;
+    const row_span to{out, tokens, row, out_stride * type_bytes(type)};
+    if (spans_overlap({rows, picks, row, rows_stride * type_bytes(type)}, to))
+        return fail_invalid("expert return: out must not overlap the rows");
+    if (!(residual == out && (residual_stride == out_stride || tokens == 1)) &&
+        spans_overlap({residual, tokens, row, residual_stride * type_bytes(type)}, to))
+        return fail_invalid("expert return: the residual is out itself or does not overlap it");
     try {
         const device_scope scope(runtime);
         check_on_device(runtime, {rows, out}, "expert return");

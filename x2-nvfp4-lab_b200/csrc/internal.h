@@ -147,6 +147,15 @@ void allow_shared_memory(Kernel kernel, size_t bytes, std::atomic<uint64_t> &don
     done.fetch_or(bit, std::memory_order_acq_rel);
 }
 
+// Rows of a call in memory: `rows` of `row_bytes`, `stride` bytes apart.
+struct row_span {
+    const void *base;
+    long long rows, row_bytes, stride;
+};
+
+// Whether two of them share a byte: rows side by side in one buffer (one stride, columns apart) do not.
+bool spans_overlap(const row_span &a, const row_span &b);
+
 // Throws when one of `pointers` (NULL skipped) is device memory of another GPU than the runtime's.
 void check_on_device(const nvfp4_runtime *runtime, std::initializer_list<const void *> pointers, const char *operation);
 

@@ -44,6 +44,7 @@ const char *fused_args(FusedLinearArgs &a, const nvfp4_runtime *runtime, const n
                        void *out, int64_t out_stride) {
     if (!runtime || !matrix || matrix->runtime != runtime || !x || !out || vectors <= 0 || !valid_type(type))
         return "invalid linear arguments or mismatched runtime/matrix";
+    if (vectors > (1 << 30)) return "linear: at most 2^30 rows of x";
     const int act = activation & ~NVFP4_ACT_GATED;
     const bool gated = (activation & NVFP4_ACT_GATED) != 0;
     if (act < NVFP4_ACT_NONE || act > NVFP4_ACT_GELU_TANH) return "unknown activation";
@@ -53,6 +54,9 @@ const char *fused_args(FusedLinearArgs &a, const nvfp4_runtime *runtime, const n
     if (x_stride < 0 || out_stride < a.out_rows) return "invalid row stride";
     if (!aligned_to_type(x, type) || !aligned_to_type(out, type) || (bias && !aligned_to_type(bias, bias_type)))
         return "linear arguments must be aligned to their elements";
+    const long long e = type == NVFP4_TYPE_F32 ? 4 : 2;
+    if (spans_overlap({x, vectors, matrix->cols * e, x_stride * e}, {out, vectors, a.out_rows * e, out_stride * e}))
+        return "linear: out must not overlap x";
     a.packed = matrix->packed;
     a.scales = matrix->scales;
     a.packed_pitch = matrix->packed_pitch;
@@ -114,7 +118,7 @@ extern "C" NVFP4_API nvfp4_status nvfp4_matrix_upload_grouped(nvfp4_runtime *run
     if (groups < 1 || groups > kLinMaxGroups) return fail_invalid("a grouped NVFP4 matrix holds 1 to 1024 groups");
     if (cols > kLinMaxCols) return fail_invalid("NVFP4 linear supports at most 49152 columns on this backend");
     const long long all_rows = static_cast<long long>(groups) * rows;
-    if (all_rows > INT_MAX) return fail_invalid("NVFP4 matrix has too many rows");
+    if (all_rows > INT_MAX - 4096) return fail_invalid("NVFP4 matrix has too many rows");
     const size_t row_packed = static_cast<size_t>(cols / 2), row_scales = static_cast<size_t>(cols / 16);
     if (packed_bytes != static_cast<size_t>(all_rows) * row_packed ||
         scale_bytes != static_cast<size_t>(all_rows) * row_scales)
@@ -198,6 +202,11 @@ extern "C" NVFP4_API nvfp4_status nvfp4_linear_fused(nvfp4_runtime *runtime, con
     if (matrix->groups != 1) return fail_invalid("a matrix of several groups runs through nvfp4_linear_grouped");
     if (residual && (residual_stride < 0 || !aligned_to_type(residual, type)))
         return fail_invalid("invalid residual stride or alignment");
+    const long long e = type == NVFP4_TYPE_F32 ? 4 : 2;
+    if (residual && !(residual == out && (residual_stride == out_stride || vectors == 1)) &&
+        spans_overlap({residual, vectors, a.out_rows * e, residual_stride * e},
+                      {out, vectors, a.out_rows * e, out_stride * e}))
+        return fail_invalid("linear: the residual is out itself or does not overlap it");
     a.residual = residual;
     a.residual_stride = residual_stride;
     return run_fused(runtime, matrix, a, workspace, workspace_bytes, stream, "linear_fused");

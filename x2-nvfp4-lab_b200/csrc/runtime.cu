@@ -267,6 +267,18 @@ void raise_device_timeouts(nvfp4_runtime *runtime) {
     }
 }
 
+bool spans_overlap(const row_span &a, const row_span &b) {
+    if (!a.base || !b.base || a.rows <= 0 || b.rows <= 0) return false;
+    const intptr_t a0 = reinterpret_cast<intptr_t>(a.base), b0 = reinterpret_cast<intptr_t>(b.base);
+    const intptr_t a1 = a0 + (a.rows - 1) * a.stride + a.row_bytes, b1 = b0 + (b.rows - 1) * b.stride + b.row_bytes;
+    if (a1 <= b0 || b1 <= a0) return false;
+    if (a.stride == b.stride && a.stride > 0) {
+        const long long d = ((b0 - a0) % a.stride + a.stride) % a.stride;  // b's columns after a's in a's rows
+        if (d >= a.row_bytes && d + b.row_bytes <= a.stride) return false;
+    }
+    return true;
+}
+
 void check_on_device(const nvfp4_runtime *runtime, std::initializer_list<const void *> pointers,
                      const char *operation) {
     for (const void *p : pointers) {

@@ -141,13 +141,14 @@ class _ExpertSort(torch.autograd.Function):
         rows, *order = _sort(rt, x, ids, experts)
         record.extend(order)
         ctx.rt = rt
-        ctx.inverse = order[1]
+        ctx.save_for_backward(order[1])
         return rows
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, drows):
-        return _return(ctx.rt, drows, ctx.inverse, None, None, None), None, None, None, None
+        (inverse,) = ctx.saved_tensors
+        return _return(ctx.rt, drows, inverse, None, None, None), None, None, None, None
 
 
 class _ExpertReturn(torch.autograd.Function):
@@ -201,6 +202,10 @@ def expert_sort(rt, x, ids, experts: int, stream=None):
 
 
 def expert_return(rt, rows, order: ExpertOrder, weights=None, residual=None, out=None, stream=None):
+    _require(order.inverse.dim() == 2 and all(t.dtype == torch.int32 and t.is_contiguous()
+                                              for t in (order.inverse, order.offsets))
+             and order.offsets.numel() == order.experts + 1 and order.offsets.device == order.inverse.device,
+             "order must come from expert_sort: contiguous int32 inverse [tokens, topk] and offsets [experts + 1]")
     tokens, topk = order.inverse.shape
     _require(rows.is_cuda and rows.dim() == 2 and rows.dtype in TYPES and rows.shape[0] == tokens * topk
              and rows.shape[1] > 0 and rows.device == order.inverse.device,
