@@ -14,16 +14,22 @@
 // Warps: 0 producer of x and 2 of weights (TMA), 1 MMA issuer, 4-15 conversion
 // (three warpgroups, every third step of 128 columns each), 16-23 epilogue (two
 // warpgroups). Tensor memory: two accumulators of
-// 160 columns and three decoded steps of 64, or of 64 columns and six. The epilogue turns 32 columns at
-// a time through shared memory, so that a lane has four consecutive outputs of
-// one row of x: bias in registers, residual and stores as vectors.
+// 160 columns and three decoded steps of 64, or of 64 columns and six. The
+// epilogue works in registers: a lane has a weight row, one value of bias, and
+// trades with its neighbours for pairs of outputs. (Turning 32 columns a page in
+// shared memory for 8-byte stores cost 3,100 cycles a page in barriers, branches
+// and generic addresses, and was the bound of short rows: 9,006 FP16 rows x 512
+// over 64 groups of 2,048 weight rows took 41.5 us, 33.0 without.)
 //
-// One persistent CTA per SM walks (group, weight tile, x tile) items; x tiles of
-// a group are of even size, and items of one weight tile are neighbours, so
-// that its bytes come from HBM once.
+// Persistent pairs of CTAs, one CTA per SM, walk (group, two weight tiles, x
+// tile) items: each CTA decodes its own weight tile and loads half of the rows
+// of x, and the even one issues the MMAs of both. x tiles of a group are of even
+// size, and items of one weight tile are neighbours, so that its bytes come from
+// HBM once.
 //
-// An MMA (128 x N x 16, A in tensor memory) takes N / 2 + 10 cycles, measured;
-// with A in shared memory N / 2 + 43.
+// An MMA (of a pair: 256 x N x 16, A in tensor memory) takes N / 2 cycles and 37
+// at least, measured, when the next one is issued in time; of one CTA with A in
+// shared memory it takes N / 2 + 43.
 //
 // FP32 x enters as two FP16 halves, scaled per row by a power of two
 // (linear_gemv.cu has the error), split by a kernel before; x that TMA cannot
@@ -51,8 +57,6 @@ constexpr int kGmSegment32 = 1;                     // steps per accumulator of 
 constexpr int kGmRawBytes = 128 * 128;              // 256 columns of packed weights
 constexpr int kGmRawScales = 128 * 16;
 constexpr int kGmRaw = kGmRawBytes + kGmRawScales;
-constexpr int kGmEpiPitch = 148;                    // floats per row of x in the epilogue's turn
-constexpr int kGmEpiBytes = 32 * kGmEpiPitch * 4;
 
 // Tiles of up to N rows of x: tensor memory holds two accumulators of N columns and decoded weights in the rest, so
 // small tiles have six 128-column steps in flight, large ones three.
@@ -64,11 +68,10 @@ struct Shape {
     static constexpr int kRawStages = TERMS == 1 ? 6 : 4;  // 18 KB of weights each, as many as fit
     static constexpr int kColA = 2 * N;              // tensor-memory column of the first decoded step
     static constexpr int kOffRaw = kStages * kStageB;
-    static constexpr int kOffEpi = kOffRaw + kRawStages * kGmRaw;
-    static constexpr int kOffBars = kOffEpi + kGmEpiGroups * kGmEpiBytes;
+    static constexpr int kOffBars = kOffRaw + kRawStages * kGmRaw;
     static constexpr int kBars = 2 * kStages + 2 * kRawStages + 2 + 2 + 1;
-    static constexpr int kOffTiles = kOffBars + kBars * 8 + 24;
-    static constexpr size_t kSmem = 1024 + kOffTiles + sizeof(int) * (kLinMaxGroups + 1);
+    static constexpr int kOffTiles = kOffBars + kBars * 8 + 8;
+    static constexpr size_t kSmem = 1024 + kOffTiles + sizeof(int) * (3 * kLinMaxGroups + 1);
     static_assert(kOffTiles % 4 == 0 && kSmem <= 232448, "shared memory overflow");
     static_assert(kColA + 64 * kStages <= 512, "tensor memory overflow");
     static_assert(kHalfB % 1024 == 0 && kOffRaw % 1024 == 0 && kGmRaw % 1024 == 0, "swizzled tiles need 1024-byte alignment");
@@ -92,7 +95,7 @@ struct GemmArgs {
     int m_pairs;             // pairs of weight tiles of a group
     int raw_steps;           // 256-column steps over K
     int k_steps;             // 128-column steps over K
-    int wide_out, wide_res;  // four outputs may move as one vector
+    int pairs_out;           // two neighbouring 16-bit outputs (and two of the residual) may move as one word
 };
 
 // A warp's wait: one try and a vote on the way that matters, the bounded wait
@@ -143,6 +146,7 @@ struct Tile {
 // Tile sizes of a group of `count` rows: as many tiles as needed, even, a multiple of 16 rows each.
 __device__ __forceinline__ int x_tiles(int count, int max_n) { return (count + max_n - 1) / max_n; }
 
+// `upto` [groups + 1]: x tiles of the groups before; after it each group's first row and number of rows.
 __device__ __forceinline__ Tile tile_of(const GemmArgs &a, const int *upto, int item) {
     // The group with upto[g] * m_pairs <= item < upto[g + 1] * m_pairs.
     Tile t;
@@ -154,8 +158,8 @@ __device__ __forceinline__ Tile tile_of(const GemmArgs &a, const int *upto, int 
         else hi = mid;
     }
     t.group = lo;
-    int first, count;
-    group_range(a.f, lo, &first, &count);
+    const int groups = a.f.offsets ? a.f.groups : 1;
+    const int first = upto[groups + 1 + lo], count = upto[2 * groups + 1 + lo];
     const int tiles = upto[lo + 1] - upto[lo];
     const int in_group = item - upto[lo] * a.m_pairs;
     t.m = 2 * (in_group / tiles) + (int)cluster_rank();
@@ -167,100 +171,123 @@ __device__ __forceinline__ Tile tile_of(const GemmArgs &a, const int *upto, int 
 }
 
 template <int TYPE>
-__device__ __forceinline__ void load4(const void *p, size_t at, bool wide, int valid, float (&v)[4]) {
-    if constexpr (TYPE == NVFP4_TYPE_F32) {
-        const float *q = static_cast<const float *>(p) + at;
-        if (wide && valid == 4) {
-            const float4 w = *reinterpret_cast<const float4 *>(q);
-            v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
-            return;
-        }
-    } else if (wide && valid == 4) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + at);
-        uint16_t h[4];
-        memcpy(h, &w, 8);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = TYPE == NVFP4_TYPE_F16 ? __half2float(__ushort_as_half(h[i])) : bf16_bits_to_f32(h[i]);
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < valid ? load_as_f32(p, TYPE, at + i) : 0.0f;
+__device__ __forceinline__ float value_of(uint16_t bits) {
+    return TYPE == NVFP4_TYPE_F16 ? __half2float(__ushort_as_half(bits)) : bf16_bits_to_f32(bits);
 }
 
 template <int TYPE>
-__device__ __forceinline__ void store4(void *p, size_t at, bool wide, int valid, const float (&v)[4]) {
-    if (wide && valid == 4) {
-        if constexpr (TYPE == NVFP4_TYPE_F32) {
-            *reinterpret_cast<float4 *>(static_cast<float *>(p) + at) = make_float4(v[0], v[1], v[2], v[3]);
-        } else {
-            uint16_t h[4];
+__device__ __forceinline__ uint32_t pair_of(float lo, float hi) {
+    uint32_t word;
+    if constexpr (TYPE == NVFP4_TYPE_F16) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        memcpy(&word, &h, 4);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        memcpy(&word, &h, 4);
+    }
+    return word;
+}
+
+// What a lane of the epilogue does for a tile: it holds one weight row's sums, of 16 rows of x at a time.
+struct Finish {
+    int out0;      // its output (with a gate the one that its row and the row 16 lanes on make together)
+    int row0, n;   // rows of x of the tile
+    float inv, bias;
+};
+
+template <int ACT, int COUNT>
+__device__ __forceinline__ void activate_all(float (&y)[COUNT]) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) h[i] = TYPE == NVFP4_TYPE_F16 ? __half_as_ushort(__float2half_rn(v[i])) : f32_to_bf16_bits(v[i]);
-            uint2 w;
-            memcpy(&w, h, 8);
-            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p) + at) = w;
+    for (int i = 0; i < COUNT; ++i) y[i] = activate<ACT>(y[i]);
+}
+
+// 16 rows of x from c0 on: scale, bias, activation, gate, residual, one rounding, store. With a gate lanes 0-15 hold
+// gate rows and lanes 16-31 their up rows: lanes of the first half finish the even rows of x, of the second the odd
+// ones. 16-bit outputs then trade with the lane beside, so that a lane stores two neighbouring outputs of one row: a
+// warp writes 64 bytes of each row (32 with a gate), whole sectors, without shared memory.
+template <int TYPE, bool GATED>
+__device__ __forceinline__ void finish_rows(const GemmArgs &a, const Finish &t, int c0, const float (&sums)[16], float row_scale) {
+    constexpr int kOut = GATED ? 8 : 16, kRowStep = GATED ? 2 : 1;
+    constexpr int kBytes = TYPE == NVFP4_TYPE_F32 ? 4 : 2;
+    const FusedLinearArgs &f = a.f;
+    const int lane = threadIdx.x & 31;
+    float y[kOut], up[kOut];
+#pragma unroll
+    for (int i = 0; i < 16; i += kRowStep) {
+        float z[2];
+#pragma unroll
+        for (int k = 0; k < kRowStep; ++k) {
+            const float scale = TYPE == NVFP4_TYPE_F32 ? t.inv * __shfl_sync(0xffffffffu, row_scale, (c0 & 16) + i + k) : t.inv;
+            z[k] = fmaf(sums[i + k], scale, t.bias);
+        }
+        y[i / kRowStep] = z[0];
+        if constexpr (GATED) {
+            const float other = __shfl_xor_sync(0xffffffffu, lane < 16 ? z[1] : z[0], 16);
+            y[i / 2] = lane < 16 ? z[0] : other;
+            up[i / 2] = lane < 16 ? other : z[1];
+        }
+    }
+    switch (f.act) {
+        case NVFP4_ACT_RELU: activate_all<NVFP4_ACT_RELU>(y); break;
+        case NVFP4_ACT_SILU: activate_all<NVFP4_ACT_SILU>(y); break;
+        case NVFP4_ACT_GELU: activate_all<NVFP4_ACT_GELU>(y); break;
+        case NVFP4_ACT_GELU_TANH: activate_all<NVFP4_ACT_GELU_TANH>(y); break;
+        default: break;
+    }
+    if constexpr (GATED) {
+#pragma unroll
+        for (int i = 0; i < kOut; ++i) y[i] *= up[i];
+    }
+    const int first = c0 + (GATED ? lane >> 4 : 0);
+    const long long out_step = kRowStep * f.out_stride * kBytes, res_step = kRowStep * f.residual_stride * kBytes;
+    if (TYPE != NVFP4_TYPE_F32 && a.pairs_out) {
+        // Words of two outputs: even lanes those of row i, odd lanes of row i + 1; `half` picks a lane's part of both.
+        const int odd = lane & 1, row = first + odd * kRowStep, col = t.out0 - odd;
+        const uint32_t half = odd ? 0x3276u : 0x5410u;
+        const int left = col < f.out_rows ? t.n - row : 0;  // rows of x that this lane may store to
+        if (f.residual) {
+            const uint8_t *res = static_cast<const uint8_t *>(f.residual) + ((t.row0 + row) * f.residual_stride + col) * kBytes;
+            uint32_t r[kOut / 2];
+#pragma unroll
+            for (int i = 0; i < kOut; i += 2) {
+                r[i / 2] = 0;
+                if (i * kRowStep < left) r[i / 2] = *reinterpret_cast<const uint32_t *>(res + i * res_step);
+            }
+#pragma unroll
+            for (int i = 0; i < kOut; i += 2) {
+                const uint32_t mine = __byte_perm(r[i / 2], __shfl_xor_sync(0xffffffffu, r[i / 2], 1), half);
+                y[i] += value_of<TYPE>(static_cast<uint16_t>(mine));
+                y[i + 1] += value_of<TYPE>(static_cast<uint16_t>(mine >> 16));
+            }
+        }
+        uint8_t *out = static_cast<uint8_t *>(f.out) + ((t.row0 + row) * f.out_stride + col) * kBytes;
+#pragma unroll
+        for (int i = 0; i < kOut; i += 2) {
+            const uint32_t mine = pair_of<TYPE>(y[i], y[i + 1]);
+            const uint32_t word = __byte_perm(mine, __shfl_xor_sync(0xffffffffu, mine, 1), half);
+            if (i * kRowStep < left) *reinterpret_cast<uint32_t *>(out + i * out_step) = word;
         }
         return;
     }
+    const int left = t.out0 < f.out_rows ? t.n - first : 0;
+    if (f.residual) {
+        const uint8_t *res = static_cast<const uint8_t *>(f.residual) + ((t.row0 + first) * f.residual_stride + t.out0) * kBytes;
+        float r[kOut];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (i < valid) store_from_f32(p, TYPE, at + i, v[i]);
+        for (int i = 0; i < kOut; ++i) r[i] = i * kRowStep < left ? load_as_f32(res + i * res_step, TYPE, 0) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kOut; ++i) y[i] += r[i];
+    }
+    uint8_t *out = static_cast<uint8_t *>(f.out) + ((t.row0 + first) * f.out_stride + t.out0) * kBytes;
+#pragma unroll
+    for (int i = 0; i < kOut; ++i)
+        if (i * kRowStep < left) store_from_f32(out + i * out_step, TYPE, 0, y[i]);
 }
 
-// A turned page of up to 32 rows of x: scale, bias, activation, gate, residual, store. A lane has four outputs (from
-// `out0`, `valid` of them) of every 4th row from `first` on, with a gate of every 8th; all of its shared-memory reads
-// are made before the first store.
-template <int TYPE, int ACT, bool GATED>
-__device__ __forceinline__ void finish_page(const GemmArgs &a, const float *page, int row0, int n, int first, int col,
-                                            int out0, int valid, float inv, const float (&bias)[4],
-                                            const float (&bias_up)[4]) {
-    constexpr int kStep = GATED ? 8 : 4, kRows = 32 / kStep;
-    const FusedLinearArgs &f = a.f;
-    if (valid <= 0) return;
-    float4 z[kRows], up[GATED ? kRows : 1];
-    float scale[kRows];
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        const int v = first + i * kStep;
-        z[i] = *reinterpret_cast<const float4 *>(page + v * kGmEpiPitch + col);
-        if constexpr (GATED) up[i] = *reinterpret_cast<const float4 *>(page + v * kGmEpiPitch + 80 + col);
-        scale[i] = inv;
-        if (TYPE == NVFP4_TYPE_F32 && v < n) scale[i] = inv * __ldcg(a.row_scale + row0 + v);
-    }
-    constexpr int kBytes = TYPE == NVFP4_TYPE_F32 ? 4 : 2;
-    uint8_t *out = static_cast<uint8_t *>(f.out) + ((row0 + first) * f.out_stride + out0) * kBytes;
-    const uint8_t *res = static_cast<const uint8_t *>(f.residual) + ((row0 + first) * f.residual_stride + out0) * kBytes;
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        if (first + i * kStep < n) {
-            float y[4] = {z[i].x, z[i].y, z[i].z, z[i].w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = activate<ACT>(fmaf(y[e], scale[i], bias[e]));
-            if constexpr (GATED) {
-                y[0] *= fmaf(up[i].x, scale[i], bias_up[0]);
-                y[1] *= fmaf(up[i].y, scale[i], bias_up[1]);
-                y[2] *= fmaf(up[i].z, scale[i], bias_up[2]);
-                y[3] *= fmaf(up[i].w, scale[i], bias_up[3]);
-            }
-            if (f.residual) {
-                float r[4];
-                load4<TYPE>(res, 0, a.wide_res, valid, r);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] += r[e];
-            }
-            store4<TYPE>(out, 0, a.wide_out, valid, y);
-        }
-        out += kStep * f.out_stride * kBytes;
-        res += kStep * f.residual_stride * kBytes;
-    }
-}
-
-template <int TYPE, int ACT>
-__device__ __forceinline__ void finish_page(const GemmArgs &a, const float *page, int row0, int n, int first, int col,
-                                            int out0, int valid, float inv, const float (&bias)[4],
-                                            const float (&bias_up)[4]) {
-    if (a.f.gated) finish_page<TYPE, ACT, true>(a, page, row0, n, first, col, out0, valid, inv, bias, bias_up);
-    else finish_page<TYPE, ACT, false>(a, page, row0, n, first, col, out0, valid, inv, bias, bias_up);
+template <int TYPE>
+__device__ __forceinline__ void finish_rows(const GemmArgs &a, const Finish &t, int c0, const float (&sums)[16], float row_scale) {
+    if (a.f.gated) finish_rows<TYPE, true>(a, t, c0, sums, row_scale);
+    else finish_rows<TYPE, false>(a, t, c0, sums, row_scale);
 }
 
 // TYPE: of x, residual and out; FP32 x arrives as FP16 parts.
@@ -273,7 +300,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
     using Z = Shape<N, kTerms>;
     constexpr int S = Z::kStages, R = Z::kRawStages;
     extern __shared__ uint8_t gm_smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(gm_smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *smem = gm_smem_raw + (-smem_u32(gm_smem_raw) & 1023u);
     const FusedLinearArgs &f = a.f;
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + Z::kOffBars);    // [S] rows of x have landed, weights are decoded (four warps); even CTA: and the odd one's have
     uint64_t *empty = full + S;                                          // [S] the step's MMAs are done with both
@@ -283,8 +310,7 @@ __global__ void __launch_bounds__(kGmThreads, 1)
     uint64_t *acc_empty = acc_full + 2;                                  // [2] (every epilogue warp of both CTAs; even CTA)
     uint64_t *drain = acc_empty + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
-    int *acc_ok = reinterpret_cast<int *>(tmem_slot + 1);                // [epilogue warpgroups]
-    int *upto = reinterpret_cast<int *>(smem + Z::kOffTiles);             // [groups + 1] x tiles of the groups before
+    int *upto = reinterpret_cast<int *>(smem + Z::kOffTiles);             // [groups + 1] x tiles of the groups before (tile_of)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int *err = f.err;
     const uint32_t rank = cluster_rank();
@@ -333,6 +359,8 @@ __global__ void __launch_bounds__(kGmThreads, 1)
             int first, count;
             group_range(f, g, &first, &count);
             upto[g] = before;
+            upto[groups + 1 + g] = first;
+            upto[2 * groups + 1 + g] = count;
             before += x_tiles(count, a.max_n);
         }
     }
@@ -546,26 +574,15 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         // ----------------------------------------------------- epilogue
         const int piece = (warp - kGmEpiWarp0) >> 2, quarter = warp & 3;
         const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
-        float *page = reinterpret_cast<float *>(smem + Z::kOffEpi + piece * kGmEpiBytes);
-        // Place of this lane's weight row in a turned row of x: gate rows first, the up rows 80 floats on.
-        const int place = !f.gated ? 32 * quarter + lane : lane < 16 ? 16 * quarter + lane : 80 + 16 * quarter + lane - 16;
-        // Outputs of this lane after the turn: four, of one row of x (with a gate 16 lanes cover a row).
-        const int lanes_row = f.gated ? 16 : 32;
-        const int col = 4 * (lane & (lanes_row - 1));
-        const int vec0 = quarter * (f.gated ? 2 : 1) + (f.gated ? lane >> 4 : 0);
-        const int tile_rows = f.gated ? 64 : 128;
+        const int tile_rows = f.gated ? 64 : 128, own = f.gated ? 16 * quarter + (lane & 15) : 32 * quarter + lane;
         int use = 0;
-        // One thread waits, so that the four warps leave at the same place after a failure.
         auto filled = [&]() {
-            if ((threadIdx.x & 127) == 0)
-                acc_ok[piece] = mbar_wait(acc_full + (use & 1), (use >> 1) & 1u, err, kSiteFusedAccFull) ? 1 : 0;
-            named_barrier(1 + piece, 128);
-            const bool is = *reinterpret_cast<volatile int *>(acc_ok + piece) != 0;
+            const bool is = wait_warp(acc_full + (use & 1), (use >> 1) & 1u, err, kSiteFusedAccFull);
             tc::fence_after_sync();
             return is;
         };
         // With more tiles than pairs the warpgroups take whole tiles in turn (each its accumulator; what one waits for at
-        // the start of a tile hides behind the other's work), else every other 32 columns of the one tile. FP32 always
+        // the start of a tile hides behind the other's work), else every other 16 columns of the one tile. FP32 always
         // does the latter: its sums are in registers.
         const bool whole = TYPE != NVFP4_TYPE_F32 && items > pairs;
         auto release = [&]() {
@@ -583,34 +600,15 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                 continue;
             }
             const Tile t = tile_of(a, upto, item);
-            const int out0 = t.m * tile_rows + col, valid = min(4, f.out_rows - out0);
-            const float inv = f.inv_globals ? __ldg(f.inv_globals + t.group) : f.inv_global;
-            float bias[4] = {0, 0, 0, 0}, bias_up[4] = {0, 0, 0, 0};
-            if (f.bias) {
-                const size_t b = (size_t)t.group * f.rows + out0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (i >= valid) continue;
-                    bias[i] = load_as_f32(f.bias, f.bias_type, b + i);
-                    if (f.gated) bias_up[i] = load_as_f32(f.bias, f.bias_type, b + f.out_rows + i);
-                }
-            }
-            auto finish = [&](int c0) {
-                named_barrier(1 + piece, 128);
-                const int row0 = t.row0 + c0, n = min(32, t.n - c0);
-                switch (f.act) {
-                    case NVFP4_ACT_RELU: finish_page<TYPE, NVFP4_ACT_RELU>(a, page, row0, n, vec0, col, out0, valid, inv, bias, bias_up); break;
-                    case NVFP4_ACT_SILU: finish_page<TYPE, NVFP4_ACT_SILU>(a, page, row0, n, vec0, col, out0, valid, inv, bias, bias_up); break;
-                    case NVFP4_ACT_GELU: finish_page<TYPE, NVFP4_ACT_GELU>(a, page, row0, n, vec0, col, out0, valid, inv, bias, bias_up); break;
-                    case NVFP4_ACT_GELU_TANH: finish_page<TYPE, NVFP4_ACT_GELU_TANH>(a, page, row0, n, vec0, col, out0, valid, inv, bias, bias_up); break;
-                    default: finish_page<TYPE, NVFP4_ACT_NONE>(a, page, row0, n, vec0, col, out0, valid, inv, bias, bias_up);
-                }
-                named_barrier(1 + piece, 128);
-            };
+            Finish to{t.m * tile_rows + own, t.row0, t.n, f.inv_globals ? __ldg(f.inv_globals + t.group) : f.inv_global, 0.0f};
+            if (f.bias && to.out0 < f.out_rows)
+                to.bias = load_as_f32(f.bias, f.bias_type,
+                                      (size_t)t.group * f.rows + to.out0 + (f.gated && lane >= 16 ? f.out_rows : 0));
             if constexpr (TYPE == NVFP4_TYPE_F32) {
-                float sum[32];
+                const float row_scale = 32 * piece + lane < t.n ? __ldcg(a.row_scale + t.row0 + 32 * piece + lane) : 0.0f;
+                float sum[2][16];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) sum[i] = 0.0f;
+                for (int i = 0; i < 32; ++i) sum[i >> 4][i & 15] = 0.0f;
                 for (int ks = 0; ks < a.k_steps; ks += a.segment, ++use) {
                     if (!filled()) {
                         ok = false;
@@ -621,25 +619,24 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                     tc::wait_ld();
                     release();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) sum[i] += __uint_as_float(r[i]);
+                    for (int i = 0; i < 32; ++i) sum[i >> 4][i & 15] += __uint_as_float(r[i]);
                 }
                 if (!ok) break;
-                if (32 * piece < t.n) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) page[i * kGmEpiPitch + place] = sum[i];
-                    finish(32 * piece);
-                }
+                for (int h = 0; h < 2; ++h)
+                    if (32 * piece + 16 * h < t.n) finish_rows<TYPE>(a, to, 32 * piece + 16 * h, sum[h], row_scale);
             } else {
                 if (!filled()) break;
-                const int step = whole ? 32 : 32 * kGmEpiGroups, c_first = whole ? 0 : 32 * piece;
+                const int step = whole ? 16 : 16 * kGmEpiGroups, c_first = whole ? 0 : 16 * piece;
                 for (int c0 = c_first; c0 < t.n; c0 += step) {
-                    uint32_t r[32];
-                    tc::ld_32x32b_x32(lanes + (use & 1) * N + c0, r);
+                    uint32_t r[16];
+                    float sum[16];
+                    tc::ld_32x32b_x16(lanes + (use & 1) * N + c0, r);
                     tc::wait_ld();
                     if (c0 + step >= t.n) release();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) page[i * kGmEpiPitch + place] = __uint_as_float(r[i]);
-                    finish(c0);
+                    for (int i = 0; i < 16; ++i) sum[i] = __uint_as_float(r[i]);
+                    finish_rows<TYPE>(a, to, c0, sum, 1.0f);
                 }
                 if (c_first >= t.n) release();
                 ++use;
@@ -758,12 +755,8 @@ void launch_linear_gemm(const FusedLinearArgs &f, const nvfp4_matrix &matrix, vo
     // One box for half of the even tiles of a single group; 16 rows for ranges known on the device.
     const int tiles = (f.vectors + g.max_n - 1) / g.max_n;
     g.box_rows = f.offsets ? 16 : ((f.vectors + tiles - 1) / tiles + 15) / 16 * 8;
-    const int e = f.type == NVFP4_TYPE_F32 ? 4 : 2;
-    auto vectors_of_4 = [&](const void *p, long long stride) {
-        return (reinterpret_cast<uintptr_t>(p) % (4 * e)) == 0 && stride % 4 == 0 ? 1 : 0;
-    };
-    g.wide_out = vectors_of_4(f.out, f.out_stride);
-    g.wide_res = f.residual ? vectors_of_4(f.residual, f.residual_stride) : 0;
+    auto words = [](const void *p, long long stride) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0 && (stride & 1) == 0; };
+    g.pairs_out = (f.out_rows & 1) == 0 && words(f.out, f.out_stride) && (!f.residual || words(f.residual, f.residual_stride));
     const bool direct = in_place(f.type, f.x, f.x_stride, f.cols);
     const void *rows = f.x;
     long long stride = f.x_stride;

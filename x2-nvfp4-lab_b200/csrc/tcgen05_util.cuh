@@ -194,6 +194,15 @@ __device__ __forceinline__ void ld_32x32b_x32(uint32_t addr, uint32_t (&r)[32]) 
         : "r"(addr));
 }
 
+// 16 of them.
+__device__ __forceinline__ void ld_32x32b_x16(uint32_t addr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+}
+
 // Four consecutive accumulator columns of the warp's 32 lanes.
 __device__ __forceinline__ void ld_32x32b_x4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
