@@ -59,19 +59,21 @@ constexpr int kGmRawScales = 128 * 16;
 constexpr int kGmRaw = kGmRawBytes + kGmRawScales;
 
 // Tiles of up to N rows of x: tensor memory holds two accumulators of N columns and decoded weights in the rest, so
-// small tiles have six 128-column steps in flight, large ones three.
+// small tiles have six decoded 128-column steps in flight, large ones three; x has a ring of its own.
 template <int N, int TERMS>
 struct Shape {
     static constexpr int kStages = (512 - 2 * N) / 64;
     static constexpr int kHalfB = TERMS * N / 2 * 128;  // a CTA's half of x's rows in a tile, 64 columns of them
     static constexpr int kStageB = 2 * kHalfB;
-    static constexpr int kRawStages = TERMS == 1 ? 6 : 4;  // 18 KB of weights each, as many as fit
+    static constexpr int kXStages = 6;               // steps of x in flight (a multiple of kStages)
+    static constexpr int kRawStages = N == kGmLargeN ? 5 : 6;  // 18 KB of weights each, as many as fit
     static constexpr int kColA = 2 * N;              // tensor-memory column of the first decoded step
-    static constexpr int kOffRaw = kStages * kStageB;
+    static constexpr int kOffRaw = kXStages * kStageB;
     static constexpr int kOffBars = kOffRaw + kRawStages * kGmRaw;
-    static constexpr int kBars = 2 * kStages + 2 * kRawStages + 2 + 2 + 1;
+    static constexpr int kBars = 2 * kStages + 2 * kXStages + 2 * kRawStages + 2 + 2 + 1;
     static constexpr int kOffTiles = kOffBars + kBars * 8 + 8;
     static constexpr size_t kSmem = 1024 + kOffTiles + sizeof(int) * (3 * kLinMaxGroups + 1);
+    static_assert(kXStages % kStages == 0, "the MMA warp's loop is unrolled over both rings");
     static_assert(kOffTiles % 4 == 0 && kSmem <= 232448, "shared memory overflow");
     static_assert(kColA + 64 * kStages <= 512, "tensor memory overflow");
     static_assert(kHalfB % 1024 == 0 && kOffRaw % 1024 == 0 && kGmRaw % 1024 == 0, "swizzled tiles need 1024-byte alignment");
@@ -84,13 +86,15 @@ enum GemmWaitSite : int {
     kSiteFusedFull = 74,
     kSiteFusedAccEmpty = 75,
     kSiteFusedAccFull = 76,
+    kSiteFusedRowsEmpty = 77,
+    kSiteFusedRowsFull = 78,
 };
 
 struct GemmArgs {
     FusedLinearArgs f;
     const float *row_scale;  // [vectors] of split FP32 x (NULL: ones)
     int max_n;               // rows of x per tile
-    int box_rows;            // rows of x per TMA box
+    int box_rows;            // rows of x per TMA box: a CTA's half of a tile, or more
     int segment;             // steps per accumulator
     int m_pairs;             // pairs of weight tiles of a group
     int raw_steps;           // 256-column steps over K
@@ -298,13 +302,15 @@ __global__ void __launch_bounds__(kGmThreads, 1)
     constexpr bool kBf16 = TYPE == NVFP4_TYPE_BF16;
     constexpr int kTerms = TYPE == NVFP4_TYPE_F32 ? 2 : 1;
     using Z = Shape<N, kTerms>;
-    constexpr int S = Z::kStages, R = Z::kRawStages;
+    constexpr int S = Z::kStages, X = Z::kXStages, R = Z::kRawStages;
     extern __shared__ uint8_t gm_smem_raw[];
     uint8_t *smem = gm_smem_raw + (-smem_u32(gm_smem_raw) & 1023u);
     const FusedLinearArgs &f = a.f;
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + Z::kOffBars);    // [S] rows of x have landed, weights are decoded (four warps); even CTA: and the odd one's have
-    uint64_t *empty = full + S;                                          // [S] the step's MMAs are done with both
-    uint64_t *raw_full = empty + S;                                      // [R] packed weights and scales have landed
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + Z::kOffBars);    // [S] weights are decoded (four warps); even CTA: and the odd one's weights and rows of x are there
+    uint64_t *empty = full + S;                                          // [S] the step's MMAs are done with the weights
+    uint64_t *x_full = empty + S;                                        // [X] rows of x have landed
+    uint64_t *x_empty = x_full + X;                                      // [X] the step's MMAs are done with them
+    uint64_t *raw_full = x_empty + X;                                      // [R] packed weights and scales have landed
     uint64_t *raw_empty = raw_full + R;                                  // [R] (four conversion warps for each of its two steps)
     uint64_t *acc_full = raw_empty + R;                                  // [2]
     uint64_t *acc_empty = acc_full + 2;                                  // [2] (every epilogue warp of both CTAs; even CTA)
@@ -318,8 +324,12 @@ __global__ void __launch_bounds__(kGmThreads, 1)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i) {
-            mbar_init(full + i, 1 + 4 + (rank == 0 ? 1 : 0));
+            mbar_init(full + i, 4 + (rank == 0 ? 1 : 0));
             mbar_init(empty + i, 1);
+        }
+        for (int i = 0; i < X; ++i) {
+            mbar_init(x_full + i, 1);
+            mbar_init(x_empty + i, 1);
         }
         for (int i = 0; i < R; ++i) {
             mbar_init(raw_full + i, 1);
@@ -380,30 +390,29 @@ __global__ void __launch_bounds__(kGmThreads, 1)
             const Tile t = tile_of(a, upto, item);
             // The pair splits the tile's rows: this CTA's are the first or the second half of N.
             const int half = ((t.n + 15) & ~15) / 2, row0 = t.row0 + (int)rank * half;
-            const int boxes = (half + a.box_rows - 1) / a.box_rows;
             for (int ks = 0; ks < a.k_steps; ++ks, ++it) {
-                const int st = it % S;
-                if (!wait_warp(empty + st, ((it / S) & 1u) ^ 1u, err, kSiteFusedEmpty)) {
+                const int st = it % X;
+                if (!wait_warp(x_empty + st, ((it / X) & 1u) ^ 1u, err, kSiteFusedRowsEmpty)) {
                     ok = false;
                     break;
                 }
                 uint8_t *b = smem + st * Z::kStageB;
                 if (tc::elect_one()) {
-                    mbar_arrive_expect_tx(full + st, 2 * kTerms * boxes * a.box_rows * 128);
-                    for (int j = 0; j < kTerms; ++j)
-                        for (int x = 0; x < boxes; ++x) {
-                            uint8_t *to = b + (j * (kGmSmallN / 2) + x * a.box_rows) * 128;
-                            const int row = j * f.vectors + row0 + x * a.box_rows;
-                            tma_load_2d(to, &tm_x, full + st, ks * 256, row);
-                            tma_load_2d(to + Z::kHalfB, &tm_x, full + st, ks * 256 + 128, row);
-                        }
+                    mbar_arrive_expect_tx(x_full + st, 2 * kTerms * a.box_rows * 128);
+#pragma unroll
+                    for (int j = 0; j < kTerms; ++j) {
+                        uint8_t *to = b + j * (kGmSmallN / 2) * 128;
+                        const int row = j * f.vectors + row0;
+                        tma_load_2d(to, &tm_x, x_full + st, ks * 256, row);
+                        tma_load_2d(to + Z::kHalfB, &tm_x, x_full + st, ks * 256 + 128, row);
+                    }
                 }
                 __syncwarp();
             }
         }
         // After a failure the copies of the last stages issued land before the CTA ends.
         if (!ok || *reinterpret_cast<volatile int *>(err) != 0)
-            for (uint32_t k = it > (uint32_t)S ? it - S : 0u; k < it; ++k) wait_drain(full + k % S, (k / S) & 1u);
+            for (uint32_t k = it > (uint32_t)X ? it - X : 0u; k < it; ++k) wait_drain(x_full + k % X, (k / X) & 1u);
         __syncwarp();
     } else if (warp == 2) {
         // ----------------------------------------- producer of weights
@@ -437,22 +446,24 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         // Everything an instruction takes is the same in every lane and known to be (reductions, loop counters).
         const uint64_t desc = tc::smem_desc_sw128(smem_u32(smem));  // its address field cannot overflow
         const int last = __reduce_max_sync(0xffffffffu, items);
-        uint32_t st = 0, ph = 0;
+        uint32_t st = 0, ph = 0, x_ph = 0;  // step in the ring of x; phases of the weights' ring and of x's
         bool ok = true;
         uint32_t use = 0;  // accumulators filled so far
         if (rank == 1) {
             // The odd CTA tells the even one, which issues for both, when its half of a step is there.
+            uint32_t wst = 0;
             for (int item = pair; item < last && ok; item += pairs) {
                 for (int ks = 0; ks < a.k_steps; ++ks) {
-                    if (!wait_warp(full + st, ph, err, kSiteFusedFull)) {
+                    if (!wait_warp(x_full + st, x_ph, err, kSiteFusedRowsFull) || !wait_warp(full + wst, ph, err, kSiteFusedFull)) {
                         ok = false;
                         break;
                     }
                     tc::fence_after_sync();
                     tc::fence_before_sync();
-                    if (tc::elect_one()) mbar_arrive_at(full + st, 0);
+                    if (tc::elect_one()) mbar_arrive_at(full + wst, 0);
                     __syncwarp();
-                    if (++st == S) st = 0, ph ^= 1;
+                    if (++wst == S) wst = 0, ph ^= 1;
+                    if (++st == X) st = 0, x_ph ^= 1;
                 }
             }
         } else {
@@ -470,9 +481,12 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                     // against 150 cycles of a step's issue, measured alone).
                     for (int todo = min(left, a.segment); todo > 0 && ok;) {
 #pragma unroll
-                        for (int stage = 0; stage < S; ++stage) {
+                        for (int stage = 0; stage < X; ++stage) {
+                            constexpr int kS = S;
+                            const int ws = stage % kS;
                             if (st != stage || todo == 0 || !ok) continue;
-                            if (!wait_warp(full + stage, ph, err, kSiteFusedFull)) {
+                            if (!wait_warp(x_full + stage, x_ph, err, kSiteFusedRowsFull) ||
+                                !wait_warp(full + ws, ph, err, kSiteFusedFull)) {
                                 ok = false;
                                 continue;
                             }
@@ -483,17 +497,19 @@ __global__ void __launch_bounds__(kGmThreads, 1)
 #pragma unroll
                                     for (int i = 0; i < 8; ++i)
                                         tc::mma_16bit_ts_pair(
-                                            acc, tmem + Z::kColA + 64 * stage + 8 * i,
+                                            acc, tmem + Z::kColA + 64 * ws + 8 * i,
                                             desc + ((stage * Z::kStageB + (i >> 2) * Z::kHalfB + j * (kGmSmallN / 2) * 128 +
                                                      32 * (i & 3)) >> 4),
                                             idesc, j != kTerms - 1 || i != 0 ? 1u : more);
-                                tc::commit_pair(empty + stage);
+                                tc::commit_pair(empty + ws);
+                                tc::commit_pair(x_empty + stage);
                             }
                             __syncwarp();
                             more = 1;
                             --todo;
-                            st = (stage + 1) % S;
-                            if (stage + 1 == S) ph ^= 1;
+                            st = (stage + 1) % X;
+                            if (ws + 1 == kS) ph ^= 1;
+                            if (stage + 1 == X) x_ph ^= 1;
                         }
                     }
                     if (ok && tc::elect_one()) tc::commit_pair(acc_full + buf);
@@ -752,9 +768,11 @@ void launch_linear_gemm(const FusedLinearArgs &f, const nvfp4_matrix &matrix, vo
     g.k_steps = (f.cols + 127) / 128;
     g.raw_steps = (f.cols + 255) / 256;
     g.segment = f.type == NVFP4_TYPE_F32 ? kGmSegment32 : g.k_steps;
-    // One box for half of the even tiles of a single group; 16 rows for ranges known on the device.
+    // A CTA's half of a tile in one box (a piece that hangs over loads rows that no sum of the tile uses): fitted to the
+    // even tiles of a single group, the most that a tile holds where the counts are on the device (boxes of 16 rows
+    // instead: 8,192 rows over 64 groups 39.3 against 38.4 us).
     const int tiles = (f.vectors + g.max_n - 1) / g.max_n;
-    g.box_rows = f.offsets ? 16 : ((f.vectors + tiles - 1) / tiles + 15) / 16 * 8;
+    g.box_rows = f.offsets ? g.max_n / 2 : ((f.vectors + tiles - 1) / tiles + 15) / 16 * 8;
     auto words = [](const void *p, long long stride) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0 && (stride & 1) == 0; };
     g.pairs_out = (f.out_rows & 1) == 0 && words(f.out, f.out_stride) && (!f.residual || words(f.residual, f.residual_stride));
     const bool direct = in_place(f.type, f.x, f.x_stride, f.cols);
