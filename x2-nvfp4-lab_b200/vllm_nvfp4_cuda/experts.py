@@ -42,10 +42,8 @@ def _row_stride(t: torch.Tensor) -> int:
 
 
 def on_stream(stream, tensors, call):
-    """``call()`` on torch's current stream, or on ``stream``: what it allocates then belongs to that stream, and
-    the given tensors are kept from reuse until the stream is done with them."""
-    if stream is None:
-        return call()
+    """``call()`` on ``stream``: what it allocates then belongs to that stream, and the given tensors are kept from reuse
+    until the stream is done with them."""
     with torch.cuda.stream(stream):
         result = call()
     for t in tensors:
@@ -69,7 +67,8 @@ def _sort(rt, x, ids, experts):
     picks = tokens * topk
     rows = x.new_empty((picks, hidden))
     table = torch.empty(2 * picks + experts + 1, dtype=torch.int32, device=x.device)
-    perm, inverse, offsets = table[:picks], table[picks:2 * picks].view(tokens, topk), table[2 * picks:]
+    perm, inverse, offsets = table.split((picks, picks, experts + 1))
+    inverse = inverse.view(tokens, topk)
     if tokens == 0:
         offsets.zero_()
         return rows, perm, inverse, offsets
@@ -134,6 +133,29 @@ def _return_backward(rt, dout, rows, inverse, offsets, weights, experts, need_ro
 # ------------------------------------------------------------------ gradients
 
 
+# Of a gradient there is no gradient: where one is recorded (create_graph) the result says so when it is asked for. The
+# guard costs several microseconds of the host, which an ordinary backward pass goes without.
+
+
+def _sort_gradient(ctx, drows):
+    (inverse,) = ctx.saved_tensors
+    return _return(ctx.rt, drows, inverse, None, None, None), None, None, None, None
+
+
+def _return_gradient(ctx, dout):
+    rows, weights, inverse, offsets = ctx.saved_tensors
+    need_rows, need_weights, need_residual = ctx.needs_input_grad[:3]
+    drows = dweights = None
+    if need_rows or need_weights:
+        drows, dweights = _return_backward(ctx.rt, dout, rows, inverse, offsets, weights, ctx.experts, need_rows,
+                                           need_weights)
+    return drows, dweights, dout if need_residual else None, None, None
+
+
+_sort_gradient_once = torch.autograd.function.once_differentiable(_sort_gradient)
+_return_gradient_once = torch.autograd.function.once_differentiable(_return_gradient)
+
+
 class _ExpertSort(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, rt, ids, experts, record):
@@ -145,10 +167,8 @@ class _ExpertSort(torch.autograd.Function):
         return rows
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, drows):
-        (inverse,) = ctx.saved_tensors
-        return _return(ctx.rt, drows, inverse, None, None, None), None, None, None, None
+        return _sort_gradient_once(ctx, drows) if torch.is_grad_enabled() else _sort_gradient(ctx, drows)
 
 
 class _ExpertReturn(torch.autograd.Function):
@@ -156,22 +176,14 @@ class _ExpertReturn(torch.autograd.Function):
     def forward(ctx, rows, weights, residual, rt, order):
         ctx.rt = rt
         ctx.experts = order.experts
-        ctx.given = (weights is not None, residual is not None)
         # The rows are kept only for the weights' gradient.
         keep = weights is not None and ctx.needs_input_grad[1]
         ctx.save_for_backward(rows if keep else None, weights, order.inverse, order.offsets)
         return _return(rt, rows, order.inverse, weights, residual, None)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        rows, weights, inverse, offsets = ctx.saved_tensors
-        need_rows, need_weights, need_residual = ctx.needs_input_grad[:3]
-        drows = dweights = None
-        if need_rows or need_weights:
-            drows, dweights = _return_backward(ctx.rt, dout, rows, inverse, offsets, weights, ctx.experts, need_rows,
-                                               need_weights)
-        return drows, dweights, dout if need_residual else None, None, None
+        return _return_gradient_once(ctx, dout) if torch.is_grad_enabled() else _return_gradient(ctx, dout)
 
 
 # ------------------------------------------------------------------ checks
@@ -187,49 +199,54 @@ def expert_sort(rt, x, ids, experts: int, stream=None):
              "x must be a CUDA bfloat16, float16 or float32 tensor [tokens, hidden]")
     _require(ids.dtype in (torch.int32, torch.int64) and ids.dim() == 2 and ids.shape[0] == x.shape[0]
              and ids.device == x.device, "ids must be int32 or int64 [tokens, topk] on x's device")
-    _require(1 <= ids.shape[1] <= MAX_TOPK, f"the expert sort supports 1 to {MAX_TOPK} picks a token")
+    _require(1 <= ids.shape[1] <= MAX_TOPK, "the expert sort supports 1 to 64 picks a token")
     experts = int(experts)
-    _require(1 <= experts <= MAX_EXPERTS, f"the expert sort supports 1 to {MAX_EXPERTS} experts")
+    _require(1 <= experts <= MAX_EXPERTS, "the expert sort supports 1 to 1024 experts")
+    grad = x.requires_grad and torch.is_grad_enabled()
 
     def call():
-        if x.requires_grad and torch.is_grad_enabled():
+        if grad:
             record = []
             return _ExpertSort.apply(x, rt, ids, experts, record), *record
         return _sort(rt, x, ids, experts)
 
-    rows, perm, inverse, offsets = on_stream(stream, (x, ids), call)
+    rows, perm, inverse, offsets = call() if stream is None else on_stream(stream, (x, ids), call)
     return rows, ExpertOrder(perm, inverse, offsets, experts)
 
 
 def expert_return(rt, rows, order: ExpertOrder, weights=None, residual=None, out=None, stream=None):
-    _require(order.inverse.dim() == 2 and all(t.dtype == torch.int32 and t.is_contiguous()
-                                              for t in (order.inverse, order.offsets))
-             and order.offsets.numel() == order.experts + 1 and order.offsets.device == order.inverse.device,
+    inverse, offsets = order.inverse, order.offsets
+    _require(inverse.dtype == torch.int32 and offsets.dtype == torch.int32 and inverse.dim() == 2
+             and inverse.is_contiguous() and offsets.is_contiguous() and offsets.numel() == order.experts + 1
+             and offsets.device == inverse.device,
              "order must come from expert_sort: contiguous int32 inverse [tokens, topk] and offsets [experts + 1]")
-    tokens, topk = order.inverse.shape
-    _require(rows.is_cuda and rows.dim() == 2 and rows.dtype in TYPES and rows.shape[0] == tokens * topk
-             and rows.shape[1] > 0 and rows.device == order.inverse.device,
+    tokens, topk = inverse.shape
+    device, hidden = rows.device, rows.shape[-1]
+    _require(rows.is_cuda and rows.dim() == 2 and rows.dtype in TYPES and rows.shape[0] == tokens * topk and hidden > 0
+             and device == inverse.device,
              "rows must be a CUDA bfloat16, float16 or float32 tensor [tokens * topk, hidden] on the order's device")
-    shape = (tokens, rows.shape[1])
+    grad = rows.requires_grad
     if weights is not None:
-        _require(tuple(weights.shape) == (tokens, topk) and weights.dtype in TYPES and weights.device == rows.device,
+        _require(weights.shape == inverse.shape and weights.dtype in TYPES and weights.device == device,
                  "weights must be bfloat16, float16 or float32 [tokens, topk] on the rows' device")
+        grad = grad or weights.requires_grad
     if residual is not None:
-        _require(tuple(residual.shape) == shape and residual.dtype == rows.dtype and residual.device == rows.device,
+        _require(residual.shape == (tokens, hidden) and residual.dtype == rows.dtype and residual.device == device,
                  "residual must match the rows' type and device, [tokens, hidden]")
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (rows, weights, residual))
+        grad = grad or residual.requires_grad
+    grad = grad and torch.is_grad_enabled()
     if out is not None:
-        _require(tuple(out.shape) == shape and out.dtype == rows.dtype and out.device == rows.device
-                 and (out.stride(1) == 1 or shape[1] == 1) and (tokens < 2 or out.stride(0) >= shape[1]),
+        _require(out.shape == (tokens, hidden) and out.dtype == rows.dtype and out.device == device
+                 and (out.stride(1) == 1 or hidden == 1) and (tokens < 2 or out.stride(0) >= hidden),
                  "out must match the rows' type and device, [tokens, hidden] with contiguous columns")
         _require(not grad and not out.requires_grad, "out cannot be given where gradients are recorded")
 
     def call():
         if grad:
             return _ExpertReturn.apply(rows, weights, residual, rt, order)
-        return _return(rt, rows, order.inverse, weights, residual, out)
+        return _return(rt, rows, inverse, weights, residual, out)
 
-    return on_stream(stream, (rows, order.inverse, order.offsets, weights, residual, out), call)
+    return call() if stream is None else on_stream(stream, (rows, inverse, offsets, weights, residual, out), call)
 
 
 __all__ = ["ExpertOrder", "expert_return", "expert_sort"]

@@ -15,6 +15,8 @@ forwards on torch tensors, routing introspection and device-side uploads.
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import importlib
 import os
 import threading
 from dataclasses import dataclass
@@ -350,6 +352,12 @@ class EpContext:
         if self.handle:
             self.runtime.lib.nvfp4_ep_destroy(self.handle)
             self.handle = C.c_void_p()
+
+
+@functools.lru_cache(maxsize=None)
+def _module(name: str):
+    """A module of this package that needs torch, imported at its first use."""
+    return importlib.import_module(f"{__package__}.{name}")
 
 
 class NativeMatrix:
@@ -1045,9 +1053,7 @@ class Runtime:
         rows is the gate: act(gate) * up, rows / 2 outputs). Sums are FP32,
         the result is rounded once. Inference only. Enqueued on ``stream``
         (None: torch's current stream)."""
-        from . import fused
-
-        return fused.linear_fused(self, matrix, x, bias, activation, residual, out, stream)
+        return _module("fused").linear_fused(self, matrix, x, bias, activation, residual, out, stream)
 
     def linear_grouped(self, matrix: NativeMatrix, x, offsets, *, bias=None, activation: str | None = None, out=None,
                        stream=None):
@@ -1056,9 +1062,7 @@ class Runtime:
         matrix and bias[g] (bias [groups, rows]). offsets: int32 [groups + 1]
         on the GPU (``ExpertOrder.offsets``). Rows of no group are zero in a
         new out and left as they were in a given one."""
-        from . import fused
-
-        return fused.linear_grouped(self, matrix, x, offsets, bias, activation, out, stream)
+        return _module("fused").linear_grouped(self, matrix, x, offsets, bias, activation, out, stream)
 
     def expert_sort(self, x, ids, experts: int, stream=None):
         """additive: (rows, order): every token's row of x [tokens, hidden]
@@ -1067,17 +1071,13 @@ class Runtime:
         dropped, and as many rows at the end are zero. Differentiable in x
         (vllm_nvfp4_cuda.experts). Enqueued on ``stream`` (None: torch's
         current stream)."""
-        from . import experts as impl
-
-        return impl.expert_sort(self, x, ids, experts, stream)
+        return _module("experts").expert_sort(self, x, ids, experts, stream)
 
     def expert_return(self, rows, order, weights=None, residual=None, out=None, stream=None):
         """additive: out[t] = residual[t] + sum_k weights[t, k] * rows[order.inverse[t, k]]
         ([tokens, hidden], dropped picks left out, FP32 sums; weights None:
         ones). Differentiable in rows, weights and residual."""
-        from . import experts as impl
-
-        return impl.expert_return(self, rows, order, weights, residual, out, stream)
+        return _module("experts").expert_return(self, rows, order, weights, residual, out, stream)
 
     def quantize_rows(self, x, terms: int):
         """additive: split BF16/FP16 rows [rows, cols] (a CUDA tensor) into
