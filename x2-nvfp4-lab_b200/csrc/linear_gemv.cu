@@ -211,6 +211,55 @@ __device__ __forceinline__ void stage_rows(const GemvArgs &a, uint8_t *xs, uint3
     __syncthreads();
 }
 
+// The same for 16-bit rows through asynchronous copies: the raw bytes go to their places, all in flight at once; then
+// every thread looks for the rows' maxima in what it copied itself, and last converts it in place.
+template <int TYPE>
+__device__ __forceinline__ void stage_rows_async(const GemvArgs &a, uint8_t *xs, uint32_t *amax, float *back, int row0, int n) {
+    const FusedLinearArgs &f = a.f;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const bool wide = ((reinterpret_cast<uintptr_t>(f.x) | (uintptr_t)(f.x_stride * 2)) & 15u) == 0;
+    // work(row, octet, place) for this thread's octets.
+    auto each = [&](auto &&work) {
+        int r = warp / a.chunks, c = warp - r * a.chunks;
+        while (r < n) {
+            work(r, 32 * c + lane, xs + r * a.token_stride + staged_byte(32 * c + lane));
+            for (c += kGvWarps; c >= a.chunks; c -= a.chunks) ++r;
+        }
+    };
+    if (threadIdx.x < n) amax[threadIdx.x] = 0u;
+    each([&](int r, int o, uint8_t *to) {
+        if (8 * o >= f.cols) {
+            *reinterpret_cast<uint4 *>(to) = make_uint4(0, 0, 0, 0);
+        } else if (wide) {
+            cp_async16(to, static_cast<const uint16_t *>(f.x) + (row0 + r) * f.x_stride + 8 * o);
+        } else {
+            const Octet<TYPE> v = load_octet<TYPE>(f, row0 + r, 8 * o, false);
+            *reinterpret_cast<uint4 *>(to) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+        }
+    });
+    cp_async_wait_all();
+    if constexpr (TYPE == NVFP4_TYPE_F16) {
+        if (threadIdx.x < n) back[threadIdx.x] = 1.0f;
+    } else {
+        auto read = [&](const uint8_t *at) {
+            const uint4 q = *reinterpret_cast<const uint4 *>(at);
+            return Octet<TYPE>{{q.x, q.y, q.z, q.w}};
+        };
+        __syncthreads();  // amax is zero
+        each([&](int r, int, const uint8_t *at) {
+            const Octet<TYPE> v = read(at);
+            float m = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(v.get(j)));
+            const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+            if (lane == 0) atomicMax(amax + r, top);
+        });
+        __syncthreads();
+        each([&](int r, int o, const uint8_t *at) { stage_octet<TYPE>(a, xs, amax, back, r, o, read(at)); });
+    }
+    __syncthreads();
+}
+
 template <int TYPE>
 __global__ void __launch_bounds__(kGvThreads, 2) linear_gemv_kernel(const __grid_constant__ GemvArgs a) {
     extern __shared__ __align__(16) uint8_t gv_smem[];
@@ -330,7 +379,15 @@ __global__ void __launch_bounds__(kGvThreads, 2) linear_gemv_kernel(const __grid
             load(b0);
             load(b1);
             __syncthreads();  // the rows staged before are no longer read
-            stage_rows<TYPE>(a, xs, amax, back, first + v0, n);
+            // 16-bit rows of more than an octet a thread go by asynchronous copies: 8 rows at 2048 x 16384 12.5 us (13.4
+            // through registers), 768 rows over 256 groups 70.9 us (73.6); one row 8.6 us (8.0), and four of FP32, whose
+            // halves lie apart, 14.5 us (11.0).
+            bool async = false;
+            if constexpr (TYPE != NVFP4_TYPE_F32) async = n * a.chunks > kGvWarps;
+            if constexpr (TYPE != NVFP4_TYPE_F32) {
+                if (async) stage_rows_async<TYPE>(a, xs, amax, back, first + v0, n);
+            }
+            if (!async) stage_rows<TYPE>(a, xs, amax, back, first + v0, n);
             // MMA columns past the staged ones repeat the last: their sums are not stored.
             const uint8_t *bcol = xs + min(g, ncols - 1) * a.token_stride + t * 160;
 
@@ -487,6 +544,10 @@ void launch_linear_gemv(const FusedLinearArgs &f, int device, int sm_count, cuda
     const long long tiles = (long long)a.tiles * (f.offsets ? std::min(f.groups, f.vectors) : 1);
     a.warps_k = 1;
     while (a.warps_k < kGvWarps && 2 * a.warps_k <= a.chunks && tiles * a.warps_k < (long long)sm_count * 8) a.warps_k *= 2;
+    // Groups make a CTA's run of tiles end in the middle of its teams' turn, twice where it crosses into the next group:
+    // two warps a tile of 2,048 columns or more as long as every team has several (256 rows over 256 groups of 1,024 x
+    // 2,048 50.9 against 54.1 us; with one tile a team 16.2 against 12.1, at 512 columns 35.4 against 31.4).
+    if (f.offsets && a.warps_k == 1 && a.chunks >= 8 && tiles > 2LL * sm_count * kGvWarps) a.warps_k = 2;
     if (f.type == NVFP4_TYPE_BF16) launch<NVFP4_TYPE_BF16>(a, device, sm_count, stream);
     else if (f.type == NVFP4_TYPE_F16) launch<NVFP4_TYPE_F16>(a, device, sm_count, stream);
     else launch<NVFP4_TYPE_F32>(a, device, sm_count, stream);
