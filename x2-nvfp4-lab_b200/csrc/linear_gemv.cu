@@ -21,9 +21,11 @@
 //
 // Bound by the weight stream (9/16 byte a weight) and, on B200, nearly as
 // much by the decode (80 weights per cycle and SM with nothing else to do; HBM
-// brings 41). Two batches of loads are in flight per warp. K is split over the
-// warps of a CTA when there are too few row tiles to give every warp its own;
-// their sums meet in shared memory in warp order.
+// brings 41). Two batches of loads are in flight per warp, two CTAs on an SM: 73%
+// of the copy bandwidth at 248,320 x 2,048 weights (60.4 us; three batches were no
+// faster, nor were asynchronous copies of the weights into shared memory). K is
+// split over the warps of a CTA when there are too few row tiles to give every
+// warp its own; their sums meet in shared memory in warp order.
 #include "linear_fused.cuh"
 #include "tma_util.cuh"
 
@@ -519,10 +521,12 @@ int staged_rows(const FusedLinearArgs &f) {
 
 }  // namespace
 
-// One group of eight MMA columns: eight rows of x, four of FP32 (high and low halves). Measured at 2048 x 16384 weights:
-// 8 rows 15.0 us, 12 rows 19.7 us, against 14.4 us for the tensor-memory kernel at any count up to 64; at 2048 x 2048
-// 9.0 and 11.6 against 13.3 us. Groups of rows whose counts are on the device go by their average: 256 groups of 1024
-// rows run 76 us at three rows a group and 100 us at four, against 113 us; 32 groups 27 and 33 us against 21 us.
+// One group of eight MMA columns: eight rows of x, four of FP32 (high and low halves). Measured against the
+// tensor-memory kernel: at 16,384 x 2,048 weights 2 rows 9.1 against 11.9 us, 4 rows 10.2, 8 rows 12.8 against 11.9; at
+// 65,536 x 2,048 8 rows 23.5 against 29.6; at 2,048 x 2,048 8 rows 8.7 against 11.0 and 4 FP32 rows 7.0 against 20.6
+// (more rows than a pass take two passes here, none there up to 64). Groups of rows whose counts are on the device go by
+// their average: over 256 groups of 1,024 x 2,048 weights three rows a group 69 against 96 us, four 99 against 97; over
+// 32 groups one row 16.4 against 18.8 us, three 22.1 against 18.9; of 2,048 x 512 over 256 groups three 46 against 72.
 bool linear_gemv_serves(const FusedLinearArgs &f) {
     const int per_row = f.type == NVFP4_TYPE_F32 ? 2 : 1;
     return staged_rows(f) >= 1 && (f.offsets ? (long long)f.vectors * per_row <= 3LL * f.groups : f.vectors * per_row <= 8);
