@@ -450,7 +450,8 @@ NVFP4_API nvfp4_status nvfp4_linear_grouped(
  *   offsets  int32 [experts + 1]: each expert's first row, then the number of
  *            rows in use
  * topk <= 64, experts <= 1024, tokens * topk below 2^31 - 16384. Enqueued on
- * `stream` (NULL: the runtime's stream); needs no workspace. */
+ * `stream` (NULL: the runtime's stream); needs no workspace. Outputs share no
+ * memory with x, ids or one another. */
 NVFP4_API nvfp4_status nvfp4_expert_sort(
     nvfp4_runtime * runtime,
     const void * x,
@@ -496,7 +497,8 @@ NVFP4_API nvfp4_status nvfp4_expert_return(
  * weights[t, k] * dout[t] (contiguous [tokens * topk, hidden], zeros from row
  * offsets[experts] on) and dweights[t, k] = <dout[t], rows[inverse[t, k]]>
  * (weights_type, 0 for a dropped pick). Either output may be NULL (rows is
- * only read for dweights, offsets for drows). */
+ * only read for dweights, offsets for drows) and shares no memory with the
+ * inputs. */
 NVFP4_API nvfp4_status nvfp4_expert_return_backward(
     nvfp4_runtime * runtime,
     const void * dout,

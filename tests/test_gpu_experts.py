@@ -308,6 +308,11 @@ def test_refusals(cuda_runtime):
     (d,) = torch.autograd.grad(r, y, torch.ones_like(r).requires_grad_(), create_graph=True)
     with pytest.raises(RuntimeError):
         d.sum().backward()
+    y = rows.clone().requires_grad_()
+    r = rt.expert_return(y, order, w)
+    (d,) = torch.autograd.grad(r, y, torch.ones_like(r).requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError):
+        d.sum().backward()
 
 
 @pytest.mark.parametrize("tokens", [1, 5, 64, 300])

@@ -190,6 +190,16 @@ def test_groups(cuda_runtime, kind, offsets):
     m.close()
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("offsets", [[0, 2], [0, 4], [1, 10], [0, 0, 17], [0, 31, 33], [3, 3, 3, 70]])
+def test_few_groups_of_few_rows(cuda_runtime, kind, offsets):
+    """Fewer rows than a tile of the many-row kernel loads, and ranges that end off its tiles."""
+    m, packed, scales, divisors = _matrix(cuda_runtime, len(offsets) - 1, 72, 208, 31)
+    x = _normal(32, offsets[-1] + 1, 208, dtype=TYPES[kind])
+    _check_grouped(cuda_runtime, m, packed, scales, divisors, x, offsets, activation="silu_mul")
+    m.close()
+
+
 @pytest.mark.parametrize("groups,most", [(1, 50), (37, 9), (300, 3), (1024, 2), (16, 200)])
 def test_many_groups_of_uneven_sizes(cuda_runtime, groups, most):
     rows, cols = 80, 64
@@ -343,5 +353,13 @@ def test_refusals(cuda_runtime):
                               np.ones(2, np.float32))
     with torch.no_grad():
         assert not rt.linear_fused(m, x.float().requires_grad_()).requires_grad
+    # At the C ABI: a workspace that is missing, too small or off its alignment, before anything is enqueued.
+    y = torch.empty(40, 65, device="cuda")
+    v = _normal(24, 40, 64)
+    size = rt.lib.nvfp4_linear_workspace_bytes(m.handle, v.data_ptr(), 2, 64, 40, 0)
+    space = torch.empty(size + 256, dtype=torch.uint8, device="cuda")
+    for at, given in ((None, size), (space.data_ptr(), size - 1), (space.data_ptr() + 16, size)):
+        assert rt.lib.nvfp4_linear_fused(rt.handle, m.handle, v.data_ptr(), 2, 64, 40, None, 0, 0, None, 0, y.data_ptr(),
+                                         65, at, given, None) == 1
     m.close()
     g.close()

@@ -84,8 +84,9 @@ const char *fused_args(FusedLinearArgs &a, const nvfp4_runtime *runtime, const n
 nvfp4_status run_fused(nvfp4_runtime *runtime, const nvfp4_matrix *matrix, const FusedLinearArgs &a, void *workspace,
                        size_t workspace_bytes, void *stream, const char *operation) {
     const bool few = linear_gemv_serves(a);
-    if (!few && workspace_bytes < linear_gemm_workspace(a.type, a.x, a.x_stride, a.vectors, a.cols))
-        return fail_invalid("the linear's workspace is too small (nvfp4_linear_workspace_bytes)");
+    const size_t needed = few ? 0 : linear_gemm_workspace(a.type, a.x, a.x_stride, a.vectors, a.cols);
+    if (needed && (!workspace || workspace_bytes < needed))
+        return fail_invalid("the linear's workspace is missing or too small (nvfp4_linear_workspace_bytes)");
     if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail_invalid("the linear's workspace must be 256-byte aligned");
     try {
         const device_scope scope(runtime);
