@@ -150,25 +150,30 @@ struct Tile {
 // Tile sizes of a group of `count` rows: as many tiles as needed, even, a multiple of 16 rows each.
 __device__ __forceinline__ int x_tiles(int count, int max_n) { return (count + max_n - 1) / max_n; }
 
-// `upto` [groups + 1]: x tiles of the groups before; after it each group's first row and number of rows.
-__device__ __forceinline__ Tile tile_of(const GemmArgs &a, const int *upto, int item) {
-    // The group with upto[g] * m_pairs <= item < upto[g + 1] * m_pairs.
+// `upto` [groups + 1]: x tiles of the groups before; after it each group's first row and number of rows. `group`: one at
+// or before the item's, left at the item's: a warp's items only go forward, and its lanes look at 32 groups at once.
+__device__ __forceinline__ Tile tile_of(const GemmArgs &a, const int *upto, int item, int &group) {
     Tile t;
-    const int at = item / a.m_pairs;
-    int lo = 0, hi = a.f.offsets ? a.f.groups : 1;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (upto[mid] <= at) lo = mid;
-        else hi = mid;
+    const int at = item / a.m_pairs, groups = a.f.offsets ? a.f.groups : 1;
+    // The last group with upto[g] <= at: as many steps on as following groups begin at or before it.
+    if (groups > 1) {
+        for (unsigned on = ~0u; on == ~0u;) {
+            const int g = group + 1 + (int)(threadIdx.x & 31);
+            on = __ballot_sync(0xffffffffu, g < groups && upto[min(g, groups)] <= at);
+            group += __popc(on);
+        }
     }
-    t.group = lo;
-    const int groups = a.f.offsets ? a.f.groups : 1;
-    const int first = upto[groups + 1 + lo], count = upto[2 * groups + 1 + lo];
-    const int tiles = upto[lo + 1] - upto[lo];
-    const int in_group = item - upto[lo] * a.m_pairs;
-    t.m = 2 * (in_group / tiles) + (int)cluster_rank();
-    const int width = ((count + tiles - 1) / tiles + 15) & ~15;
-    const int v = in_group % tiles * width;
+    t.group = group;
+    const int first = upto[groups + 1 + group], count = upto[2 * groups + 1 + group];
+    const int before = upto[group], tiles = upto[group + 1] - before;
+    const int in_group = item - before * a.m_pairs;
+    int m = in_group, v = 0, width = (count + 15) & ~15;
+    if (tiles > 1) {
+        m = in_group / tiles;
+        width = ((count + tiles - 1) / tiles + 15) & ~15;
+        v = (in_group - m * tiles) * width;
+    }
+    t.m = 2 * m + (int)cluster_rank();
     t.row0 = first + v;
     t.n = min(width, count - v);
     return t;
@@ -385,9 +390,10 @@ __global__ void __launch_bounds__(kGmThreads, 1)
     if (warp == 0) {
         // ----------------------------------------------- producer of x
         uint32_t it = 0;
+        int group = 0;
         bool ok = true;
         for (int item = pair; item < items && ok; item += pairs) {
-            const Tile t = tile_of(a, upto, item);
+            const Tile t = tile_of(a, upto, item, group);
             // The pair splits the tile's rows: this CTA's are the first or the second half of N.
             const int half = ((t.n + 15) & ~15) / 2, row0 = t.row0 + (int)rank * half;
             for (int ks = 0; ks < a.k_steps; ++ks, ++it) {
@@ -417,9 +423,10 @@ __global__ void __launch_bounds__(kGmThreads, 1)
     } else if (warp == 2) {
         // ----------------------------------------- producer of weights
         uint32_t rt = 0;
+        int group = 0;
         bool ok = true;
         for (int item = pair; item < items && ok; item += pairs) {
-            const Tile t = tile_of(a, upto, item);
+            const Tile t = tile_of(a, upto, item, group);
             const int w0 = t.group * f.rows + t.m * (f.gated ? 64 : 128), w1 = w0 + (f.gated ? f.out_rows : 64);
             for (int rs = 0; rs < a.raw_steps; ++rs, ++rt) {
                 const int st = rt % R;
@@ -467,8 +474,9 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                 }
             }
         } else {
+            int group = 0;
             for (int item = pair; item < last && ok; item += pairs) {
-                const uint32_t n = __reduce_max_sync(0xffffffffu, tile_of(a, upto, item).n);
+                const uint32_t n = __reduce_max_sync(0xffffffffu, tile_of(a, upto, item, group).n);
                 const uint32_t idesc = tc::idesc_16bit_pair((n + 15) & ~15u, kBf16 ? 1u : 0u);
                 for (int left = a.k_steps; left > 0 && ok; left -= a.segment, ++use) {
                     const uint32_t buf = use & 1, acc = tmem + buf * N;
@@ -610,12 +618,13 @@ __global__ void __launch_bounds__(kGmThreads, 1)
             }
         };
         bool ok = true;
+        int group = 0;
         for (int item = pair; item < items && ok; item += pairs) {
             if (whole && (use & 1) != piece) {
                 ++use;
                 continue;
             }
-            const Tile t = tile_of(a, upto, item);
+            const Tile t = tile_of(a, upto, item, group);
             Finish to{t.m * tile_rows + own, t.row0, t.n, f.inv_globals ? __ldg(f.inv_globals + t.group) : f.inv_global, 0.0f};
             if (f.bias && to.out0 < f.out_rows)
                 to.bias = load_as_f32(f.bias, f.bias_type,
