@@ -21,8 +21,8 @@
 //
 // Bound by the weight stream (9/16 byte a weight) and, on B200, nearly as
 // much by the decode (80 weights per cycle and SM with nothing else to do; HBM
-// brings 41). Two batches of loads are in flight per warp, two CTAs on an SM: 73%
-// of the copy bandwidth at 248,320 x 2,048 weights (60.4 us; three batches were no
+// brings 41). Two batches of loads are in flight per warp, two CTAs on an SM: 81%
+// of the copy bandwidth at 248,320 x 2,048 weights (53.9 us; three batches were no
 // faster, nor were asynchronous copies of the weights into shared memory). K is
 // split over the warps of a CTA when there are too few row tiles to give every
 // warp its own; their sums meet in shared memory in warp order.
@@ -57,8 +57,10 @@ struct Batch {
     uint32_t s[2];
 };
 
+// With the line after it into L2: the warp's next chunk (248,320 x 2,048 weights 53.9 us, 60.6 without; L2 prefetches of
+// whole tiles or of the first ones behind the staging of x were slower than that).
 __device__ __forceinline__ void load_codes(const uint8_t *p, uint32_t (&q)[8]) {
-    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7])
                  : "l"(p));
 }
@@ -548,10 +550,6 @@ void launch_linear_gemv(const FusedLinearArgs &f, int device, int sm_count, cuda
     const long long tiles = (long long)a.tiles * (f.offsets ? std::min(f.groups, f.vectors) : 1);
     a.warps_k = 1;
     while (a.warps_k < kGvWarps && 2 * a.warps_k <= a.chunks && tiles * a.warps_k < (long long)sm_count * 8) a.warps_k *= 2;
-    // Groups make a CTA's run of tiles end in the middle of its teams' turn, twice where it crosses into the next group:
-    // two warps a tile of 2,048 columns or more as long as every team has several (256 rows over 256 groups of 1,024 x
-    // 2,048 50.9 against 54.1 us; with one tile a team 16.2 against 12.1, at 512 columns 35.4 against 31.4).
-    if (f.offsets && a.warps_k == 1 && a.chunks >= 8 && tiles > 2LL * sm_count * kGvWarps) a.warps_k = 2;
     if (f.type == NVFP4_TYPE_BF16) launch<NVFP4_TYPE_BF16>(a, device, sm_count, stream);
     else if (f.type == NVFP4_TYPE_F16) launch<NVFP4_TYPE_F16>(a, device, sm_count, stream);
     else launch<NVFP4_TYPE_F32>(a, device, sm_count, stream);
