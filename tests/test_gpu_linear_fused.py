@@ -200,6 +200,27 @@ def test_few_groups_of_few_rows(cuda_runtime, kind, offsets):
     m.close()
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("offsets", [[0, 1, 2, 3, 4, 5, 6], [2, 2, 8, 9, 9, 14, 15], [0, 8, 16, 16, 17, 18, 18],
+                                     [0, 3, 2, 5, 4, 9, 9], [0, 9, 10, 11, 11, 11, 12], [0, 0, 0, 0, 0, 0, 16]])
+def test_rows_of_several_groups_staged_together(cuda_runtime, kind, offsets):
+    """Few rows over groups of few weight rows: a block's tiles cross groups that are empty, full or too large to share
+    its stage. Offsets that decrease give some row to two groups, and the rows of neither are compared."""
+    m, packed, scales, divisors = _matrix(cuda_runtime, 6, 40, 272, 33)
+    x = _normal(34, 18, 272, dtype=TYPES[kind])
+    if all(a <= b for a, b in zip(offsets, offsets[1:])):
+        bias = _normal(35, 6, 40, dtype=TYPES[kind])
+        _check_grouped(cuda_runtime, m, packed, scales, divisors, x, offsets, bias=bias, activation="relu")
+    else:
+        y = cuda_runtime.linear_grouped(m, x, torch.tensor(offsets, dtype=torch.int32, device="cuda"))
+        owners = [[g for g in range(6) if offsets[g] <= v < offsets[g + 1]] for v in range(18)]
+        for v, own in enumerate(owners):
+            if len(own) == 1:
+                want, tol = ref.linear(x[v:v + 1], packed[own[0]], scales[own[0]], divisors[own[0]])
+                ref.check(y[v:v + 1], want, tol, v)
+    m.close()
+
+
 @pytest.mark.parametrize("groups,most", [(1, 50), (37, 9), (300, 3), (1024, 2), (16, 200)])
 def test_many_groups_of_uneven_sizes(cuda_runtime, groups, most):
     rows, cols = 80, 64

@@ -37,6 +37,7 @@ namespace {
 constexpr int kGvThreads = 256;
 constexpr int kGvWarps = kGvThreads / 32;
 constexpr int kGvCols = 8;                          // columns of an MMA: rows of x, or halves of FP32 rows
+constexpr int kGvStaged = 16;                      // most rows of x staged at a time
 constexpr int kGvRedPitch = 20;                    // floats per column of a partial tile: conflict-free stores
 constexpr size_t kGvSmem = 232384;                 // dynamic shared memory of a CTA (64 bytes are static)
 constexpr size_t kGvSmemSm = 233472;               // and of an SM, of which every CTA takes 1 KB more
@@ -46,8 +47,8 @@ struct GemvArgs {
     int chunks;       // 256-column chunks
     int tiles;        // 16-row weight tiles of a group (eight outputs each with a gate)
     int warps_k;      // warps that share a tile's columns (a power of two)
-    int pass_rows;    // rows of x staged at a time
-    int pass_cols;    // their MMA columns (two per row for FP32)
+    int pass_rows;    // rows of a group that the MMA columns hold
+    int seg_rows;     // rows of x staged at a time, of several groups: pass_rows or more
     int token_stride; // bytes of a staged column
 };
 
@@ -264,8 +265,10 @@ __device__ __forceinline__ void stage_rows_async(const GemvArgs &a, uint8_t *xs,
     __syncthreads();
 }
 
-template <int TYPE>
+template <int TYPE, bool GROUPED>
 __global__ void __launch_bounds__(kGvThreads, 2) linear_gemv_kernel(const __grid_constant__ GemvArgs a) {
+    constexpr int kPerRow = TYPE == NVFP4_TYPE_F32 ? 2 : 1;  // MMA columns
+    constexpr bool kSeveral = GROUPED && TYPE != NVFP4_TYPE_F32;  // rows of several groups staged together
     extern __shared__ __align__(16) uint8_t gv_smem[];
     const FusedLinearArgs &f = a.f;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -274,15 +277,16 @@ __global__ void __launch_bounds__(kGvThreads, 2) linear_gemv_kernel(const __grid
     const int kw = warp & (warps_k - 1), wr = warp / warps_k;
 
     uint8_t *xs = gv_smem;
-    float *red = reinterpret_cast<float *>(gv_smem + (size_t)a.pass_cols * a.token_stride);  // [2][warps][kGvCols][pitch]
+    float *red = reinterpret_cast<float *>(gv_smem + (size_t)a.seg_rows * kPerRow * a.token_stride);  // [2][warps][kGvCols][pitch]
     uint32_t *amax = reinterpret_cast<uint32_t *>(red + 2 * kGvWarps * kGvCols * kGvRedPitch);
-    float *back = reinterpret_cast<float *>(amax + kGvCols);
-    int *active = reinterpret_cast<int *>(back + kGvCols);  // [groups] groups with rows (grouped calls)
+    float *back = reinterpret_cast<float *>(amax + kGvStaged);
+    int *active = reinterpret_cast<int *>(back + kGvStaged);  // [3][groups] groups with rows, their first row and count
+    int *active_first = active + f.groups, *active_count = active_first + f.groups;
     __shared__ int warp_sum[kGvWarps];
     __shared__ int s_active;
 
     int n_active = 1;
-    if (f.offsets) {
+    if constexpr (GROUPED) {
         // Compact list of the groups that have rows.
         const int per = (f.groups + kGvThreads - 1) / kGvThreads;
         const int g0 = min((int)threadIdx.x * per, f.groups), g1 = min(g0 + per, f.groups);
@@ -305,7 +309,7 @@ __global__ void __launch_bounds__(kGvThreads, 2) linear_gemv_kernel(const __grid
         for (int i = g0; i < g1; ++i) {
             int first, count;
             group_range(f, i, &first, &count);
-            if (count > 0) active[at++] = i;
+            if (count > 0) active[at] = i, active_first[at] = first, active_count[at++] = count;
         }
         if (threadIdx.x == kGvThreads - 1) s_active = at;
         __syncthreads();
@@ -314,49 +318,65 @@ __global__ void __launch_bounds__(kGvThreads, 2) linear_gemv_kernel(const __grid
 
     // This CTA's row tiles: a run of (group, tile), taken in turn by its teams of warps_k warps.
     const long long work = (long long)n_active * a.tiles;
-    long long u = work * blockIdx.x / gridDim.x;
-    const long long u_end = work * (blockIdx.x + 1) / gridDim.x;
+    int u = (int)(work * blockIdx.x / gridDim.x);
+    const int u_end = (int)(work * (blockIdx.x + 1) / gridDim.x);
     const int batches = ((a.chunks - kw + warps_k - 1) / warps_k + 1) & ~1;  // of this warp; even: two buffers in turn
     int parity = 0;
 
+    // Place of a tile of the run: its group, the tile there, and the group's rows.
+    struct Place {
+        int group, tile, first, count;
+    };
+    auto place = [&](int unit) {
+        if constexpr (!GROUPED) return Place{0, unit, 0, f.vectors};
+        const int ai = unit / a.tiles;
+        return Place{active[ai], unit - ai * a.tiles, active_first[ai], active_count[ai]};
+    };
+
     while (u < u_end) {
-        const int ai = (int)(u / a.tiles);
-        const int tile0 = (int)(u - (long long)ai * a.tiles);
-        const int tile1 = (int)min((long long)a.tiles, tile0 + (u_end - u));
-        u += tile1 - tile0;
-        const int group = f.offsets ? active[ai] : 0;
-        int first, count;
-        group_range(f, group, &first, &count);
-        const uint8_t *packed = f.packed + (size_t)group * f.rows * f.packed_pitch;
-        const uint8_t *scales = f.scales + (size_t)group * f.rows * f.scale_pitch;
-        const float inv = f.inv_globals ? __ldg(f.inv_globals + group) : f.inv_global;
+        // A piece of the run whose rows of x are staged together: of one group, in several passes if it has more rows than
+        // the MMA columns hold, else of as many groups one after the other as fit, so that the teams' turn and the loads go on from
+        // group to group (256 rows over 256 groups of 1,024 x 2,048 weights 44.5 us, 48.5 a group at a time).
+        const Place start = place(u);
+        int end = min(u_end, u - start.tile + a.tiles), rows = start.count;
+        if (kSeveral && rows <= a.pass_rows) {
+            while (end < u_end) {
+                const Place p = place(end);
+                if (p.count > a.pass_rows || rows + p.count > a.seg_rows || p.first != start.first + rows) break;
+                rows += p.count;
+                end = min(u_end, end + a.tiles);
+            }
+        }
+        const bool several = kSeveral && rows > start.count;
+        const int limit = several ? rows : a.pass_rows;  // rows a pass
 
-        for (int v0 = 0; v0 < count; v0 += a.pass_rows) {
-            const int n = min(a.pass_rows, count - v0);
-            const int ncols = TYPE == NVFP4_TYPE_F32 ? 2 * n : n;
+        for (int v0 = 0; v0 < rows; v0 += limit) {
+            const int n = min(limit, rows - v0), row0 = start.first + v0;
 
-            // The loads run ahead of the arithmetic: (l_tile, l_batch) is the next batch to request.
+            // The loads run ahead of the arithmetic: (l_unit, l_batch) is the next batch to request.
             // A lane's chunks end with its row's pitch (zero scales follow the last column, whatever codes the padding
             // holds); past it the scales are set to zero and nothing is read.
-            int l_tile = tile0 + wr, l_batch = 0, l_chunk = kw;
+            int l_unit = u + wr, l_batch = 0, l_chunk = kw;
             const int lane_chunks = (f.packed_pitch - t * 32 + 127) / 128;
             const uint8_t *p0, *p1, *s0, *s1;
             auto set_rows = [&]() {
                 // Rows of this lane, clamped to the last (its sums are not stored).
+                l_batch = 0;
+                l_chunk = l_unit < end ? kw : a.chunks;
+                const Place p = place(min(l_unit, end - 1));
                 int r0, r1;
                 if (f.gated) {
-                    r0 = min(l_tile * 8 + g, f.out_rows - 1);
+                    r0 = min(p.tile * 8 + g, f.out_rows - 1);
                     r1 = r0 + f.out_rows;
                 } else {
-                    r0 = min(l_tile * 16 + g, f.rows - 1);
-                    r1 = min(l_tile * 16 + g + 8, f.rows - 1);
+                    r0 = min(p.tile * 16 + g, f.rows - 1);
+                    r1 = min(p.tile * 16 + g + 8, f.rows - 1);
                 }
-                p0 = packed + (size_t)r0 * f.packed_pitch + kw * 128 + t * 32;
-                p1 = packed + (size_t)r1 * f.packed_pitch + kw * 128 + t * 32;
-                s0 = scales + (size_t)r0 * f.scale_pitch + kw * 16 + t * 4;
-                s1 = scales + (size_t)r1 * f.scale_pitch + kw * 16 + t * 4;
-                l_batch = 0;
-                l_chunk = l_tile < tile1 ? kw : a.chunks;
+                const size_t g0 = (size_t)p.group * f.rows;
+                p0 = f.packed + (g0 + r0) * f.packed_pitch + kw * 128 + t * 32;
+                p1 = f.packed + (g0 + r1) * f.packed_pitch + kw * 128 + t * 32;
+                s0 = f.scales + (g0 + r0) * f.scale_pitch + kw * 16 + t * 4;
+                s1 = f.scales + (g0 + r1) * f.scale_pitch + kw * 16 + t * 4;
             };
             set_rows();
             auto load = [&](Batch &b) {
@@ -369,7 +389,7 @@ __global__ void __launch_bounds__(kGvThreads, 2) linear_gemv_kernel(const __grid
                     b.s[0] = b.s[1] = 0u;
                 }
                 if (++l_batch == batches) {
-                    l_tile += teams;
+                    l_unit += teams;
                     set_rows();
                 } else {
                     p0 += warps_k * 128;
@@ -389,19 +409,16 @@ __global__ void __launch_bounds__(kGvThreads, 2) linear_gemv_kernel(const __grid
             bool async = false;
             if constexpr (TYPE != NVFP4_TYPE_F32) async = n * a.chunks > kGvWarps;
             if constexpr (TYPE != NVFP4_TYPE_F32) {
-                if (async) stage_rows_async<TYPE>(a, xs, amax, back, first + v0, n);
+                if (async) stage_rows_async<TYPE>(a, xs, amax, back, row0, n);
             }
-            if (!async) stage_rows<TYPE>(a, xs, amax, back, first + v0, n);
-            // MMA columns past the staged ones repeat the last: their sums are not stored.
-            const uint8_t *bcol = xs + min(g, ncols - 1) * a.token_stride + t * 160;
-
+            if (!async) stage_rows<TYPE>(a, xs, amax, back, row0, n);
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 
             // One output from its sum (and its up sum with a gate).
-            auto output = [&](int row, int v, float z, float z_up) {
-                const float scale = inv * back[v];
+            auto output = [&](const Place &p, float inv, int col0, int row, int v, float z, float z_up) {
+                const float scale = inv * back[col0 + v];
                 z *= scale;
-                const size_t at = (size_t)group * f.rows + row;
+                const size_t at = (size_t)p.group * f.rows + row;
                 if (f.bias) z += load_as_f32(f.bias, f.bias_type, at);
                 z = activate(z, f.act);
                 if (f.gated) {
@@ -409,12 +426,13 @@ __global__ void __launch_bounds__(kGvThreads, 2) linear_gemv_kernel(const __grid
                     if (f.bias) z_up += load_as_f32(f.bias, f.bias_type, at + f.out_rows);
                     z *= z_up;
                 }
-                const long long vec = (long long)first + v0 + v;
+                const long long vec = (long long)row0 + col0 + v;
                 if (f.residual) z += load_as_f32(f.residual, f.type, (size_t)(vec * f.residual_stride + row));
                 store_from_f32(f.out, f.type, (size_t)(vec * f.out_stride + row), z);
             };
-            auto finish = [&](int tile) {
-                const int per_col = f.gated ? 8 : 16, row0 = tile * per_col;
+            auto finish = [&](const Place &p, int col0, int n) {
+                const int per_col = f.gated ? 8 : 16, r0 = p.tile * per_col;
+                const float inv = f.inv_globals ? __ldg(f.inv_globals + p.group) : f.inv_global;
                 if (warps_k == 1) {
                     // The lane has rows g and g + 8 of MMA columns 2 t and 2 t + 1.
 #pragma unroll
@@ -423,21 +441,21 @@ __global__ void __launch_bounds__(kGvThreads, 2) linear_gemv_kernel(const __grid
                         if (v >= n) continue;
                         const float z = TYPE == NVFP4_TYPE_F32 ? sum[0] + sum[1] : sum[b];
                         const float y = TYPE == NVFP4_TYPE_F32 ? sum[2] + sum[3] : sum[2 + b];
-                        if (row0 + g < f.out_rows) output(row0 + g, v, z, y);
-                        if (!f.gated && row0 + g + 8 < f.out_rows) output(row0 + g + 8, v, y, 0.0f);
+                        if (r0 + g < f.out_rows) output(p, inv, col0, r0 + g, v, z, y);
+                        if (!f.gated && r0 + g + 8 < f.out_rows) output(p, inv, col0, r0 + g + 8, v, y, 0.0f);
                     }
                 } else {
                     // Partial tiles meet in shared memory; the warps of a tile share its epilogue.
-                    float *p = red + ((size_t)parity * kGvWarps + warp) * kGvCols * kGvRedPitch + 2 * t * kGvRedPitch + g;
-                    p[0] = sum[0];
-                    p[kGvRedPitch] = sum[1];
-                    p[8] = sum[2];
-                    p[kGvRedPitch + 8] = sum[3];
+                    float *to = red + ((size_t)parity * kGvWarps + warp) * kGvCols * kGvRedPitch + 2 * t * kGvRedPitch + g;
+                    to[0] = sum[0];
+                    to[kGvRedPitch] = sum[1];
+                    to[8] = sum[2];
+                    to[kGvRedPitch + 8] = sum[3];
                     named_barrier(1 + wr, warps_k * 32);
                     const float *part = red + ((size_t)parity * kGvWarps + wr * warps_k) * kGvCols * kGvRedPitch;
                     for (int i = kw * 32 + lane; i < n * per_col; i += warps_k * 32) {
                         const int v = f.gated ? i >> 3 : i >> 4, r = i & (per_col - 1);
-                        if (row0 + r >= f.out_rows) continue;
+                        if (r0 + r >= f.out_rows) continue;
                         const int c0 = (TYPE == NVFP4_TYPE_F32 ? 2 * v : v) * kGvRedPitch + r;
                         float z = 0.0f, z_up = 0.0f;
                         for (int k = 0; k < warps_k; ++k) {
@@ -445,14 +463,14 @@ __global__ void __launch_bounds__(kGvThreads, 2) linear_gemv_kernel(const __grid
                             z += TYPE == NVFP4_TYPE_F32 ? q[0] + q[kGvRedPitch] : q[0];
                             if (f.gated) z_up += TYPE == NVFP4_TYPE_F32 ? q[8] + q[kGvRedPitch + 8] : q[8];
                         }
-                        output(row0 + r, v, z, z_up);
+                        output(p, inv, col0, r0 + r, v, z, z_up);
                     }
                     parity ^= 1;
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sum[i] = 0.0f;
             };
-            auto step = [&](const Batch &b, int c, float (&acc)[2][4], bool fresh) {
+            auto step = [&](const Batch &b, const uint8_t *bcol, int c, float (&acc)[2][4], bool fresh) {
                 const uint32_t f0[2] = {e4m3x2_to_f16x2((uint16_t)b.s[0]), e4m3x2_to_f16x2((uint16_t)(b.s[0] >> 16))};
                 const uint32_t f1[2] = {e4m3x2_to_f16x2((uint16_t)b.s[1]), e4m3x2_to_f16x2((uint16_t)(b.s[1] >> 16))};
 #pragma unroll
@@ -477,40 +495,53 @@ __global__ void __launch_bounds__(kGvThreads, 2) linear_gemv_kernel(const __grid
                     }
                 }
             };
-            for (int tile = tile0 + wr; tile < tile1; tile += teams) {
+            for (int unit = u + wr; unit < end; unit += teams) {
+                const Place p = place(unit);
+                const int col0 = several ? p.first - start.first : 0;
+                const int here = several ? p.count : n;
+                // MMA columns past the group's repeat the last: their sums are not stored.
+                const uint8_t *bcol = xs + (col0 * kPerRow + min(g, here * kPerRow - 1)) * a.token_stride + t * 160;
                 for (int c = kw; c < a.chunks; c += 2 * warps_k) {
                     float acc[2][4];  // two chains
-                    step(b0, c, acc, true);
+                    step(b0, bcol, c, acc, true);
                     load(b0);
-                    if (c + warps_k < a.chunks) step(b1, c + warps_k, acc, false);
+                    if (c + warps_k < a.chunks) step(b1, bcol, c + warps_k, acc, false);
                     load(b1);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) sum[i] += acc[0][i] + acc[1][i];
                 }
-                finish(tile);
+                finish(p, col0, here);
             }
         }
+        u = end;
     }
     zero_other_rows(f);
 }
 
 // Shared memory besides the staged rows: partial tiles, scales, the list of groups.
 size_t other_smem(const FusedLinearArgs &f) {
-    return sizeof(float) * 2 * kGvWarps * kGvCols * kGvRedPitch + 8 * kGvCols + (f.offsets ? sizeof(int) * f.groups : 0);
+    return sizeof(float) * 2 * kGvWarps * kGvCols * kGvRedPitch + 8 * kGvStaged +
+           (f.offsets ? 3 * sizeof(int) * f.groups : 0);
 }
 
-template <int TYPE>
+template <int TYPE, bool GROUPED>
 void launch(GemvArgs &a, int device, int sm_count, cudaStream_t stream) {
-    const size_t smem = (size_t)a.pass_cols * a.token_stride + other_smem(a.f);
+    const size_t smem = (size_t)a.seg_rows * (TYPE == NVFP4_TYPE_F32 ? 2 : 1) * a.token_stride + other_smem(a.f);
     static std::atomic<uint64_t> done{0};
-    allow_shared_memory(linear_gemv_kernel<TYPE>, kGvSmem, done, device, "cudaFuncSetAttribute(linear_gemv_kernel)");
+    allow_shared_memory(linear_gemv_kernel<TYPE, GROUPED>, kGvSmem, done, device, "cudaFuncSetAttribute(linear_gemv_kernel)");
     // Two CTAs on an SM (the kernel's registers) where their shared memory fits.
     const int per_sm = 2 * (smem + 1024) <= kGvSmemSm ? 2 : 1;
     const long long teams = kGvWarps / a.warps_k;
     const long long work = ((long long)a.tiles * (a.f.offsets ? std::min(a.f.groups, a.f.vectors) : 1) + teams - 1) / teams;
     const long long grid = std::min(work, (long long)sm_count * per_sm);
-    linear_gemv_kernel<TYPE><<<static_cast<int>(std::max<long long>(1, grid)), kGvThreads, smem, stream>>>(a);
+    linear_gemv_kernel<TYPE, GROUPED><<<static_cast<int>(std::max<long long>(1, grid)), kGvThreads, smem, stream>>>(a);
     check_cuda(cudaGetLastError(), "linear_gemv_kernel");
+}
+
+template <int TYPE>
+void launch_type(GemvArgs &a, int device, int sm_count, cudaStream_t stream) {
+    if (a.f.offsets) launch<TYPE, true>(a, device, sm_count, stream);
+    else launch<TYPE, false>(a, device, sm_count, stream);
 }
 
 // Shared memory of a staged MMA column.
@@ -544,15 +575,22 @@ void launch_linear_gemv(const FusedLinearArgs &f, int device, int sm_count, cuda
     // Groups may have more rows than their average: further rows in further passes. (MMA columns for 16 rows made every
     // pass slower: a batch of 32 tokens over 256 groups 91 against 54 us.)
     a.pass_rows = std::max(1, std::min({8 / per_row, staged_rows(f), f.vectors}));
-    a.pass_cols = a.pass_rows * per_row;
+    a.seg_rows = a.pass_rows;
+    // Rows of several groups staged together: 16 of up to 2,048 columns, and of more as many as that much shared memory
+    // holds. More of it leaves the L1 too little for the scales, of which a load uses half a sector (with 24 rows 512 rows
+    // over 256 groups of 1,024 x 2,048 weights took 70.9 us, with 16 60.1); FP32 gains nothing (66 us, 62.2 a group at a
+    // time: 256 rows over 256 groups).
+    a.seg_rows = a.pass_rows;
+    if (f.offsets && f.type != NVFP4_TYPE_F32)
+        a.seg_rows = std::max(a.pass_rows, std::min({kGvStaged, f.vectors, kGvStaged * column_bytes(2048) / a.token_stride}));
     // As few warps share a tile as leave every SM eight teams at work (half of its warps): 16,384 x 2,048 weights take
     // 8.0 us with two warps a tile and 10.2 with eight, whose barriers cost more than their even shares bring.
     const long long tiles = (long long)a.tiles * (f.offsets ? std::min(f.groups, f.vectors) : 1);
     a.warps_k = 1;
     while (a.warps_k < kGvWarps && 2 * a.warps_k <= a.chunks && tiles * a.warps_k < (long long)sm_count * 8) a.warps_k *= 2;
-    if (f.type == NVFP4_TYPE_BF16) launch<NVFP4_TYPE_BF16>(a, device, sm_count, stream);
-    else if (f.type == NVFP4_TYPE_F16) launch<NVFP4_TYPE_F16>(a, device, sm_count, stream);
-    else launch<NVFP4_TYPE_F32>(a, device, sm_count, stream);
+    if (f.type == NVFP4_TYPE_BF16) launch_type<NVFP4_TYPE_BF16>(a, device, sm_count, stream);
+    else if (f.type == NVFP4_TYPE_F16) launch_type<NVFP4_TYPE_F16>(a, device, sm_count, stream);
+    else launch_type<NVFP4_TYPE_F32>(a, device, sm_count, stream);
 }
 
 }  // namespace nvfp4
