@@ -554,15 +554,15 @@ int staged_rows(const FusedLinearArgs &f) {
 
 }  // namespace
 
-// One group of eight MMA columns: eight rows of x, four of FP32 (high and low halves). Measured against the
-// tensor-memory kernel: at 16,384 x 2,048 weights 2 rows 9.1 against 11.9 us, 4 rows 10.2, 8 rows 12.8 against 11.9; at
-// 65,536 x 2,048 8 rows 23.5 against 29.6; at 2,048 x 2,048 8 rows 8.7 against 11.0 and 4 FP32 rows 7.0 against 20.6
-// (more rows than a pass take two passes here, none there up to 64). Groups of rows whose counts are on the device go by
-// their average: over 256 groups of 1,024 x 2,048 weights three rows a group 69 against 96 us, four 99 against 97; over
-// 32 groups one row 16.4 against 18.8 us, three 22.1 against 18.9; of 2,048 x 512 over 256 groups three 46 against 72.
+// Eight rows: one pass of the MMA columns, of FP32 two passes of four rows (high and low halves). Measured against the
+// tensor-memory kernel at 16,384 x 2,048 weights: 2 BF16 rows 8.9 against 12.1 us, 4 rows 10.2, 8 rows 12.9 against 12.1,
+// 12 rows 20.7; 8 FP32 rows 18.7 against 22.1, 12 rows 26.7; at 65,536 x 2,048 8 BF16 rows 23.4 against 29.5, at 2,048 x
+// 2,048 8.5 against 11.2 and 8 FP32 rows 11.2 against 21.3. Groups of rows whose counts are on the device go by their
+// average: over 256 groups of 1,024 x 2,048 weights three BF16 rows a group 63 against 92 us, four 94 against 93, six FP32
+// rows 179 against 206; over 32 groups three BF16 rows 17.6 against 18.8, four 22.1, four FP32 rows 30.6 against 37.6.
 bool linear_gemv_serves(const FusedLinearArgs &f) {
-    const int per_row = f.type == NVFP4_TYPE_F32 ? 2 : 1;
-    return staged_rows(f) >= 1 && (f.offsets ? (long long)f.vectors * per_row <= 3LL * f.groups : f.vectors * per_row <= 8);
+    return staged_rows(f) >= 1 &&
+           (f.offsets ? f.vectors <= (f.type == NVFP4_TYPE_F32 ? 6LL : 3LL) * f.groups : f.vectors <= kGvCols);
 }
 
 void launch_linear_gemv(const FusedLinearArgs &f, int device, int sm_count, cudaStream_t stream) {
