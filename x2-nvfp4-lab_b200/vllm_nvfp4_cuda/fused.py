@@ -53,11 +53,12 @@ def _check(matrix, x, bias, activation, others):
     return matrix.rows // 2
 
 
-def _workspace(rt, matrix, x, grouped):
+def _workspace(rt, matrix, x, at, stride, grouped):
     """(tensor, address, bytes) of the call's device workspace, from torch's allocator on the current stream. The
     tensor is held until the kernels are enqueued; its memory then goes to later work of the same stream."""
-    size = rt.lib.nvfp4_linear_workspace_bytes(matrix.handle, x.data_ptr(), TYPES[x.dtype], _row_stride(x), x.shape[0],
-                                               grouped)
+    if at % 16 == 0 and stride % 8 == 0 and stride >= matrix.cols and x.dtype != torch.float32:
+        return None, None, 0  # rows that every kernel reads where they lie
+    size = rt.lib.nvfp4_linear_workspace_bytes(matrix.handle, at, TYPES[x.dtype], stride, x.shape[0], grouped)
     if not size:
         return None, None, 0
     held = torch.empty(size, dtype=torch.uint8, device=x.device)
@@ -96,10 +97,11 @@ def _linear(rt, matrix, x, bias, activation, residual, out, width, shape):
         r2 = _rows2d(residual, width)
         r_at, r_stride = r2.data_ptr(), _row_stride(r2)
     _held_bias, b_at, b_type = _bias(bias)
-    _held, space, size = _workspace(rt, matrix, x2, 0)
+    x_at, x_stride = x2.data_ptr(), _row_stride(x2)
+    _held, space, size = _workspace(rt, matrix, x2, x_at, x_stride, 0)
     rt._check(
-        rt.lib.nvfp4_linear_fused(rt.handle, matrix.handle, x2.data_ptr(), TYPES[x.dtype], _row_stride(x2), count, b_at,
-                                  b_type, ACTIVATIONS[activation], r_at, r_stride, y.data_ptr(), stride, space, size,
+        rt.lib.nvfp4_linear_fused(rt.handle, matrix.handle, x_at, TYPES[x.dtype], x_stride, count, b_at, b_type,
+                                  ACTIVATIONS[activation], r_at, r_stride, y.data_ptr(), stride, space, size,
                                   stream_of(x.device)),
         "nvfp4_linear_fused")
     return y
@@ -126,10 +128,11 @@ def _grouped(rt, matrix, x, offsets, bias, activation, out, shape):
         return y
     x2, o = _rows_of(x), offsets.contiguous()
     _held_bias, b_at, b_type = _bias(bias)
-    _held, space, size = _workspace(rt, matrix, x2, 1)
+    x_at, x_stride = x2.data_ptr(), _row_stride(x2)
+    _held, space, size = _workspace(rt, matrix, x2, x_at, x_stride, 1)
     rt._check(
-        rt.lib.nvfp4_linear_grouped(rt.handle, matrix.handle, x2.data_ptr(), TYPES[x.dtype], _row_stride(x2), count,
-                                    o.data_ptr(), b_at, b_type, ACTIVATIONS[activation], y.data_ptr(),
+        rt.lib.nvfp4_linear_grouped(rt.handle, matrix.handle, x_at, TYPES[x.dtype], x_stride, count, o.data_ptr(),
+                                    b_at, b_type, ACTIVATIONS[activation], y.data_ptr(),
                                     width if out is None else _row_stride(y), 1 if out is None else 0, space, size,
                                     stream_of(x.device)),
         "nvfp4_linear_grouped")
