@@ -37,8 +37,8 @@ namespace {
 constexpr int kGvThreads = 256;
 constexpr int kGvWarps = kGvThreads / 32;
 constexpr int kGvCols = 8;                          // columns of an MMA: rows of x, or halves of FP32 rows
-constexpr int kGvStaged = 16;                      // most rows of x staged at a time
-constexpr int kGvRedPitch = 20;                    // floats per column of a partial tile: conflict-free stores
+constexpr int kGvStaged = 16;                       // most rows of x staged at a time
+constexpr int kGvRedPitch = 20;                     // floats per column of a partial tile: conflict-free stores
 constexpr size_t kGvSmem = 232384;                 // dynamic shared memory of a CTA (64 bytes are static)
 constexpr size_t kGvSmemSm = 233472;               // and of an SM, of which every CTA takes 1 KB more
 
@@ -335,8 +335,8 @@ __global__ void __launch_bounds__(kGvThreads, 2) linear_gemv_kernel(const __grid
 
     while (u < u_end) {
         // A piece of the run whose rows of x are staged together: of one group, in several passes if it has more rows than
-        // the MMA columns hold, else of as many groups one after the other as fit, so that the teams' turn and the loads go on from
-        // group to group (256 rows over 256 groups of 1,024 x 2,048 weights 44.5 us, 48.5 a group at a time).
+        // the MMA columns hold, else of as many groups one after the other as fit, so that the teams' turn and the loads go
+        // on from group to group (256 rows over 256 groups of 1,024 x 2,048 weights 44.5 us, 48.5 a group at a time).
         const Place start = place(u);
         int end = min(u_end, u - start.tile + a.tiles), rows = start.count;
         if (kSeveral && rows <= a.pass_rows) {
