@@ -212,10 +212,11 @@ def test_rows_past_32_bit_offsets(cuda_runtime):
     assert torch.equal(out, x)
 
 
-def test_streams_and_graphs(cuda_runtime):
+@pytest.mark.parametrize("tokens", [300, 1500])  # a one-CTA sort, and a cluster's with a dependent launch
+def test_streams_and_graphs(cuda_runtime, tokens):
     """On another stream, and a forward and backward pass captured and replayed on new values."""
     rt = cuda_runtime
-    tokens, topk, experts, hidden = 300, 4, 32, 64
+    topk, experts, hidden = 4, 32, 64
 
     def step(x, ids, weights, g):
         rows, order = rt.expert_sort(x, ids, experts)
@@ -243,7 +244,8 @@ def test_streams_and_graphs(cuda_runtime):
     with torch.no_grad():
         for a, b in zip(first, second):
             a.copy_(b)
-    graph.replay()
+    for _ in range(3):
+        graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
