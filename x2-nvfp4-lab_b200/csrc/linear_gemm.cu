@@ -541,7 +541,8 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                 }
             }
         }
-        // Every MMA has completed before tensor memory is freed (the odd CTA waits for the even one below).
+        // Every MMA has completed before tensor memory is freed. The last commit arrives at the same place in both CTAs:
+        // each waits for its own arrival, the odd one after the cluster's barrier, by which it has been issued.
         if (rank == 0) {
             if (tc::elect_one()) tc::commit_pair(drain);
             __syncwarp();
@@ -690,6 +691,8 @@ __global__ void __launch_bounds__(kGmThreads, 1)
     __syncthreads();
     cluster_sync();  // neither CTA leaves while the other may reach its shared memory
     if (warp == 1) {
+        if (rank == 1) wait_drain(drain, 0);  // no arrival is on its way to this shared memory when the CTA ends
+        __syncwarp();
         tc::fence_after_sync();
         tc::tmem_dealloc_pair(tmem, 512);
     }
