@@ -451,7 +451,8 @@ NVFP4_API nvfp4_status nvfp4_linear_grouped(
  *            rows in use
  * topk <= 64, experts <= 1024, tokens * topk below 2^31 - 16384. Enqueued on
  * `stream` (NULL: the runtime's stream); needs no workspace. Outputs share no
- * memory with x, ids or one another. */
+ * memory with x, ids or one another. Every array here and in the two entry
+ * points below is aligned to its elements; others are refused. */
 NVFP4_API nvfp4_status nvfp4_expert_sort(
     nvfp4_runtime * runtime,
     const void * x,

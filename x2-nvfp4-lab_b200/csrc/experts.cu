@@ -514,6 +514,13 @@ int vector_bytes(std::initializer_list<unsigned long long> places) {
     return static_cast<int>(all & (~all + 1));  // lowest set bit, at most 16
 }
 unsigned long long place_of(const void *p) { return reinterpret_cast<uintptr_t>(p); }
+// Whether every address (NULL too) is a multiple of an element's bytes: a kernel that took another would fault.
+bool aligned_to(int bytes, std::initializer_list<const void *> addresses) {
+    for (const void *p : addresses)
+        if (place_of(p) % bytes != 0) return false;
+    return true;
+}
+constexpr const char *kMisaligned = "arrays of the expert sort and return must be aligned to their elements";
 
 // Threads that share a token: a power of two near its vectors, from 8 to a whole CTA.
 int group_of(int nvec) {
@@ -523,12 +530,10 @@ int group_of(int nvec) {
 }
 
 template <typename Args>
-void launch(void (*kernel)(Args), int grid, size_t smem, cudaStream_t stream, bool dependent, const Args &args,
-            const char *name) {
+void launch(void (*kernel)(Args), int grid, cudaStream_t stream, bool dependent, const Args &args, const char *name) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kExThreads);
-    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -542,7 +547,7 @@ template <int B>
 void launch_sort(SortArgs &a, int device, cudaStream_t s) {
     a.group = group_of(a.row_bytes / B);
     if (a.picks <= kExSmallPicks) {
-        launch(expert_sort_small_kernel<B>, a.tokens + 1, 0, s, false, a, "expert_sort_small_kernel");
+        launch(expert_sort_small_kernel<B>, a.tokens + 1, s, false, a, "expert_sort_small_kernel");
         return;
     }
     const size_t smem = sizeof(int) * (kRankWarps + 2) * (a.experts + 1);
@@ -562,33 +567,30 @@ void launch_sort(SortArgs &a, int device, cudaStream_t s) {
     cfg.numAttrs = 1;
     check_cuda(cudaLaunchKernelEx(&cfg, expert_rank_kernel, a), "expert_rank_kernel");
     const int per_cta = kExThreads / a.group;
-    launch(expert_copy_kernel<B>, (a.tokens + per_cta - 1) / per_cta, 0, s, true, a, "expert_copy_kernel");
+    launch(expert_copy_kernel<B>, (a.tokens + per_cta - 1) / per_cta, s, true, a, "expert_copy_kernel");
 }
 
 template <int TYPE, int B>
 void launch_return(ReturnArgs &a, bool backward, cudaStream_t s) {
-    if constexpr (B < (TYPE == kF32 ? 4 : 2)) {
-        throw invalid_argument_error("rows must be aligned to their elements");
-    } else {
-        a.group = group_of(a.row_bytes / B);
-        // The weights' gradient ends in a sum over the threads of a token: one warp a token, once
-        // tokens give every SM 16 of them and rows are no longer than 16 vectors a lane (4,096 tokens with eight BF16 rows
-        // of 2,048: 55 us, 59 us with a CTA a token).
-        if (backward && a.tokens >= 2368 && a.row_bytes / B <= 512) a.group = std::min(a.group, 32);
-        const int per_cta = kExThreads / a.group, grid = (a.tokens + per_cta - 1) / per_cta;
-        if (backward)
-            launch(expert_return_backward_kernel<TYPE, B>, grid, 0, s, false, a, "expert_return_backward_kernel");
-        else
-            launch(expert_return_kernel<TYPE, B>, grid, 0, s, false, a, "expert_return_kernel");
-    }
+    a.group = group_of(a.row_bytes / B);
+    // The weights' gradient ends in a sum over the threads of a token: one warp a token, once
+    // tokens give every SM 16 of them and rows are no longer than 16 vectors a lane (4,096 tokens with eight BF16 rows
+    // of 2,048: 55 us, 59 us with a CTA a token).
+    if (backward && a.tokens >= 2368 && a.row_bytes / B <= 512) a.group = std::min(a.group, 32);
+    const int per_cta = kExThreads / a.group, grid = (a.tokens + per_cta - 1) / per_cta;
+    if (backward)
+        launch(expert_return_backward_kernel<TYPE, B>, grid, s, false, a, "expert_return_backward_kernel");
+    else
+        launch(expert_return_kernel<TYPE, B>, grid, s, false, a, "expert_return_kernel");
 }
 
+// `vec` is an element at least: the entry points refuse addresses off their elements.
 template <int TYPE>
 void dispatch_return(ReturnArgs &a, int vec, bool backward, cudaStream_t s) {
     if (vec == 16) launch_return<TYPE, 16>(a, backward, s);
     else if (vec == 8) launch_return<TYPE, 8>(a, backward, s);
-    else if (vec == 4) launch_return<TYPE, 4>(a, backward, s);
-    else launch_return<TYPE, 2>(a, backward, s);
+    else if (TYPE == kF32 || vec == 4) launch_return<TYPE, 4>(a, backward, s);
+    else if constexpr (TYPE != kF32) launch_return<TYPE, 2>(a, backward, s);
 }
 
 void run_return(ReturnArgs &a, int type, int vec, bool backward, cudaStream_t s) {
@@ -615,6 +617,9 @@ extern "C" NVFP4_API nvfp4_status nvfp4_expert_sort(nvfp4_runtime *runtime, cons
         (ids_bytes != 4 && ids_bytes != 8) || ids_stride < 0 || x_stride < 0)
         return fail_invalid("invalid expert sort arguments");
     if (experts < 1 || experts > kExMaxExperts) return fail_invalid("the expert sort supports 1 to 1024 experts");
+    if (!aligned_to(type_bytes(type), {x, rows}) || !aligned_to(ids_bytes, {ids}) ||
+        !aligned_to(4, {perm, inverse, offsets}))
+        return fail_invalid(kMisaligned);
     try {
         const device_scope scope(runtime);
         check_on_device(runtime, {x, ids, rows}, "expert sort");
@@ -642,8 +647,7 @@ extern "C" NVFP4_API nvfp4_status nvfp4_expert_sort(nvfp4_runtime *runtime, cons
                 if (vec == 16) launch_sort<16>(a, runtime->device, s);
                 else if (vec == 8) launch_sort<8>(a, runtime->device, s);
                 else if (vec == 4) launch_sort<4>(a, runtime->device, s);
-                else if (vec == 2) launch_sort<2>(a, runtime->device, s);
-                else throw invalid_argument_error("expert sort: rows must be aligned to their elements");
+                else launch_sort<2>(a, runtime->device, s);
             });
         });
         clear_last_error();
@@ -661,6 +665,9 @@ extern "C" NVFP4_API nvfp4_status nvfp4_expert_return(nvfp4_runtime *runtime, co
     if (!runtime || !rows || !inverse || !out || !valid_sizes(type, tokens, topk, hidden) ||
         (weights && !valid_type(weights_type)) || rows_stride < 0 || residual_stride < 0 || out_stride < hidden)
         return fail_invalid("invalid expert return arguments");
+    if (!aligned_to(type_bytes(type), {rows, residual, out}) || !aligned_to(4, {inverse}) ||
+        (weights && !aligned_to(type_bytes(weights_type), {weights})))
+        return fail_invalid(kMisaligned);
     const long long row = static_cast<long long>(hidden) * type_bytes(type), picks = static_cast<long long>(tokens) * topk;
     const row_span to{out, tokens, row, out_stride * type_bytes(type)};
     if (spans_overlap({rows, picks, row, rows_stride * type_bytes(type)}, to))
@@ -710,6 +717,9 @@ extern "C" NVFP4_API nvfp4_status nvfp4_expert_return_backward(
         (dweights && !rows) || !valid_sizes(type, tokens, topk, hidden) ||
         ((weights || dweights) && !valid_type(weights_type)) || dout_stride < 0 || rows_stride < 0)
         return fail_invalid("invalid expert return gradient arguments");
+    if (!aligned_to(type_bytes(type), {dout, rows, drows}) || !aligned_to(4, {inverse, offsets}) ||
+        ((weights || dweights) && !aligned_to(type_bytes(weights_type), {weights, dweights})))
+        return fail_invalid(kMisaligned);
     try {
         const device_scope scope(runtime);
         check_on_device(runtime, {dout, drows ? drows : dweights}, "expert return gradient");
