@@ -473,6 +473,8 @@ NVFP4_API nvfp4_status nvfp4_expert_sort(
 
 /* additive: out[t] = residual[t] + sum_k weights[t, k] * rows[inverse[t, k]],
  * picks with inverse -1 left out, in FP32 and the order of k, rounded once.
+ * inverse as the sort wrote it, or with further picks set to -1 (a capacity
+ * limit); no two picks name the same row.
  * rows, residual and out are of `type` with row strides in elements; weights
  * [tokens, topk] (contiguous, a type of their own) may be NULL for ones (the
  * gradient of nvfp4_expert_sort to x), residual may be NULL, or out itself;
@@ -496,7 +498,8 @@ NVFP4_API nvfp4_status nvfp4_expert_return(
 
 /* additive: gradients of nvfp4_expert_return: drows[inverse[t, k]] =
  * weights[t, k] * dout[t] (contiguous [tokens * topk, hidden], zeros from row
- * offsets[experts] on) and dweights[t, k] = <dout[t], rows[inverse[t, k]]>
+ * offsets[experts] on and in rows below that no pick names) and
+ * dweights[t, k] = <dout[t], rows[inverse[t, k]]>
  * (weights_type, 0 for a dropped pick). Either output may be NULL (rows is
  * only read for dweights, offsets for drows) and shares no memory with the
  * inputs. */

@@ -37,3 +37,98 @@ def test_short_calls_one_after_the_other(cuda_runtime, kind):
         assert torch.equal(a, want_many) and torch.equal(b, want_few) and torch.equal(c, want_many)
     rt.synchronize()
     m.close()
+
+
+# ------------------------------------------------------------------ an order changed after the sort
+
+
+def _dropped(order, seed, share):
+    """The order with some picks dropped after the sort, by a capacity limit say."""
+    gen = torch.Generator().manual_seed(seed)
+    gone = (torch.rand(order.inverse.shape, generator=gen) < share).cuda()
+    return order._replace(inverse=torch.where(gone, -1, order.inverse))
+
+
+def _return_gradients(order, g, rows, weights):
+    """(drows, dweights) of the return by their formulas in 64 bits."""
+    inverse, has = order.inverse.long(), order.inverse >= 0
+    count = inverse.numel()
+    drows = torch.zeros(count + 1, g.shape[1], dtype=torch.float64, device="cuda")
+    drows[torch.where(has, inverse, count)] = weights.double()[..., None] * g.double()[:, None]
+    taken = rows.double()[inverse.clamp(min=0)] * has[..., None]
+    products = g.double()[:, None] * taken
+    return drows[:-1], products.sum(2), products.abs().sum(2)
+
+
+# The last one has more rows than one CTA marks at a time, the third fewer picks than threads.
+@pytest.mark.parametrize("share", [0.3, 1.0])
+@pytest.mark.parametrize("tokens,topk,experts,hidden", [(1, 1, 1, 8), (1, 8, 256, 40), (5, 3, 4, 33), (128, 8, 64, 96),
+                                                        (700, 6, 1024, 20), (3001, 8, 256, 24), (40000, 8, 16, 2)])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_gradients_of_picks_dropped_after_the_sort(cuda_runtime, kind, tokens, topk, experts, hidden, share):
+    """A pick set to -1 after the sort is left out of the sum, and its row has a gradient of zero: whatever the memory
+    of the gradient held, through autograd and at the C ABI, with every kind of output asked for."""
+    from vllm_nvfp4_cuda.experts import TYPES as CODES, stream_of
+
+    rt, dtype = cuda_runtime, TYPES[kind]
+    gen = torch.Generator().manual_seed(tokens)
+    ids = torch.randint(-1, experts, (tokens, topk), generator=gen, dtype=torch.int32).cuda()
+    rows, order = rt.expert_sort(_normal(81, tokens, hidden, dtype=dtype), ids, experts)
+    order = _dropped(order, 82, share)
+    weights, g = _normal(83, tokens, topk).requires_grad_(), _normal(84, tokens, hidden, dtype=dtype)
+    want, dw, dw_size = _return_gradients(order, g, rows, weights.detach())
+    half, unit, tiny = torch.finfo(dtype).eps / 2, 2.0 ** -24, torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    tol, dw_tol = (unit * (1 + half) + half) * want.abs() + tiny, hidden * unit * dw_size + 2 * unit * dw.abs()
+    rows = rows.requires_grad_()
+    out = rt.expert_return(rows, order, weights)
+    torch.full_like(rows, float("nan"))  # in the memory that the gradient gets next
+    drows, dweights = torch.autograd.grad(out, (rows, weights), g)
+    ref.check(drows, want, tol, "drows")
+    ref.check(dweights, dw, dw_tol, "dweights")
+    for with_weights in (True, False):
+        for with_dweights in (True, False):
+            drows, dweights = torch.full_like(g.new_empty(tokens * topk, hidden), float("nan")), torch.zeros_like(weights)
+            status = rt.lib.nvfp4_expert_return_backward(
+                rt.handle, g.data_ptr(), CODES[dtype], hidden, rows.data_ptr() if with_dweights else None, hidden,
+                order.inverse.data_ptr(), order.offsets.data_ptr(), weights.data_ptr() if with_weights else None, 2,
+                tokens, topk, hidden, experts, drows.data_ptr(), dweights.data_ptr() if with_dweights else None,
+                stream_of(g.device))
+            assert status == 0
+            if with_weights:
+                ref.check(drows, want, tol, "drows at the C ABI")
+            else:
+                named = want.abs().sum(1) > 0
+                assert not bool(drows[~named].any()) and bool(drows[named].isfinite().all())
+            if with_dweights:
+                ref.check(dweights, dw, dw_tol, "dweights at the C ABI")
+
+
+def test_captured_gradients_of_another_order(cuda_runtime):
+    """Both passes captured once and replayed on orders with other picks dropped, none and all among them."""
+    rt, tokens, topk, experts, hidden = cuda_runtime, 900, 6, 40, 72
+    gen = torch.Generator().manual_seed(5)
+    ids = torch.randint(0, experts, (tokens, topk), generator=gen, dtype=torch.int32).cuda()
+    rows, sorted_order = rt.expert_sort(_normal(85, tokens, hidden), ids, experts)
+    rows, weights = rows.requires_grad_(), _normal(86, tokens, topk).requires_grad_()
+    g = _normal(87, tokens, hidden)
+    order = sorted_order._replace(inverse=sorted_order.inverse.clone())
+
+    def step():
+        return torch.autograd.grad(rt.expert_return(rows, order, weights), (rows, weights), g)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        drows, dweights = step()
+    for share in (0.2, 0.0, 1.0, 0.01):
+        order.inverse.copy_(_dropped(sorted_order, 88, share).inverse)
+        want, dw, size = _return_gradients(order, g, rows.detach(), weights.detach())
+        drows.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        ref.check(drows, want, 2.0 ** -24 * want.abs(), share)
+        ref.check(dweights, dw, hidden * 2.0 ** -24 * size + 2.0 ** -23 * dw.abs(), share)

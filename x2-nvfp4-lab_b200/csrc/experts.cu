@@ -6,7 +6,8 @@
 //                                               row of expert e, offsets[E] = the number of rows in use
 //   its dx    dx[t]   = sum_k drows[inverse[t, k]]                          (the return with weights of one)
 //   return    out[t]  = residual[t] + sum_k w[t, k] * rows[inverse[t, k]]
-//   its dX    drows[inverse[t, k]] = w[t, k] * dout[t],  dw[t, k] = <dout[t], rows[inverse[t, k]]>
+//   its dX    drows[inverse[t, k]] = w[t, k] * dout[t],  dw[t, k] = <dout[t], rows[inverse[t, k]]>; zero in rows that
+//             no pick names (a pick may be set to -1 after the sort)
 //
 // Every kernel moves T*K rows of H values once and does next to nothing with them, so HBM bounds them. One group of
 // threads owns a token: the sort reads a token's row once and stores it K times, the return reads its K rows and
@@ -410,6 +411,64 @@ __global__ void __launch_bounds__(kExThreads) expert_return_kernel(ReturnArgs a)
     }
 }
 
+// Zeros to the rows of drows below offsets[experts] that no pick names: those of picks dropped after the sort. There are
+// none in an order as the sort made it, and then the kernel only counts: a cluster's CTAs a share of the picks each, their
+// counts added up through distributed shared memory, and the gradient kernel, launched behind it, waits for that before
+// its first store, with its loads under way (4,096 tokens with eight BF16 rows of 2,048: 54.1 us both, 54.6 without the
+// count and the loads ahead; 32 tokens 6.1 against 5.3). Else each CTA marks which of its own rows are named, a bit a row,
+// from the picks of all (61.8 us with a tenth of the picks dropped).
+constexpr int kUnnamedThreads = 512, kUnnamedCluster = 8;
+constexpr int kUnnamedWords = 8192;  // 262,144 rows marked at a time
+
+template <int B>
+__global__ void __launch_bounds__(kUnnamedThreads) expert_unnamed_rows_kernel(ReturnArgs a) {
+    using V = typename Vec<B>::type;
+    __shared__ uint32_t named[kUnnamedWords];
+    __shared__ int count;
+    pdl_launch_dependents();
+    const int picks = a.tokens * a.topk, rank = (int)cluster_rank();
+    const int used = min(max(__ldg(a.offsets + a.experts), 0), picks);
+    if (threadIdx.x == 0) count = 0;
+    __syncthreads();
+    int own = 0;
+#pragma unroll 4
+    for (long long i = rank * kUnnamedThreads + (int)threadIdx.x; i < picks; i += kUnnamedCluster * kUnnamedThreads)
+        own += (unsigned)__ldg(a.inverse + i) < (unsigned)used ? 1 : 0;
+    own = __reduce_add_sync(0xffffffffu, own);
+    if ((threadIdx.x & 31) == 0 && own != 0) atomicAdd(&count, own);
+    cluster_sync();
+    int all = 0;
+#pragma unroll
+    for (int r = 0; r < kUnnamedCluster; ++r) all += load_cluster(&count, r);
+    cluster_sync();  // no CTA leaves while another may read its count
+    if (all == used) return;
+    const long long first = (long long)used * blockIdx.x / gridDim.x, last = (long long)used * (blockIdx.x + 1) / gridDim.x;
+    const int nvec = a.row_bytes / B;
+    for (long long r0 = first; r0 < last; r0 += 32 * kUnnamedWords) {
+        const int n = (int)min(last - r0, 32LL * kUnnamedWords);
+        for (int i = threadIdx.x; i < (n + 31) / 32; i += kUnnamedThreads) named[i] = 0u;
+        __syncthreads();
+        for (long long i = threadIdx.x; i < picks; i += kExRows * kUnnamedThreads) {
+            unsigned at[kExRows];
+#pragma unroll
+            for (int u = 0; u < kExRows; ++u) {
+                const long long pick = i + u * kUnnamedThreads;
+                at[u] = (pick < picks ? (unsigned)__ldg(a.inverse + pick) : ~0u) - (unsigned)r0;
+            }
+#pragma unroll
+            for (int u = 0; u < kExRows; ++u)
+                if (at[u] < (unsigned)n) atomicOr(named + (at[u] >> 5), 1u << (at[u] & 31));
+        }
+        __syncthreads();
+        for (int r = threadIdx.x >> 5; r < n; r += kUnnamedThreads / 32) {
+            if ((named[r >> 5] >> (r & 31)) & 1u) continue;
+            V *to = reinterpret_cast<V *>(a.drows + (r0 + r) * a.row_bytes);
+            for (int v = threadIdx.x & 31; v < nvec; v += 32) to[v] = zero_vec<V>();
+        }
+        __syncthreads();
+    }
+}
+
 // The gradient keeps four rows' loads in flight per thread and four CTAs on an SM: with eight rows its 166 registers
 // left one CTA, and 4,096 tokens with eight BF16 rows of 2,048 took 136 us instead of 59.
 constexpr int kExBackRows = 4;
@@ -443,8 +502,10 @@ __global__ void __launch_bounds__(kExThreads, 4) expert_return_backward_kernel(R
                 for (int j = 0; j < kExBackRows; ++j)
                     if (p[j] >= 0) val[j] = reinterpret_cast<const V *>(a.rows + (long long)p[j] * a.rows_stride)[v];
             }
+            const V dv = dout[v];
+            pdl_wait();  // the zeros of rows that no pick names; what is read above depends on no launch of this call
             float g[L::kN];
-            L::unpack(dout[v], g);
+            L::unpack(dv, g);
 #pragma unroll
             for (int j = 0; j < kExBackRows; ++j) {
                 if (a.drows && p[j] >= 0) {
@@ -570,6 +631,23 @@ void launch_sort(SortArgs &a, int device, cudaStream_t s) {
     launch(expert_copy_kernel<B>, (a.tokens + per_cta - 1) / per_cta, s, true, a, "expert_copy_kernel");
 }
 
+template <int B>
+void launch_unnamed_rows(const ReturnArgs &a, cudaStream_t s) {
+    // A cluster for every 8,192 picks, up to 16: more than one only pay where rows are zeroed (both kernels at 4,096 x 8
+    // rows of 128 bytes: 5.8 us with one, 7.0 with five, 7.4 with 16; a tenth of the picks dropped 34, 16.7 and 14.1 us).
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(kUnnamedCluster * std::min(1 + a.tokens * a.topk / 8192, 16));
+    cfg.blockDim = dim3(kUnnamedThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kUnnamedCluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    check_cuda(cudaLaunchKernelEx(&cfg, expert_unnamed_rows_kernel<B>, a), "expert_unnamed_rows_kernel");
+}
+
 template <int TYPE, int B>
 void launch_return(ReturnArgs &a, bool backward, cudaStream_t s) {
     a.group = group_of(a.row_bytes / B);
@@ -578,10 +656,12 @@ void launch_return(ReturnArgs &a, bool backward, cudaStream_t s) {
     // of 2,048: 55 us, 59 us with a CTA a token).
     if (backward && a.tokens >= 2368 && a.row_bytes / B <= 512) a.group = std::min(a.group, 32);
     const int per_cta = kExThreads / a.group, grid = (a.tokens + per_cta - 1) / per_cta;
-    if (backward)
-        launch(expert_return_backward_kernel<TYPE, B>, grid, s, false, a, "expert_return_backward_kernel");
-    else
+    if (backward) {
+        if (a.drows) launch_unnamed_rows<B>(a, s);
+        launch(expert_return_backward_kernel<TYPE, B>, grid, s, a.drows != nullptr, a, "expert_return_backward_kernel");
+    } else {
         launch(expert_return_kernel<TYPE, B>, grid, s, false, a, "expert_return_kernel");
+    }
 }
 
 // `vec` is an element at least: the entry points refuse addresses off their elements.

@@ -24,7 +24,10 @@ MAX_TOPK, MAX_EXPERTS = 64, 1024
 
 
 class ExpertOrder(NamedTuple):
-    """Where ``expert_sort`` put the picks (int32 CUDA tensors)."""
+    """Where ``expert_sort`` put the picks (int32 CUDA tensors). A pick may be
+    dropped after the sort too (a capacity limit), by an ``inverse`` of its own
+    with -1 there: ``order._replace(inverse=...)``. The return leaves it out,
+    and the gradient of its row is zero. No two picks may name the same row."""
 
     perm: torch.Tensor     # [T*K] flat pick token*K + k of each row, -1 past the last expert's rows
     inverse: torch.Tensor  # [T, K] row of each pick, -1 where its id names no expert
