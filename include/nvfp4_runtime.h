@@ -387,11 +387,13 @@ NVFP4_API size_t nvfp4_linear_workspace_bytes(
  * [vectors, rows] (rows / 2 with a gate) are of `type`, each with its own row
  * stride in elements (columns contiguous); bias [rows] has a type of its own;
  * bias and residual may be NULL, residual may be out itself (else neither it
- * nor x shares memory with out). The weights'
- * values are exact in the products, sums are FP32, and the result is rounded
- * once. BF16 and FP32 elements of x below 2^-29 of their row's largest finite
- * value may lose low bits (by less than 2^-39 of that value). No memory is
- * allocated and the matrix is only read: calls may overlap and be captured in
+ * nor x shares memory with out). The weights' values are exact in the
+ * products, sums are FP32, and the result is rounded once. FP32 elements of x
+ * enter right to 2^-23 of themselves, or to 2^-39 of their row's largest finite
+ * value where that is more (from 2^-16 of it down); BF16 elements exactly, but
+ * in calls of few rows those below 2^-31 of their row's largest, to 2^-39 of
+ * it; FP16 elements exactly. No memory is allocated and the matrix is only
+ * read: calls may overlap and be captured in
  * CUDA graphs. Up to 2^30 vectors. */
 NVFP4_API nvfp4_status nvfp4_linear_fused(
     nvfp4_runtime * runtime,

@@ -132,3 +132,50 @@ def test_captured_gradients_of_another_order(cuda_runtime):
         torch.cuda.synchronize()
         ref.check(drows, want, 2.0 ** -24 * want.abs(), share)
         ref.check(dweights, dw, hidden * 2.0 ** -24 * size + 2.0 ** -23 * dw.abs(), share)
+
+
+# ------------------------------------------------------------------ ranges of values
+
+
+@pytest.mark.parametrize("vectors", [1, 4, 50])
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_tiny_rows_and_large_divisors(cuda_runtime, kind, vectors):
+    """Rows near the smallest normal numbers under divisors of real checkpoints: the results are normal numbers, and as
+    many of their bits are right as elsewhere."""
+    rt, dtype = cuda_runtime, TYPES[kind]
+    packed, scales, _ = ref.random_matrix(2, 70, 256, 90)
+    divisors = torch.tensor([9e3, 1.1e5])
+    m = rt.upload_grouped(packed.cuda(), scales.cuda(), divisors.cuda())
+    one = rt.upload_grouped(packed[1:].cuda(), scales[1:].cuda(), divisors[1:].cuda())
+    for size in (1e-32, 1e-34):
+        x = (_normal(91, vectors, 256).double() * size).to(dtype)
+        bias = (_normal(92, 70).double() * size * 1e-4).float()
+        want, tol = ref.linear(x, packed[1].cuda(), scales[1].cuda(), divisors[1].cuda(), bias)
+        assert float(want.abs().median()) > 2.0 ** -126
+        ref.check(rt.linear_fused(one, x, bias=bias), want, tol, size)
+        offsets = torch.tensor([0, 0, vectors], dtype=torch.int32, device="cuda")
+        both = torch.stack([bias, bias])
+        ref.check(rt.linear_grouped(m, x, offsets, bias=both), want, tol, size)
+    m.close()
+    one.close()
+
+
+@pytest.mark.parametrize("vectors", [1, 6, 50])
+def test_bits_of_fp32_elements(cuda_runtime, vectors):
+    """Elements of an FP32 row are right to 2^-23 of themselves, or to 2^-39 of the row's largest value where that is
+    more (from 2^-16 of it down): shown with the largest value in columns whose weights are zero."""
+    rt, rows, cols = cuda_runtime, 48, 160
+    packed, scales, divisors = ref.random_matrix(1, rows, cols, 93)
+    packed[:, :, :8] = 0  # the first 16 columns
+    m = rt.upload_grouped(packed.cuda(), scales.cuda(), divisors.cuda())
+    w = ref.weights(packed[0], scales[0]).cuda()
+    inv = (1.0 / divisors.cuda()).double()
+    for largest in (1.0, 2.0 ** 15, 2.0 ** 20, 2.0 ** 29):
+        x = _normal(94, vectors, cols)
+        x[:, 3] = largest
+        got = rt.linear_fused(m, x).double()
+        xd = x.double()
+        element = torch.maximum(xd.abs() * 2.0 ** -23, xd.abs().amax(1, keepdim=True) * 2.0 ** -39)
+        _, tol = ref.linear(x[:, 16:], packed[0, :, 8:].cuda(), scales[0, :, 1:].cuda(), divisors[0].cuda())
+        ref.check(got, xd @ w.t() * inv, tol + element @ w.abs().t() * inv, largest)
+    m.close()

@@ -226,8 +226,12 @@ __device__ __forceinline__ void finish_rows(const GemmArgs &a, const Finish &t, 
         float z[2];
 #pragma unroll
         for (int k = 0; k < kRowStep; ++k) {
-            const float scale = TYPE == NVFP4_TYPE_F32 ? t.inv * __shfl_sync(0xffffffffu, row_scale, (c0 & 16) + i + k) : t.inv;
-            z[k] = fmaf(sums[i + k], scale, t.bias);
+            // The row's power of two comes last: with the divisor first the product may be subnormal where the result is
+            // not.
+            if constexpr (TYPE == NVFP4_TYPE_F32)
+                z[k] = fmaf(sums[i + k] * t.inv, __shfl_sync(0xffffffffu, row_scale, (c0 & 16) + i + k), t.bias);
+            else
+                z[k] = fmaf(sums[i + k], t.inv, t.bias);
         }
         y[i / kRowStep] = z[0];
         if constexpr (GATED) {

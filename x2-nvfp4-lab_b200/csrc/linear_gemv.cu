@@ -13,7 +13,9 @@
 // (largest finite value to [2^14, 2^15)), which is exact for every element
 // down to 2^-31 of the row's largest and off by less than 2^-39 of it below;
 // FP32 scaled the same way as two columns, high and low half (22 bits and a
-// sign, 2^-23 of an element). The scale comes back in the epilogue.
+// sign): off by 2^-23 of an element at most down to 2^-16 of the row's largest,
+// where the low half becomes subnormal, and by 2^-39 of that largest below it.
+// The scale comes back in the epilogue.
 //
 // Every 512 columns the MMAs' sums are added to FP32 registers: the tensor
 // core rounds its running sum towards zero, which over long rows would grow
@@ -416,13 +418,15 @@ __global__ void __launch_bounds__(kGvThreads, 2) linear_gemv_kernel(const __grid
 
             // One output from its sum (and its up sum with a gate).
             auto output = [&](const Place &p, float inv, int col0, int row, int v, float z, float z_up) {
-                const float scale = inv * back[col0 + v];
-                z *= scale;
+                // The row's power of two comes last: with the divisor first the product may be subnormal where the result
+                // is not.
+                const float scale = back[col0 + v];
+                z = z * inv * scale;
                 const size_t at = (size_t)p.group * f.rows + row;
                 if (f.bias) z += load_as_f32(f.bias, f.bias_type, at);
                 z = activate(z, f.act);
                 if (f.gated) {
-                    z_up *= scale;
+                    z_up = z_up * inv * scale;
                     if (f.bias) z_up += load_as_f32(f.bias, f.bias_type, at + f.out_rows);
                     z *= z_up;
                 }
