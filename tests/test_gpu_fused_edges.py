@@ -179,3 +179,38 @@ def test_bits_of_fp32_elements(cuda_runtime, vectors):
         _, tol = ref.linear(x[:, 16:], packed[0, :, 8:].cuda(), scales[0, :, 1:].cuda(), divisors[0].cuda())
         ref.check(got, xd @ w.t() * inv, tol + element @ w.abs().t() * inv, largest)
     m.close()
+
+
+@pytest.mark.parametrize("cols", [4112, 8192, 11008, 49152])
+@pytest.mark.parametrize("vectors", [3, 40, 200])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_long_sums_of_one_sign(cuda_runtime, kind, vectors, cols):
+    """Products of one sign over long rows, the rounded sum taken off again by the residual, so that what is left shows
+    the FP32 sum itself: low by less than 2^-14 of it (an eighth of FP16's half step) whatever the length, and the bits
+    of a second call."""
+    rt, dtype, rows = cuda_runtime, TYPES[kind], 301
+    packed, scales, divisors = ref.random_matrix(2, rows, cols, 95)
+    packed &= 0x77  # no weight below zero
+    divisors = divisors * (cols / 64)
+    m = rt.upload_grouped(packed[:1].cuda(), scales[:1].cuda(), divisors[:1].cuda())
+    gen = torch.Generator().manual_seed(96)
+    x = torch.rand(vectors, cols, generator=gen).to(dtype).cuda()
+    z = x.double() @ ref.weights(packed[0].cuda(), scales[0].cuda()).t() * (1.0 / divisors[0]).double().cuda()
+    taken = (-z).to(dtype)
+    want = z + taken.double()
+    half = torch.finfo(dtype).eps / 2
+    got = rt.linear_fused(m, x, residual=taken)
+    ref.check(got, want, 2.0 ** -14 * z * (1 + half) + half * want.abs() + torch.finfo(dtype).tiny)
+    assert torch.equal(got, rt.linear_fused(m, x, residual=taken))
+    m.close()
+    # The same sums with a gate over groups of uneven rows, against the plain bound of the type.
+    m = rt.upload_grouped(packed[:, :300].contiguous().cuda(), scales[:, :300].contiguous().cuda(), divisors.cuda())
+    cut = vectors // 3
+    offsets = torch.tensor([0, cut, vectors], dtype=torch.int32, device="cuda")
+    got = rt.linear_grouped(m, x, offsets, activation="relu_mul")
+    for g, rows_of in enumerate((slice(0, cut), slice(cut, vectors))):
+        w = ref.weights(packed[g, :300].cuda(), scales[g, :300].cuda())
+        z = x[rows_of].double() @ w.t() * (1.0 / divisors[g]).double().cuda()
+        want = z[:, :150] * z[:, 150:]
+        ref.check(got[rows_of], want, (2.0 ** -13 + 2.0 ** -20 + half) * want)
+    m.close()

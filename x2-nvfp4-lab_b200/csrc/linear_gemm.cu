@@ -54,6 +54,7 @@ constexpr int kGmThreads = 32 * (kGmEpiWarp0 + 4 * kGmEpiGroups);
 constexpr int kGmLargeN = 160;                      // rows of x per tile
 constexpr int kGmSmallN = 64;                       // of calls with few, and of split FP32 x (32 per epilogue warpgroup)
 constexpr int kGmSegment32 = 1;                     // steps per accumulator of split FP32 x
+constexpr int kGmSegment16 = 32;                    // and at most of 16-bit x
 constexpr int kGmRawBytes = 128 * 128;              // 256 columns of packed weights
 constexpr int kGmRawScales = 128 * 16;
 constexpr int kGmRaw = kGmRawBytes + kGmRawScales;
@@ -319,8 +320,9 @@ __device__ __forceinline__ void finish_rows(const GemmArgs &a, const Finish &t, 
     else finish_rows<TYPE, false, false>(a, t, c0, sums, row_scale);
 }
 
-// TYPE: of x, residual and out; FP32 x arrives as FP16 parts.
-template <int TYPE, int N>
+// TYPE: of x, residual and out; FP32 x arrives as FP16 parts. CARRIED: rows of 16-bit x too long for one accumulator; the
+// second one carries the sums of the segments before.
+template <int TYPE, int N, bool CARRIED>
 __global__ void __launch_bounds__(kGmThreads, 1)
     linear_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_s,
                        const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ GemmArgs a) {
@@ -499,8 +501,10 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                 const uint32_t n = __reduce_max_sync(0xffffffffu, tile_of(a, upto, item, group).n);
                 const uint32_t idesc = tc::idesc_16bit_pair((n + 15) & ~15u, kBf16 ? 1u : 0u);
                 for (int left = a.k_steps; left > 0 && ok; left -= a.segment, ++use) {
-                    const uint32_t buf = use & 1, acc = tmem + buf * N;
-                    if (use > 1 && !wait_warp(acc_empty + buf, ((use >> 1) - 1) & 1u, err, kSiteFusedAccEmpty)) {
+                    const uint32_t buf = use & 1, acc = tmem + (CARRIED ? 0 : buf * N);
+                    // The last use of this accumulator: two before, or the one before.
+                    const uint32_t prior = use - (CARRIED ? 1 : 2);
+                    if ((int)prior >= 0 && !wait_warp(acc_empty + (prior & 1), (prior >> 1) & 1u, err, kSiteFusedAccEmpty)) {
                         ok = false;
                         break;
                     }
@@ -628,8 +632,8 @@ __global__ void __launch_bounds__(kGmThreads, 1)
         };
         // With more tiles than pairs the warpgroups take whole tiles in turn (each its accumulator; what one waits for at
         // the start of a tile hides behind the other's work), else every other 16 columns of the one tile. FP32 always
-        // does the latter: its sums are in registers.
-        const bool whole = TYPE != NVFP4_TYPE_F32 && items > pairs;
+        // does the latter, its sums are in registers, and so do rows of several segments.
+        const bool whole = TYPE != NVFP4_TYPE_F32 && items > pairs && !CARRIED;
         auto release = [&]() {
             tc::fence_before_sync();
             __syncwarp();
@@ -672,20 +676,48 @@ __global__ void __launch_bounds__(kGmThreads, 1)
                 for (int h = 0; h < 2; ++h)
                     if (32 * piece + 16 * h < t.n) finish_rows<TYPE>(a, to, 32 * piece + 16 * h, sum[h], row_scale);
             } else {
-                if (!filled()) break;
+                uint32_t from = lanes + (use & 1) * N;
+                if constexpr (CARRIED) {
+                    // Each segment's sums to those of the segments before, which the rest of the tile is made of.
+                    from = lanes + N;
+                    for (int ks = 0; ks < a.k_steps && ok; ks += a.segment) {
+                        ok = filled();
+                        if (!ok) break;
+                        for (int c0 = 16 * piece; c0 < t.n; c0 += 16 * kGmEpiGroups) {
+                            uint32_t r[16], before[16];
+                            tc::ld_32x32b_x16(lanes + c0, r);
+                            if (ks != 0) tc::ld_32x32b_x16(from + c0, before);
+                            tc::wait_ld();
+                            if (ks != 0) {
+#pragma unroll
+                                for (int i = 0; i < 16; ++i)
+                                    r[i] = __float_as_uint(__uint_as_float(before[i]) + __uint_as_float(r[i]));
+                            }
+                            tc::st_32x32b_x16(from + c0, r);
+                        }
+                        tc::wait_st();
+                        release();
+                        ++use;
+                    }
+                } else {
+                    ok = filled();
+                }
+                if (!ok) break;
                 const int step = whole ? 16 : 16 * kGmEpiGroups, c_first = whole ? 0 : 16 * piece;
                 for (int c0 = c_first; c0 < t.n; c0 += step) {
                     uint32_t r[16];
                     float sum[16];
-                    tc::ld_32x32b_x16(lanes + (use & 1) * N + c0, r);
+                    tc::ld_32x32b_x16(from + c0, r);
                     tc::wait_ld();
-                    if (c0 + step >= t.n) release();
+                    if (!CARRIED && c0 + step >= t.n) release();
 #pragma unroll
                     for (int i = 0; i < 16; ++i) sum[i] = __uint_as_float(r[i]);
                     finish_rows<TYPE>(a, to, c0, sum, 1.0f);
                 }
-                if (c_first >= t.n) release();
-                ++use;
+                if (!CARRIED) {
+                    if (c_first >= t.n) release();
+                    ++use;
+                }
             }
         }
     }
@@ -784,11 +816,11 @@ size_t parts_bytes(int type, int vectors, int cols) {
     return ((size_t)vectors * cols * (type == NVFP4_TYPE_F32 ? 4 : 2) + 255) & ~size_t(255);
 }
 
-template <int TYPE, int N>
-void launch(const GemmArgs &g, const nvfp4_matrix &matrix, const CUtensorMap &map_x, int grid, bool dependent,
+template <int TYPE, int N, bool CARRIED>
+void launch_as(const GemmArgs &g, const nvfp4_matrix &matrix, const CUtensorMap &map_x, int grid, bool dependent,
             cudaStream_t stream) {
     static std::atomic<uint64_t> done{0};
-    allow_shared_memory(linear_gemm_kernel<TYPE, N>, Shape<N, TYPE == NVFP4_TYPE_F32 ? 2 : 1>::kSmem, done,
+    allow_shared_memory(linear_gemm_kernel<TYPE, N, CARRIED>, Shape<N, TYPE == NVFP4_TYPE_F32 ? 2 : 1>::kSmem, done,
                         matrix.runtime->device, "cudaFuncSetAttribute(linear_gemm_kernel)");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
@@ -803,8 +835,16 @@ void launch(const GemmArgs &g, const nvfp4_matrix &matrix, const CUtensorMap &ma
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = dependent ? 2 : 1;
-    check_cuda(cudaLaunchKernelEx(&cfg, linear_gemm_kernel<TYPE, N>, matrix.map_w, matrix.map_s, map_x, g),
+    check_cuda(cudaLaunchKernelEx(&cfg, linear_gemm_kernel<TYPE, N, CARRIED>, matrix.map_w, matrix.map_s, map_x, g),
                "linear_gemm_kernel");
+}
+
+template <int TYPE, int N>
+void launch(const GemmArgs &g, const nvfp4_matrix &matrix, const CUtensorMap &map_x, int grid, bool dependent,
+            cudaStream_t stream) {
+    if constexpr (TYPE == NVFP4_TYPE_F32) launch_as<TYPE, N, false>(g, matrix, map_x, grid, dependent, stream);
+    else if (g.segment < g.k_steps) launch_as<TYPE, N, true>(g, matrix, map_x, grid, dependent, stream);
+    else launch_as<TYPE, N, false>(g, matrix, map_x, grid, dependent, stream);
 }
 
 }  // namespace
@@ -824,7 +864,8 @@ void launch_linear_gemm(const FusedLinearArgs &f, const nvfp4_matrix &matrix, vo
     g.m_pairs = f.gated ? (f.out_rows + 127) / 128 : (f.rows + 255) / 256;
     g.k_steps = (f.cols + 127) / 128;
     g.raw_steps = (f.cols + 255) / 256;
-    g.segment = f.type == NVFP4_TYPE_F32 ? kGmSegment32 : g.k_steps;
+    const int segments = (g.k_steps + kGmSegment16 - 1) / kGmSegment16;
+    g.segment = f.type == NVFP4_TYPE_F32 ? kGmSegment32 : (g.k_steps + segments - 1) / segments;
     // A CTA's half of a tile in one box (a piece that hangs over loads rows that no sum of the tile uses): fitted to the
     // even tiles of a single group, the most that a tile holds where the counts are on the device (boxes of 16 rows
     // instead: 8,192 rows over 64 groups 39.3 against 38.4 us).
