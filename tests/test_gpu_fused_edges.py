@@ -3,6 +3,8 @@ long rows, orders changed after the sort, calls one after the other (needs an sm
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -213,4 +215,31 @@ def test_long_sums_of_one_sign(cuda_runtime, kind, vectors, cols):
         z = x[rows_of].double() @ w.t() * (1.0 / divisors[g]).double().cuda()
         want = z[:, :150] * z[:, 150:]
         ref.check(got[rows_of], want, (2.0 ** -13 + 2.0 ** -20 + half) * want)
+    m.close()
+
+
+@pytest.mark.parametrize("vectors", [8, 640])
+def test_fp32_activations_to_their_last_bits(cuda_runtime, vectors):
+    """SiLU and GELU's tanh form of FP32 rows against 64 bits, relative to the result: exp and the fast division (by 1 to
+    2) are off by two units at most (2^-23 each), the sum and a product by half of one each: five. The tanh form's
+    argument u, whose error exp passes on, takes half a unit for its factor, its last product and the FMA each, and for
+    three more roundings of the cubic part: six halves of a unit of u."""
+    rt = cuda_runtime
+    # The identity: code 2 is 1, scale byte 0x38 is 1.
+    packed = torch.zeros(1, 16, 8, dtype=torch.uint8)
+    for r in range(16):
+        packed[0, r, r // 2] = 2 << (4 * (r % 2))
+    m = rt.upload_grouped(packed.cuda(), torch.full((1, 16, 1), 0x38, dtype=torch.uint8).cuda(), torch.ones(1).cuda())
+    for name, low in (("silu", -87.0), ("gelu_tanh", -9.0)):
+        x = torch.linspace(low, 20.0, vectors * 16).reshape(vectors, 16).cuda()
+        z = rt.linear_fused(m, x).double()  # what the activation gets
+        u = z if name == "silu" else 2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)
+        want = z * torch.sigmoid(u)
+        units = 5.0 if name == "silu" else 5.0 + 3.0 * u.abs()
+        ref.check(rt.linear_fused(m, x, activation=name), want, units * 2.0 ** -23 * want.abs() + 2.0 ** -149, name)
+        up = rt.upload_grouped(packed.repeat(1, 2, 1).cuda(), torch.full((1, 32, 1), 0x38, dtype=torch.uint8).cuda(),
+                               torch.ones(1).cuda())
+        ref.check(rt.linear_fused(up, x, activation=name + "_mul"), want * z, (units + 0.5) * 2.0 ** -23 * (want * z).abs()
+                  + 2.0 ** -140, name)
+        up.close()
     m.close()

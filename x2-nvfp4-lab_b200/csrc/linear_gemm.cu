@@ -211,10 +211,10 @@ struct Finish {
     float inv, bias;
 };
 
-template <int ACT, int COUNT>
+template <int ACT, bool FP32, int COUNT>
 __device__ __forceinline__ void activate_all(float (&y)[COUNT]) {
 #pragma unroll
-    for (int i = 0; i < COUNT; ++i) y[i] = activate<ACT>(y[i]);
+    for (int i = 0; i < COUNT; ++i) y[i] = activate<ACT, FP32>(y[i]);
 }
 
 // 16 rows of x from c0 on: scale, bias, activation, gate, residual, one rounding, store. With a gate lanes 0-15 hold
@@ -224,7 +224,8 @@ __device__ __forceinline__ void activate_all(float (&y)[COUNT]) {
 template <int TYPE, bool GATED, bool ACTIVE>
 __device__ __forceinline__ void finish_rows(const GemmArgs &a, const Finish &t, int c0, const float (&sums)[16], float row_scale) {
     constexpr int kOut = GATED ? 8 : 16, kRowStep = GATED ? 2 : 1;
-    constexpr int kBytes = TYPE == NVFP4_TYPE_F32 ? 4 : 2;
+    constexpr bool kFp32 = TYPE == NVFP4_TYPE_F32;
+    constexpr int kBytes = kFp32 ? 4 : 2;
     const FusedLinearArgs &f = a.f;
     const int lane = threadIdx.x & 31;
     float y[kOut], up[kOut];
@@ -248,10 +249,10 @@ __device__ __forceinline__ void finish_rows(const GemmArgs &a, const Finish &t, 
         }
     }
     if constexpr (ACTIVE) switch (f.act) {
-        case NVFP4_ACT_RELU: activate_all<NVFP4_ACT_RELU>(y); break;
-        case NVFP4_ACT_SILU: activate_all<NVFP4_ACT_SILU>(y); break;
-        case NVFP4_ACT_GELU: activate_all<NVFP4_ACT_GELU>(y); break;
-        case NVFP4_ACT_GELU_TANH: activate_all<NVFP4_ACT_GELU_TANH>(y); break;
+        case NVFP4_ACT_RELU: activate_all<NVFP4_ACT_RELU, kFp32>(y); break;
+        case NVFP4_ACT_SILU: activate_all<NVFP4_ACT_SILU, kFp32>(y); break;
+        case NVFP4_ACT_GELU: activate_all<NVFP4_ACT_GELU, kFp32>(y); break;
+        case NVFP4_ACT_GELU_TANH: activate_all<NVFP4_ACT_GELU_TANH, kFp32>(y); break;
         default: break;
     }
     if constexpr (GATED) {

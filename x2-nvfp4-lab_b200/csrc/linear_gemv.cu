@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(kGvThreads, 2) linear_gemv_kernel(const __grid
                 z = z * inv * scale;
                 const size_t at = (size_t)p.group * f.rows + row;
                 if (f.bias) z += load_as_f32(f.bias, f.bias_type, at);
-                z = activate(z, f.act);
+                z = activate<TYPE == NVFP4_TYPE_F32>(z, f.act);
                 if (f.gated) {
                     z_up = z_up * inv * scale;
                     if (f.bias) z_up += load_as_f32(f.bias, f.bias_type, at + f.out_rows);
