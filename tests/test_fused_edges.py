@@ -4,9 +4,14 @@ of test_fused_refusals.py (no GPU)."""
 from __future__ import annotations
 
 import ctypes as C
+from types import SimpleNamespace
 
 import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.autograd import forward_ad
 
+from vllm_nvfp4_cuda import experts, fused
 from vllm_nvfp4_cuda.runtime import load_library
 
 
@@ -68,3 +73,65 @@ MISALIGNED = {
 def test_misaligned_addresses_are_refused(lib, what):
     assert MISALIGNED[what](lib) == 1
     assert b"aligned" in lib.nvfp4_last_error()
+
+
+# ------------------------------------------------------------------ tensors without memory: the Python checks
+
+
+class _Unreached:
+    """Stands for the runtime: a call that is refused in time never asks it for anything."""
+
+    def __getattr__(self, name):
+        raise AssertionError(f"the runtime was reached ({name})")
+
+
+RT = _Unreached()
+
+
+def _cuda(*shape, dtype=torch.bfloat16):
+    return torch.empty(shape, dtype=dtype, device="cuda:0")
+
+
+def _matrix(rows=64, cols=64, groups=1):
+    return SimpleNamespace(rows=rows, cols=cols, groups=groups, device=0)
+
+
+def _order(tokens=5, topk=2, n=4):
+    return experts.ExpertOrder(_cuda(tokens * topk, dtype=torch.int32), _cuda(tokens, topk, dtype=torch.int32),
+                               _cuda(n + 1, dtype=torch.int32), n)
+
+
+def _dual(*shape):
+    return forward_ad.make_dual(_cuda(*shape), _cuda(*shape))
+
+
+DUALS = {
+    "linear of x": lambda: fused.linear_fused(RT, _matrix(), _dual(3, 64), None, None, None, None, None),
+    "linear of bias": lambda: fused.linear_fused(RT, _matrix(), _cuda(3, 64), _dual(64), None, None, None, None),
+    "linear of residual": lambda: fused.linear_fused(RT, _matrix(), _cuda(3, 64), None, None, _dual(3, 64), None, None),
+    "grouped linear of x": lambda: fused.linear_grouped(RT, _matrix(groups=2), _dual(3, 64),
+                                                        _cuda(3, dtype=torch.int32), None, None, None, None),
+    "grouped linear of bias": lambda: fused.linear_grouped(RT, _matrix(groups=2), _cuda(3, 64),
+                                                           _cuda(3, dtype=torch.int32), _dual(2, 64), None, None, None),
+    "sort of x": lambda: experts.expert_sort(RT, _dual(5, 8), _cuda(5, 2, dtype=torch.int32), 4),
+    "return of rows": lambda: experts.expert_return(RT, _dual(10, 8), _order()),
+    "return of weights": lambda: experts.expert_return(RT, _cuda(10, 8), _order(), _dual(5, 2)),
+    "return of residual": lambda: experts.expert_return(RT, _cuda(10, 8), _order(), None, _dual(5, 8)),
+}
+
+
+@pytest.mark.parametrize("what", list(DUALS))
+def test_forward_mode_derivatives_are_refused(what):
+    """A tangent would be dropped without a word; a dual level without tangents, or no_grad within one, changes nothing."""
+    with FakeTensorMode(), forward_ad.dual_level():
+        with pytest.raises(ValueError, match="forward-mode"):
+            DUALS[what]()
+        with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+            DUALS[what]()
+
+
+def test_calls_in_a_dual_level_without_tangents():
+    with FakeTensorMode(), forward_ad.dual_level():
+        assert fused.linear_fused(RT, _matrix(), _cuda(0, 64), None, None, None, None, None).shape == (0, 64)
+        rows, order = experts.expert_sort(RT, _cuda(0, 8), _cuda(0, 2, dtype=torch.int32), 4)
+        assert experts.expert_return(RT, rows, order).shape == (0, 8)

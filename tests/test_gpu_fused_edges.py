@@ -243,3 +243,23 @@ def test_fp32_activations_to_their_last_bits(cuda_runtime, vectors):
                   + 2.0 ** -140, name)
         up.close()
     m.close()
+
+
+# ------------------------------------------------------------------ what a call does to its tensors
+
+
+def test_forward_mode_derivatives_of_gradients_are_refused(cuda_runtime):
+    """A tangent that comes in with the gradient of the sort or the return would be dropped."""
+    from torch.autograd import forward_ad
+
+    ids = torch.tensor([[0], [1], [0]], dtype=torch.int32, device="cuda")
+    x = _normal(101, 3, 8).requires_grad_()
+    rows, order = cuda_runtime.expert_sort(x, ids, 2)
+    out = cuda_runtime.expert_return(rows, order)
+    with forward_ad.dual_level():
+        for result in (rows, out):
+            g = forward_ad.make_dual(torch.ones_like(result), torch.ones_like(result))
+            with pytest.raises(ValueError, match="forward-mode"):
+                torch.autograd.grad(result, x, g, retain_graph=True)
+    (dx,) = torch.autograd.grad(out, x, torch.ones_like(out))
+    assert torch.equal(dx, torch.ones_like(x))

@@ -15,6 +15,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .runtime import CUDA_STREAM_LEGACY
 
@@ -42,6 +43,17 @@ def _rows_of(t: torch.Tensor) -> torch.Tensor:
 
 def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def refuse_tangents(tensors):
+    """Raises where one of the tensors (or None) carries a forward-mode derivative: ``requires_grad`` does not say so, and
+    the result would come without it."""
+    if forward_ad._current_level < 0 or not torch._C._is_fwd_grad_enabled():
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError("no forward-mode derivative goes through this operator: call it on the primal tensors "
+                             "(torch.autograd.forward_ad.unpack_dual)")
 
 
 def on_stream(stream, tensors, call):
@@ -141,11 +153,13 @@ def _return_backward(rt, dout, rows, inverse, offsets, weights, experts, need_ro
 
 
 def _sort_gradient(ctx, drows):
+    refuse_tangents((drows,))
     (inverse,) = ctx.saved_tensors
     return _return(ctx.rt, drows, inverse, None, None, None), None, None, None, None
 
 
 def _return_gradient(ctx, dout):
+    refuse_tangents((dout,))
     rows, weights, inverse, offsets = ctx.saved_tensors
     need_rows, need_weights, need_residual = ctx.needs_input_grad[:3]
     drows = dweights = None
@@ -205,6 +219,7 @@ def expert_sort(rt, x, ids, experts: int, stream=None):
     _require(1 <= ids.shape[1] <= MAX_TOPK, "the expert sort supports 1 to 64 picks a token")
     experts = int(experts)
     _require(1 <= experts <= MAX_EXPERTS, "the expert sort supports 1 to 1024 experts")
+    refuse_tangents((x,))
     grad = x.requires_grad and torch.is_grad_enabled()
 
     def call():
@@ -238,6 +253,7 @@ def expert_return(rt, rows, order: ExpertOrder, weights=None, residual=None, out
                  "residual must match the rows' type and device, [tokens, hidden]")
         grad = grad or residual.requires_grad
     grad = grad and torch.is_grad_enabled()
+    refuse_tangents((rows, weights, residual))
     if out is not None:
         _require(out.shape == (tokens, hidden) and out.dtype == rows.dtype and out.device == device
                  and (out.stride(1) == 1 or hidden == 1) and (tokens < 2 or out.stride(0) >= hidden),

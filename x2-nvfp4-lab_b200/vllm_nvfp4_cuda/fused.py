@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import torch
 
-from .experts import TYPES, _row_stride, _rows_of, on_stream, stream_of
+from .experts import TYPES, _row_stride, _rows_of, on_stream, refuse_tangents, stream_of
 from .runtime import ACTIVATIONS
 
 # A call on one token is over on the GPU in a few microseconds, less than its way through Python: messages are made only
@@ -42,6 +42,7 @@ def _check(matrix, x, bias, activation, others):
         recorded = recorded or bias.requires_grad
     if recorded and torch.is_grad_enabled():
         _refuse("the NVFP4 linear records no gradient: call it under torch.no_grad() or on detached tensors")
+    refuse_tangents((x, bias, *others))
     if activation is None:
         return matrix.rows
     if activation not in ACTIVATIONS:
