@@ -135,3 +135,33 @@ def test_calls_in_a_dual_level_without_tangents():
         assert fused.linear_fused(RT, _matrix(), _cuda(0, 64), None, None, None, None, None).shape == (0, 64)
         rows, order = experts.expert_sort(RT, _cuda(0, 8), _cuda(0, 2, dtype=torch.int32), 4)
         assert experts.expert_return(RT, rows, order).shape == (0, 8)
+
+
+def _repeated(rows, columns, dtype=torch.bfloat16):
+    return _cuda(1, columns, dtype=dtype).expand(rows, columns)
+
+
+# Numbers that pass what the C ABI takes: an int of it would hold the low 32 bits, 3 or 8 here, and the call would do a
+# part of the work.
+HUGE = {
+    "linear of 2^32 + 3 rows": lambda: fused.linear_fused(RT, _matrix(1, 16), _repeated(2 ** 32 + 3, 16), None, None, None,
+                                                          None, None),
+    "linear of 2^30 + 1 rows": lambda: fused.linear_fused(RT, _matrix(1, 16), _repeated(2 ** 30 + 1, 16), None, None, None,
+                                                          None, None),
+    "linear of 2^32 + 3 rows of three axes": lambda: fused.linear_fused(
+        RT, _matrix(1, 16), _cuda(1, 1, 16).expand(2, 2 ** 31 + 2, 16), None, None, None, None, None),
+    "grouped linear of 2^32 + 3 rows": lambda: fused.linear_grouped(
+        RT, _matrix(1, 16, 2), _repeated(2 ** 32 + 3, 16), _cuda(3, dtype=torch.int32), None, None, None, None),
+    "sort of 2^32 + 3 tokens": lambda: experts.expert_sort(RT, _repeated(2 ** 32 + 3, 1),
+                                                           _repeated(2 ** 32 + 3, 1, torch.int32), 4),
+    "sort of 2^31 picks": lambda: experts.expert_sort(RT, _repeated(2 ** 30, 1), _repeated(2 ** 30, 2, torch.int32), 4),
+    "sort of 2^32 + 8 columns": lambda: experts.expert_sort(RT, _cuda(1, 2 ** 32 + 8), _cuda(1, 1, dtype=torch.int32), 4),
+    "return of 2^32 + 3 tokens": lambda: experts.expert_return(RT, _repeated(2 ** 32 + 3, 1), _order(2 ** 32 + 3, 1)),
+    "return of 2^32 + 8 columns": lambda: experts.expert_return(RT, _cuda(1, 2 ** 32 + 8), _order(1, 1)),
+}
+
+
+@pytest.mark.parametrize("what", list(HUGE))
+def test_numbers_past_the_c_abi_are_refused(what):
+    with FakeTensorMode(), pytest.raises(ValueError, match="at most"):
+        HUGE[what]()

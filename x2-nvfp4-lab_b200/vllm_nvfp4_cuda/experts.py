@@ -22,6 +22,8 @@ from .runtime import CUDA_STREAM_LEGACY
 # Element types of the C ABI (NVFP4_TYPE_*).
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_TOPK, MAX_EXPERTS = 64, 1024
+# Checked here although the library does so too: its arguments are 32-bit, and ctypes would pass a larger number's low bits.
+MAX_PICKS, MAX_HIDDEN = 2 ** 31 - 16385, 1 << 24
 
 
 class ExpertOrder(NamedTuple):
@@ -217,6 +219,8 @@ def expert_sort(rt, x, ids, experts: int, stream=None):
     _require(ids.dtype in (torch.int32, torch.int64) and ids.dim() == 2 and ids.shape[0] == x.shape[0]
              and ids.device == x.device, "ids must be int32 or int64 [tokens, topk] on x's device")
     _require(1 <= ids.shape[1] <= MAX_TOPK, "the expert sort supports 1 to 64 picks a token")
+    _require(ids.numel() <= MAX_PICKS and x.shape[1] <= MAX_HIDDEN,
+             "the expert sort supports at most 2^31 - 16385 picks and 2^24 columns")
     experts = int(experts)
     _require(1 <= experts <= MAX_EXPERTS, "the expert sort supports 1 to 1024 experts")
     refuse_tangents((x,))
@@ -243,6 +247,8 @@ def expert_return(rt, rows, order: ExpertOrder, weights=None, residual=None, out
     _require(rows.is_cuda and rows.dim() == 2 and rows.dtype in TYPES and rows.shape[0] == tokens * topk and hidden > 0
              and device == inverse.device,
              "rows must be a CUDA bfloat16, float16 or float32 tensor [tokens * topk, hidden] on the order's device")
+    _require(rows.shape[0] <= MAX_PICKS and hidden <= MAX_HIDDEN,
+             "the expert return supports at most 2^31 - 16385 rows and 2^24 columns")
     grad = rows.requires_grad
     if weights is not None:
         _require(weights.shape == inverse.shape and weights.dtype in TYPES and weights.device == device,

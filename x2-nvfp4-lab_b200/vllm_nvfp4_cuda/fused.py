@@ -16,6 +16,10 @@ from .runtime import ACTIVATIONS
 # when they are raised, and nothing is asked of a tensor twice.
 
 
+# The library's limit, checked here because ctypes would pass a larger number's low 32 bits.
+MAX_ROWS = 1 << 30
+
+
 def _refuse(message):
     raise ValueError(message)
 
@@ -24,6 +28,8 @@ def _check(matrix, x, bias, activation, others):
     """Outputs a row, after the checks that both forms share; ``others``: the optional tensors besides bias."""
     if not (x.is_cuda and x.dtype in TYPES and x.dim() >= 1 and x.shape[-1] == matrix.cols):
         _refuse("x must be a CUDA bfloat16, float16 or float32 tensor [..., cols]")
+    if x.numel() > MAX_ROWS * matrix.cols:
+        _refuse("x must have at most 2^30 rows")
     device, home = x.device, matrix.device
     if home is not None and device.index != home:
         _refuse(f"x is on {device} but the matrix is resident on cuda:{home}")
