@@ -453,7 +453,7 @@ NVFP4_API nvfp4_status nvfp4_linear_grouped(
  *   inverse  int32 [tokens, topk]: the row of each pick, -1 for a dropped one
  *   offsets  int32 [experts + 1]: each expert's first row, then the number of
  *            rows in use
- * topk <= 64, experts <= 1024, tokens * topk below 2^31 - 16384. Enqueued on
+ * topk <= 64, experts <= 1024, tokens * topk below 2^31 - 16385. Enqueued on
  * `stream` (NULL: the runtime's stream); needs no workspace. Outputs share no
  * memory with x, ids or one another. Every array here and in the two entry
  * points below is aligned to its elements; others are refused. */

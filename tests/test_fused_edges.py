@@ -165,3 +165,20 @@ HUGE = {
 def test_numbers_past_the_c_abi_are_refused(what):
     with FakeTensorMode(), pytest.raises(ValueError, match="at most"):
         HUGE[what]()
+
+
+ELSEWHERE = SimpleNamespace(device=torch.device("cuda:1"), cuda_stream=0)  # of a stream, all that is looked at here
+STREAMS = {
+    "linear": lambda: fused.linear_fused(RT, _matrix(), _cuda(0, 64), None, None, None, None, ELSEWHERE),
+    "grouped linear": lambda: fused.linear_grouped(RT, _matrix(), _cuda(0, 64), _cuda(2, dtype=torch.int32), None, None, None,
+                                                   ELSEWHERE),
+    "sort": lambda: experts.expert_sort(RT, _cuda(0, 8), _cuda(0, 2, dtype=torch.int32), 4, ELSEWHERE),
+    "return": lambda: experts.expert_return(RT, _cuda(0, 8), _order(0), stream=ELSEWHERE),
+}
+
+
+@pytest.mark.parametrize("what", list(STREAMS))
+def test_a_stream_of_another_gpu_is_refused(what):
+    """The work would run on the current stream of the tensors' GPU instead, in no order with the given one."""
+    with FakeTensorMode(), pytest.raises(ValueError, match="stream"):
+        STREAMS[what]()

@@ -23,7 +23,7 @@ from .runtime import CUDA_STREAM_LEGACY
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_TOPK, MAX_EXPERTS = 64, 1024
 # Checked here although the library does so too: its arguments are 32-bit, and ctypes would pass a larger number's low bits.
-MAX_PICKS, MAX_HIDDEN = 2 ** 31 - 16385, 1 << 24
+MAX_PICKS, MAX_HIDDEN = 2 ** 31 - 16386, 1 << 24
 
 
 class ExpertOrder(NamedTuple):
@@ -59,8 +59,10 @@ def refuse_tangents(tensors):
 
 
 def on_stream(stream, tensors, call):
-    """``call()`` on ``stream``: what it allocates then belongs to that stream, and the given tensors are kept from reuse
-    until the stream is done with them."""
+    """``call()`` on ``stream``, of the GPU of the first tensor: what it allocates then belongs to that stream, and the
+    given tensors are kept from reuse until the stream is done with them."""
+    if stream.device != tensors[0].device:
+        raise ValueError(f"the stream is of {stream.device}, the tensors are on {tensors[0].device}")
     with torch.cuda.stream(stream):
         result = call()
     for t in tensors:
@@ -220,7 +222,7 @@ def expert_sort(rt, x, ids, experts: int, stream=None):
              and ids.device == x.device, "ids must be int32 or int64 [tokens, topk] on x's device")
     _require(1 <= ids.shape[1] <= MAX_TOPK, "the expert sort supports 1 to 64 picks a token")
     _require(ids.numel() <= MAX_PICKS and x.shape[1] <= MAX_HIDDEN,
-             "the expert sort supports at most 2^31 - 16385 picks and 2^24 columns")
+             "the expert sort supports at most 2^31 - 16386 picks and 2^24 columns")
     experts = int(experts)
     _require(1 <= experts <= MAX_EXPERTS, "the expert sort supports 1 to 1024 experts")
     refuse_tangents((x,))
@@ -248,7 +250,7 @@ def expert_return(rt, rows, order: ExpertOrder, weights=None, residual=None, out
              and device == inverse.device,
              "rows must be a CUDA bfloat16, float16 or float32 tensor [tokens * topk, hidden] on the order's device")
     _require(rows.shape[0] <= MAX_PICKS and hidden <= MAX_HIDDEN,
-             "the expert return supports at most 2^31 - 16385 rows and 2^24 columns")
+             "the expert return supports at most 2^31 - 16386 rows and 2^24 columns")
     grad = rows.requires_grad
     if weights is not None:
         _require(weights.shape == inverse.shape and weights.dtype in TYPES and weights.device == device,
