@@ -263,3 +263,34 @@ def test_forward_mode_derivatives_of_gradients_are_refused(cuda_runtime):
                 torch.autograd.grad(result, x, g, retain_graph=True)
     (dx,) = torch.autograd.grad(out, x, torch.ones_like(out))
     assert torch.equal(dx, torch.ones_like(x))
+
+
+def test_writing_to_out_is_seen_by_autograd(cuda_runtime):
+    """A tensor that autograd keeps for a gradient and that a call then writes to as its out: the backward pass says so,
+    as after any other operation in place."""
+    rt = cuda_runtime
+    packed, scales, divisors = ref.random_matrix(2, 32, 32, 97)
+    one = rt.upload_grouped(packed[:1].cuda(), scales[:1].cuda(), divisors[:1].cuda())
+    two = rt.upload_grouped(packed.cuda(), scales.cuda(), divisors.cuda())
+    x = _normal(98, 6, 32)
+    ids = torch.tensor([[0], [1], [0], [0], [1], [1]], dtype=torch.int32, device="cuda")
+    rows, order = rt.expert_sort(x, ids, 2)
+    calls = [lambda out: rt.linear_fused(one, x, out=out),
+             lambda out: rt.linear_fused(one, x.view(2, 3, 32), out=out.view(2, 3, 32)),
+             lambda out: rt.linear_grouped(two, rows, order.offsets, out=out),
+             lambda out: rt.expert_return(rows, order, out=out),
+             lambda out: rt.linear_fused(one, x[:0], out=out[:0])]
+    for i, call in enumerate(calls):
+        scale, kept = torch.ones(1, device="cuda", requires_grad=True), _normal(99, 6, 32)
+        value = (scale * kept).sum()
+        call(kept)
+        if i < 4:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                value.backward()
+        else:  # nothing was written
+            value.backward()
+    with torch.inference_mode():
+        out = torch.empty(6, 32, device="cuda")
+        assert rt.linear_fused(one, x, out=out) is out
+    one.close()
+    two.close()

@@ -71,6 +71,14 @@ def on_stream(stream, tensors, call):
     return result
 
 
+def written(out):
+    """Tells autograd that a call has written to a tensor of the caller's: one that it keeps for a gradient must not change
+    without a word."""
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+    return out
+
+
 def stream_of(device) -> int:
     """torch's current stream on ``device`` as the C ABI takes it (its default stream has handle 0, which the ABI would
     read as the runtime's own)."""
@@ -104,7 +112,8 @@ def _sort(rt, x, ids, experts):
 def _return(rt, rows, inverse, weights, residual, out):
     tokens, topk = inverse.shape
     hidden = rows.shape[1]
-    if out is None:
+    given = out is not None
+    if not given:
         out = rows.new_empty((tokens, hidden))
     if tokens == 0:
         return out
@@ -122,7 +131,7 @@ def _return(rt, rows, inverse, weights, residual, out):
             _row_stride(residual) if residual is not None else 0, tokens, topk, hidden, out.data_ptr(),
             _row_stride(out), stream_of(rows.device)),
         "nvfp4_expert_return")
-    return out
+    return written(out) if given else out
 
 
 def _return_backward(rt, dout, rows, inverse, offsets, weights, experts, need_rows, need_weights):

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import torch
 
-from .experts import TYPES, _row_stride, _rows_of, on_stream, refuse_tangents, stream_of
+from .experts import TYPES, _row_stride, _rows_of, on_stream, refuse_tangents, stream_of, written
 from .runtime import ACTIVATIONS
 
 # A call on one token is over on the GPU in a few microseconds, less than its way through Python: messages are made only
@@ -111,7 +111,7 @@ def _linear(rt, matrix, x, bias, activation, residual, out, width, shape):
                                   ACTIVATIONS[activation], r_at, r_stride, y.data_ptr(), stride, space, size,
                                   stream_of(x.device)),
         "nvfp4_linear_fused")
-    return y
+    return y if out is None else written(y)
 
 
 def linear_fused(rt, matrix, x, bias, activation, residual, out, stream):
@@ -143,7 +143,7 @@ def _grouped(rt, matrix, x, offsets, bias, activation, out, shape):
                                     width if out is None else _row_stride(y), 1 if out is None else 0, space, size,
                                     stream_of(x.device)),
         "nvfp4_linear_grouped")
-    return y
+    return y if out is None else written(y)
 
 
 def linear_grouped(rt, matrix, x, offsets, bias, activation, out, stream):
