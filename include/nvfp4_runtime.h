@@ -354,7 +354,8 @@ enum {
  * one after the other: packed [groups, rows, cols/2], scales_e4m3
  * [groups, rows, cols/16], divisors FP32 [groups], in host or device memory
  * (device sources must be complete: the copy runs on the runtime's stream and
- * is waited for). 1 to 1024 groups, cols a multiple of 16, at most 49152. The
+ * is waited for). 1 to 1024 groups, cols a multiple of 16, at most 49152, no
+ * divisor zero. The
  * handle works with nvfp4_linear_fused (one group), nvfp4_linear_grouped and
  * nvfp4_matrix_destroy; the FP32 nvfp4_linear_* entry points refuse it. */
 NVFP4_API nvfp4_status nvfp4_matrix_upload_grouped(

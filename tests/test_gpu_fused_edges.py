@@ -294,3 +294,16 @@ def test_writing_to_out_is_seen_by_autograd(cuda_runtime):
         assert rt.linear_fused(one, x, out=out) is out
     one.close()
     two.close()
+
+
+def test_divisors_of_zero_are_refused(cuda_runtime):
+    """As the dense upload refuses one: from host and device memory, wherever in the list it stands."""
+    packed, scales, divisors = ref.random_matrix(3, 16, 32, 100)
+    for at in range(3):
+        bad = divisors.clone()
+        bad[at] = 0.0
+        with pytest.raises(RuntimeError, match="divisor"):
+            cuda_runtime.upload_grouped(packed.numpy(), scales.numpy(), bad.numpy())
+        with pytest.raises(RuntimeError, match="divisor"):
+            cuda_runtime.upload_grouped(packed.cuda(), scales.cuda(), bad.cuda())
+    cuda_runtime.upload_grouped(packed.numpy(), scales.numpy(), divisors.numpy()).close()

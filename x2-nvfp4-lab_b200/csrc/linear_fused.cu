@@ -137,6 +137,12 @@ extern "C" NVFP4_API nvfp4_status nvfp4_matrix_upload_grouped(nvfp4_runtime *run
         const size_t packed_total = static_cast<size_t>(all_rows) * m->packed_pitch;
         std::lock_guard<std::mutex> lock(runtime->queue_mutex);
         cudaStream_t s = runtime->stream;
+        std::vector<float> divisor(groups);
+        check_cuda(cudaMemcpyAsync(divisor.data(), divisors, sizeof(float) * groups, cudaMemcpyDefault, s),
+                   "cudaMemcpyAsync(divisors)");
+        check_cuda(cudaStreamSynchronize(s), "cudaStreamSynchronize(divisors)");
+        for (float d : divisor)
+            if (d == 0.0f) throw invalid_argument_error("a divisor of a grouped NVFP4 matrix is zero");
         device_memory raw;
         check_cuda(cudaMalloc(&m->packed, packed_total), "cudaMalloc(matrix packed)");
         check_cuda(cudaMalloc(&m->scales, static_cast<size_t>(all_rows) * m->scale_pitch), "cudaMalloc(matrix scales)");
