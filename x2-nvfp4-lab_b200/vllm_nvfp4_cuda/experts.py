@@ -49,8 +49,9 @@ def _row_stride(t: torch.Tensor) -> int:
 
 def refuse_tangents(tensors):
     """Raises where one of the tensors (or None) carries a forward-mode derivative: ``requires_grad`` does not say so, and
-    the result would come without it."""
-    if forward_ad._current_level < 0 or not torch._C._is_fwd_grad_enabled():
+    the result would come without it. Asked only within a dual level (``forward_ad._current_level``): there are none
+    outside."""
+    if not torch._C._is_fwd_grad_enabled():
         return
     for t in tensors:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:
@@ -166,13 +167,15 @@ def _return_backward(rt, dout, rows, inverse, offsets, weights, experts, need_ro
 
 
 def _sort_gradient(ctx, drows):
-    refuse_tangents((drows,))
+    if forward_ad._current_level >= 0:
+        refuse_tangents((drows,))
     (inverse,) = ctx.saved_tensors
     return _return(ctx.rt, drows, inverse, None, None, None), None, None, None, None
 
 
 def _return_gradient(ctx, dout):
-    refuse_tangents((dout,))
+    if forward_ad._current_level >= 0:
+        refuse_tangents((dout,))
     rows, weights, inverse, offsets = ctx.saved_tensors
     need_rows, need_weights, need_residual = ctx.needs_input_grad[:3]
     drows = dweights = None
@@ -234,7 +237,8 @@ def expert_sort(rt, x, ids, experts: int, stream=None):
              "the expert sort supports at most 2^31 - 16386 picks and 2^24 columns")
     experts = int(experts)
     _require(1 <= experts <= MAX_EXPERTS, "the expert sort supports 1 to 1024 experts")
-    refuse_tangents((x,))
+    if forward_ad._current_level >= 0:
+        refuse_tangents((x,))
     grad = x.requires_grad and torch.is_grad_enabled()
 
     def call():
@@ -270,7 +274,8 @@ def expert_return(rt, rows, order: ExpertOrder, weights=None, residual=None, out
                  "residual must match the rows' type and device, [tokens, hidden]")
         grad = grad or residual.requires_grad
     grad = grad and torch.is_grad_enabled()
-    refuse_tangents((rows, weights, residual))
+    if forward_ad._current_level >= 0:
+        refuse_tangents((rows, weights, residual))
     if out is not None:
         _require(out.shape == (tokens, hidden) and out.dtype == rows.dtype and out.device == device
                  and (out.stride(1) == 1 or hidden == 1) and (tokens < 2 or out.stride(0) >= hidden),

@@ -8,6 +8,7 @@ linear has FP32 activations and leaves bias and activation to its caller
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from .experts import TYPES, _row_stride, _rows_of, on_stream, refuse_tangents, stream_of, written
 from .runtime import ACTIVATIONS
@@ -48,7 +49,8 @@ def _check(matrix, x, bias, activation, others):
         recorded = recorded or bias.requires_grad
     if recorded and torch.is_grad_enabled():
         _refuse("the NVFP4 linear records no gradient: call it under torch.no_grad() or on detached tensors")
-    refuse_tangents((x, bias, *others))
+    if forward_ad._current_level >= 0:
+        refuse_tangents((x, bias, *others))
     if activation is None:
         return matrix.rows
     if activation not in ACTIVATIONS:
