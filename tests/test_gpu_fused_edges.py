@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -307,3 +308,81 @@ def test_divisors_of_zero_are_refused(cuda_runtime):
         with pytest.raises(RuntimeError, match="divisor"):
             cuda_runtime.upload_grouped(packed.cuda(), scales.cuda(), bad.cuda())
     cuda_runtime.upload_grouped(packed.numpy(), scales.numpy(), divisors.numpy()).close()
+
+
+# ------------------------------------------------------------------ many picks, far addresses
+
+
+def _plain_order(ids, experts):
+    """perm, inverse and offsets of a stable sort, on the host."""
+    flat = ids.reshape(-1).astype(np.int64)
+    kept = np.flatnonzero((flat >= 0) & (flat < experts))
+    picks = kept[np.argsort(flat[kept], kind="stable")]
+    perm, inverse = np.full(flat.size, -1), np.full(flat.size, -1)
+    perm[:picks.size] = picks
+    inverse[picks] = np.arange(picks.size)
+    return perm, inverse.reshape(ids.shape), np.concatenate(([0], np.cumsum(np.bincount(flat[kept], minlength=experts))))
+
+
+@pytest.mark.parametrize("how", ["all", "some", "one", "runs"])
+@pytest.mark.parametrize("tokens,topk,experts,hidden", [(8192, 8, 256, 4), (9001, 8, 256, 4), (70001, 1, 9, 1),
+                                                        (66000, 2, 1024, 3), (33000, 8, 16, 8)])
+def test_order_of_many_picks(cuda_runtime, tokens, topk, experts, hidden, how):
+    """More picks than the ranking cluster's warps hold at a time (65,536): the stable order, each time."""
+    rng = np.random.default_rng(tokens + topk)
+    ids = rng.integers(0, experts, size=(tokens, topk))
+    if how == "one":
+        ids[:] = experts - 1
+    elif how == "some":
+        ids[rng.random(ids.shape) < 0.3] = experts + 5
+    elif how == "runs":  # picks of a warp all alike, those of the next another expert's
+        ids = (np.arange(tokens * topk) // 640 % experts).reshape(tokens, topk)
+    perm, inverse, offsets = _plain_order(ids, experts)
+    x = _normal(110, tokens, hidden, dtype=torch.bfloat16)
+    for _ in range(2):
+        rows, order = cuda_runtime.expert_sort(x, torch.from_numpy(ids.astype(np.int32)).cuda(), experts)
+        np.testing.assert_array_equal(order.perm.cpu().numpy(), perm)
+        np.testing.assert_array_equal(order.inverse.cpu().numpy(), inverse)
+        np.testing.assert_array_equal(order.offsets.cpu().numpy(), offsets)
+        used = int(offsets[-1])
+        assert torch.equal(rows[:used], x[torch.from_numpy(perm[:used] // topk).cuda()]) and not bool(rows[used:].any())
+
+
+def test_row_strides_past_32_bits(cuda_runtime):
+    """Rows so far apart that their places pass 2^32 bytes and 2^31 elements, read and written by every operator."""
+    rt, step = cuda_runtime, 260_000_008
+    far = torch.zeros(11 * step + 256, dtype=torch.bfloat16, device="cuda")
+    assert far.numel() > 2 ** 31
+    packed, scales, divisors = ref.random_matrix(1, 40, 48, 111)
+    m = rt.upload_grouped(packed.cuda(), scales.cuda(), divisors.cuda())
+    ids = torch.tensor([[i % 3] for i in range(12)], dtype=torch.int32, device="cuda")
+    for rows in (7, 12):
+        x, out = far.as_strided((rows, 48), (step, 1)), far.as_strided((rows, 40), (step, 1), 48 + 8)
+        x.copy_(_normal(112, rows, 48, dtype=torch.bfloat16))
+        want, tol = ref.linear(x.contiguous(), packed[0].cuda(), scales[0].cuda(), divisors[0].cuda())
+        for start in (0, 1):  # where TMA can read the rows, and where it cannot
+            y = x if start == 0 else far.as_strided((rows, 48), (step, 1), 1).copy_(x.clone())
+            ref.check(rt.linear_fused(m, y, out=out), want, tol)
+            out.zero_()
+            offsets = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+            ref.check(rt.linear_grouped(m, y, offsets, out=out), want, tol)
+            near, order = rt.expert_sort(y, ids[:rows], 3)
+            assert torch.equal(near, y[order.perm.long()])
+            back = rt.expert_return(y, order, out=far.as_strided((rows, 48), (step, 1), 104))
+            assert torch.equal(back, y[order.inverse[:, 0].long()])
+    m.close()
+
+
+def test_results_past_32_bits(cuda_runtime):
+    """More than 2^31 outputs of one call, the first and the last of them looked at."""
+    rt, rows, vectors = cuda_runtime, 140_000, 15_500
+    packed, scales, divisors = ref.random_matrix(1, rows, 16, 113)
+    m = rt.upload_grouped(packed.cuda(), scales.cuda(), divisors.cuda())
+    x = _normal(114, vectors, 16, dtype=torch.float16)
+    out = rt.linear_fused(m, x)
+    assert out.numel() > 2 ** 31
+    for v in (slice(0, 70), slice(-70, None)):
+        for r in (slice(0, 300), slice(rows - 300, rows)):
+            want, tol = ref.linear(x[v], packed[0, r].cuda(), scales[0, r].cuda(), divisors[0].cuda())
+            ref.check(out[v, r], want, tol)
+    m.close()
