@@ -23,9 +23,10 @@
 //
 // Bound by the weight stream (9/16 byte a weight) and, on B200, nearly as
 // much by the decode (80 weights per cycle and SM with nothing else to do; HBM
-// brings 41). Two batches of loads are in flight per warp, two CTAs on an SM: 81%
-// of the copy bandwidth at 248,320 x 2,048 weights (53.9 us; three batches were no
-// faster, nor were asynchronous copies of the weights into shared memory). K is
+// brings 41). Two batches of loads are in flight per warp, two CTAs on an SM: 78-81%
+// of the copy bandwidth at 248,320 x 2,048 weights (53.9-55.9 us in replayed graphs, as
+// all times here, 61.6 as a call in a row of calls; three batches were no faster, nor
+// were asynchronous copies of the weights into shared memory). K is
 // split over the warps of a CTA when there are too few row tiles to give every
 // warp its own; their sums meet in shared memory in warp order.
 #include "linear_fused.cuh"
@@ -579,7 +580,6 @@ void launch_linear_gemv(const FusedLinearArgs &f, int device, int sm_count, cuda
     // Groups may have more rows than their average: further rows in further passes. (MMA columns for 16 rows made every
     // pass slower: a batch of 32 tokens over 256 groups 91 against 54 us.)
     a.pass_rows = std::max(1, std::min({8 / per_row, staged_rows(f), f.vectors}));
-    a.seg_rows = a.pass_rows;
     // Rows of several groups staged together: 16 of up to 2,048 columns, and of more as many as that much shared memory
     // holds. More of it leaves the L1 too little for the scales, of which a load uses half a sector (with 24 rows 512 rows
     // over 256 groups of 1,024 x 2,048 weights took 70.9 us, with 16 60.1); FP32 gains nothing (66 us, 62.2 a group at a

@@ -1076,7 +1076,8 @@ class Runtime:
     def expert_return(self, rows, order, weights=None, residual=None, out=None, stream=None):
         """additive: out[t] = residual[t] + sum_k weights[t, k] * rows[order.inverse[t, k]]
         ([tokens, hidden], dropped picks left out, FP32 sums; weights None:
-        ones). Differentiable in rows, weights and residual."""
+        ones). Differentiable in rows, weights and residual; picks may be
+        dropped after the sort too (vllm_nvfp4_cuda.experts.ExpertOrder)."""
         return _module("experts").expert_return(self, rows, order, weights, residual, out, stream)
 
     def quantize_rows(self, x, terms: int):
