@@ -386,3 +386,50 @@ def test_results_past_32_bits(cuda_runtime):
             want, tol = ref.linear(x[v], packed[0, r].cuda(), scales[0, r].cuda(), divisors[0].cuda())
             ref.check(out[v, r], want, tol)
     m.close()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_long_rows_over_several_tiles_a_pair(cuda_runtime, kind):
+    """Rows of several segments where every pair of CTAs has several tiles, dense with a residual and over groups of uneven
+    rows: the bits of calls of one tile a pair, which are right to the plain bound."""
+    rt, dtype, cols = cuda_runtime, TYPES[kind], 8208
+    half = torch.finfo(dtype).eps / 2
+    gen = torch.Generator(device="cuda").manual_seed(115)
+
+    def matrix(groups, rows):
+        packed = torch.randint(0, 256, (groups, rows, cols // 2), generator=gen, dtype=torch.uint8, device="cuda")
+        scales = torch.randint(0x28, 0x48, (groups, rows, cols // 16), generator=gen, dtype=torch.uint8, device="cuda")
+        divisors = torch.rand(groups, generator=gen, device="cuda") * 2000 + 3000
+        return rt.upload_grouped(packed, scales, divisors), packed, scales, divisors
+
+    def near(got, x, packed, scales, divisor, residual=None):
+        w = ref.weights(packed, scales)
+        z, size = x.double() @ w.t() / divisor.double(), x.double().abs() @ w.abs().t() / divisor.double()
+        z = z if residual is None else z + residual.double()
+        # A chain's truncations are of its running sum, which is far below the sum of sizes; the divisor's inverse is FP32.
+        ref.check(got, z, half * z.abs() * (1 + half) + 2.0 ** -14 * size + torch.finfo(dtype).tiny)
+
+    rows, vectors = 5000, 900  # 20 pairs of weight tiles, six tiles of rows: 120 items for 74 pairs
+    m, packed, scales, divisors = matrix(1, rows)
+    x, residual = _normal(116, vectors, cols, dtype=dtype), _normal(117, vectors, rows, dtype=dtype)
+    out = rt.linear_fused(m, x, residual=residual)
+    for v in range(0, vectors, 150):
+        part = slice(v, v + 150)
+        assert torch.equal(out[part], rt.linear_fused(m, x[part], residual=residual[part]))
+    near(out[:150, :700], x[:150], packed[0, :700], scales[0, :700], divisors[0], residual[:150, :700])
+    m.close()
+    groups, counts = 8, [0, 1, 300, 0, 161, 17, 160, 500]
+    m, packed, scales, divisors = matrix(groups, 1400)
+    offsets = [0, *np.cumsum(counts).tolist()]
+    x = _normal(118, offsets[-1] + 4, cols, dtype=dtype)
+    out = rt.linear_grouped(m, x, torch.tensor(offsets, dtype=torch.int32, device="cuda"))
+    assert not bool(out[offsets[-1]:].any())
+    for g, count in enumerate(counts):
+        part = slice(offsets[g], offsets[g + 1])
+        one = rt.upload_grouped(packed[g:g + 1], scales[g:g + 1], divisors[g:g + 1])
+        if count > 8:
+            assert torch.equal(out[part], rt.linear_fused(one, x[part]))
+        if count:
+            near(out[part], x[part], packed[g], scales[g], divisors[g])
+        one.close()
+    m.close()
